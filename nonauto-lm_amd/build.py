@@ -13,8 +13,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmivae.so")
 SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
+# packed-fp32-ops off: hipcc -O3 otherwise forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some operand forms
+# of these have been seen to return wrong values now and then.  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
-         "-Wno-unused-result"]
+         "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # The MFMA kernels keep their f32 VALU work single-issue: beside MFMAs a packed v_pk_*_f32 costs more than the two plain
 # instructions it replaces (MI355X_MICROARCH.md, "price of one filler beside MFMAs").
 EXTRA_FLAGS = {"nice_big.hip": ["-fno-slp-vectorize"], "nll.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}

@@ -68,7 +68,7 @@ static __host__ __device__ int64_t stream_items(const BigGeom& g, int st) {
 // q = cubic least-squares fit on [0, 5]; max abs error 1.2e-5 in fp32 arithmetic (the result is rounded to bf16
 // for the second MFMA, 4e-3 relative).  act_pair / act_pair_d / act_pair_fd below evaluate it stage by stage over the
 // eight accumulator registers of a 32-wide hidden chunk (independent chains interleave), the polynomials on whole
-// vectors (v_pk_fma_f32); v_med3_f32 instead of fmin / fmax avoids the canonicalising v_max the IEEE forms cost.
+// vectors; v_med3_f32 instead of fmin / fmax avoids the canonicalising v_max the IEEE forms cost.
 // max(x, 0) as ONE instruction: v_med3_f32 with a finite upper bound (fmaxf and med3 with an infinite bound lower to
 // v_max(x, x) + v_max).  NOT inline asm: hipcc pads no MFMA -> VALU hazard wait states around an asm statement, and an
 // asm v_max reading a fresh MFMA result returned the accumulator without the last product (found the hard way).
@@ -329,7 +329,7 @@ __device__ __forceinline__ void act_pair(int act, f32x4& lo, f32x4& hi) {
     f32x8v x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, a, q;
 #pragma unroll
     for (int r = 0; r < 8; ++r) a[r] = __builtin_amdgcn_fmed3f(fabsf(x[r]), 0.f, 5.0f);
-    q = kGq3 * a + kGq2;          // whole-vector cubic: v_pk_fma_f32 (see act_pair_d)
+    q = kGq3 * a + kGq2;          // whole-vector cubic (see act_pair_d)
     q = q * a + kGq1;
     q = q * a + kGq0;
     q = q * a - 1.0f;
@@ -354,8 +354,7 @@ __device__ __forceinline__ void act_pair_d(int act, const f32x4& lo, const f32x4
     f32x8v x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, a, q, e, d;
 #pragma unroll
     for (int r = 0; r < 8; ++r) a[r] = __builtin_amdgcn_fmed3f(fabsf(x[r]), 0.f, 5.0f);
-    // the two cubics on whole vectors: v_pk_fma_f32, two elements per instruction (this phase runs between the MFMA
-    // phases, where the packed form is a gain; the file is built without SLP vectorisation for the MFMA-paced loops)
+    // the two cubics on whole vectors (scalar instructions: the library is built without packed fp32)
     q = kGq3 * a + kGq2;
     e = kGr3 * a + kGr2;
     q = q * a + kGq1;
@@ -388,8 +387,7 @@ __device__ __forceinline__ void act_pair_fd(int act, f32x4& lo, f32x4& hi, f32x4
     f32x8v x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, a, q, e, d;
 #pragma unroll
     for (int r = 0; r < 8; ++r) a[r] = __builtin_amdgcn_fmed3f(fabsf(x[r]), 0.f, 5.0f);
-    // the two cubics on whole vectors: v_pk_fma_f32, two elements per instruction (this phase runs between the MFMA
-    // phases, where the packed form is a gain; the file is built without SLP vectorisation for the MFMA-paced loops)
+    // the two cubics on whole vectors (scalar instructions: the library is built without packed fp32)
     q = kGq3 * a + kGq2;
     e = kGr3 * a + kGr2;
     q = q * a + kGq1;
@@ -580,7 +578,7 @@ __global__ void __launch_bounds__(512) k_big_chain(BigArgs a) {
           RowIO<T, 4>::load(xh + ft, xp);
         }
         if constexpr (HT <= 4) {
-          // whole-vector arithmetic (v_pk_mul / v_pk_fma: two elements per instruction)
+          // whole-vector arithmetic
           const f32x4 g1 = x1[v] * m;
           const f32x4 t4 = (acc[v] + lds4(b2 + 16 * v)) * 1.44269504088896341f;
           f32x4 e4;
@@ -699,7 +697,7 @@ __global__ void __launch_bounds__(512) k_big_chain(BigArgs a) {
           if (nn == 0) {
             if (a.x1_hist) store_tiles<NF>(a.x1_hist + ((int64_t)k * a.N + tok) * h, valid, h, g, x1);
 #pragma unroll
-            for (int v = 0; v < NF; ++v) {     // whole-vector arithmetic: v_pk_add / v_pk_mul, two elements per instruction
+            for (int v = 0; v < NF; ++v) {     // whole-vector arithmetic
               const f32x4 s4 = acc[v] + lds4(b2 + 16 * v);
               const f32x4 t4 = s4 * 1.44269504088896341f;
               f32x4 e4;
