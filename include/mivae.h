@@ -88,6 +88,70 @@ int mivae_attention_bwd(const void* q, const void* k, const void* v, const int64
                         int64_t S, int64_t heads, int64_t head_size, int64_t q_batch_stride, int64_t q_row_stride,
                         int64_t k_batch_stride, int64_t k_row_stride, int64_t v_batch_stride, int64_t v_row_stride,
                         int64_t grad_row_stride, int causal, float scale, void* stream);
+/* Attention whose scores are capped, biased by distance and limited by masks, documents and a prefix.
+ *   s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);
+ *   slopes: s -= slopes[head] |i - j|;  table: s += table[buckets[clamp(j - i, -distance, distance) + distance]][head];
+ *   out_i = sum_j softmax_j(s) v_j over the keys j that query i sees, 0 where it sees none (and no gradient then).
+ * i = q_start + row is the query's position, j the key's.  A query sees a key if (not causal, or j <= i, or j < prefix[b])
+ * and mask[b][j] != 0 and documents[b][j] == documents[b][i] >= 0; each condition only where its pointer is given.
+ * Keys that mask or a negative document hides may hold anything, NaN included.
+ * Query head h reads key head h / (heads / kv_heads).  Operands float32 or bfloat16 (all of one dtype), element
+ * (b, row, head, c) at base + b stride[0] + row stride[1] + head stride[2] + c, 16-byte aligned; out / dout / dq
+ * (batch, q_len, heads, head_size) and dk / dv (batch, k_len, kv_heads, head_size) contiguous.
+ * head_size a multiple of 8 up to 128, lengths 1 .. 2^24, num_buckets <= 256, distance <= 1024 (bucket values outside
+ * 0 .. num_buckets - 1 are clamped). */
+typedef struct mivae_attention_args {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;                 /* (batch, heads, q_len): written forward (or NULL), read backward */
+  const int64_t* mask;        /* (batch, k_len), or NULL */
+  const int32_t* documents;   /* (batch, k_len), or NULL */
+  const int32_t* prefix;      /* (batch), or NULL; needs causal */
+  const int32_t* q_starts;    /* (batch), or NULL: q_start for every batch row */
+  const float* slopes;        /* (heads), or NULL */
+  const float* table;         /* (num_buckets, heads), or NULL; not together with slopes */
+  const int32_t* buckets;     /* (2 distance + 1) */
+  int32_t* codes;             /* mivae_biased_attention_codes_ints values, 16-byte aligned; with mask or documents: written
+                                 forward, read backward */
+  const void* dout;           /* backward only from here on */
+  void *dq, *dk, *dv;         /* dq may be NULL, dk and dv together */
+  float* dtable;              /* (num_buckets, heads), or NULL */
+  float* scratch;             /* forward: mivae_biased_attention_fwd_floats values; backward: .._bwd_floats */
+  int64_t batch, q_len, k_len, heads, kv_heads, head_size;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t q_start, num_buckets, distance;
+  float scale, softcap;
+  int causal, dtype;
+} mivae_attention_args;
+int64_t mivae_biased_attention_codes_ints(int64_t batch, int64_t q_len, int64_t k_len, int documents);
+int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t heads, int64_t num_buckets);
+int mivae_biased_attention_fwd(const mivae_attention_args* args, void* stream);
+int mivae_biased_attention_bwd(const mivae_attention_args* args, void* stream);
+/* Norm of every query and key head, learned scale and position rotation in one pass.
+ *   norm: n = x / sqrt(mean_d x^2 + eps) * weight (weight (head_size), shared by the heads, NULL: 1), else n = x;
+ *   freq: pair i < rotary_dim / 2 of n turns by 2 pi position freq[i]; pairs are (i, rotary_dim / 2 + i) or, interleaved,
+ *   (2 i, 2 i + 1); what lies beyond rotary_dim stays.  positions element (b, s) at b position_stride[0] + s position_stride[1]
+ *   (NULL: start + s); the angle is reduced to a turn in 64 bits.
+ * q (batch, len, heads, head_size) and k (.., kv_heads, ..) of one dtype, element (b, s, h, c) at b stride[0] + s stride[1] +
+ * h stride[2] + c; q_out / k_out / dq_out / dk_out contiguous.  Backward: q_out / k_out receive dq / dk (q, k may be NULL
+ * without a norm), dq_weight / dk_weight (head_size) may be NULL, scratch holds mivae_qk_norm_rotary_scratch_floats.
+ * head_size even, 2 .. 256.  16-byte accesses where alignment, strides and rotary_dim allow, else element by element. */
+typedef struct mivae_rotary_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float *q_weight, *k_weight;
+  const double* freq;
+  const int64_t* positions;
+  const void *dq_out, *dk_out;
+  float *dq_weight, *dk_weight, *scratch;
+  int64_t batch, len, heads, kv_heads, head_size, rotary_dim;
+  int64_t q_stride[3], k_stride[3], position_stride[2], start;
+  float eps;
+  int norm, interleaved, dtype;
+} mivae_rotary_args;
+int64_t mivae_qk_norm_rotary_scratch_floats(int64_t head_size);
+int mivae_qk_norm_rotary_fwd(const mivae_rotary_args* args, void* stream);
+int mivae_qk_norm_rotary_bwd(const mivae_rotary_args* args, void* stream);
 /* last_idx[b] = sum_s mask[b,s] - 1; ctx[b,:] = out[b, last_idx[b], :] (index -1 wraps like torch).
  * Replaces Encoder.forward's gather, models/base/encoders/encoder.py:35-37.  last_idx may be NULL. */
 int mivae_gather_last(const void* out, const int64_t* mask, void* ctx, int64_t* last_idx, int64_t B,

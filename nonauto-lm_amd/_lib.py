@@ -3,6 +3,7 @@
 No torch types cross the boundary: raw device pointers, sizes and the HIP stream handle only.
 The library is mandatory: there is no CPU or eager-PyTorch fallback for the hot path.
 """
+import contextlib
 import ctypes
 import os
 
@@ -16,6 +17,26 @@ I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
 F64 = ctypes.c_double
+
+
+class AttentionArgs(ctypes.Structure):
+    """mivae_attention_args of include/mivae.h"""
+    _fields_ = ([(n, P) for n in ("q", "k", "v", "out", "lse", "mask", "documents", "prefix", "q_starts", "slopes",
+                                  "table", "buckets", "codes", "dout", "dq", "dk", "dv", "dtable", "scratch")]
+                + [(n, I64) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_size")]
+                + [(n, I64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, I64) for n in ("q_start", "num_buckets", "distance")]
+                + [("scale", F32), ("softcap", F32), ("causal", I32), ("dtype", I32)])
+
+
+class RotaryArgs(ctypes.Structure):
+    """mivae_rotary_args of include/mivae.h"""
+    _fields_ = ([(n, P) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "freq", "positions", "dq_out", "dk_out",
+                                  "dq_weight", "dk_weight", "scratch")]
+                + [(n, I64) for n in ("batch", "len", "heads", "kv_heads", "head_size", "rotary_dim")]
+                + [("q_stride", I64 * 3), ("k_stride", I64 * 3), ("position_stride", I64 * 2), ("start", I64)]
+                + [("eps", F32), ("norm", I32), ("interleaved", I32), ("dtype", I32)])
+
 
 # name -> argument ctypes (every entry returns int status unless listed in _RET)
 SIGNATURES = {
@@ -31,6 +52,13 @@ SIGNATURES = {
     "mivae_attention_fwd": [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, F32, P],
     "mivae_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, F32,
                             P],
+    "mivae_biased_attention_codes_ints": [I64, I64, I64, I32],
+    "mivae_biased_attention_bwd_floats": [I64, I64, I64, I64],
+    "mivae_biased_attention_fwd": [P, P],
+    "mivae_biased_attention_bwd": [P, P],
+    "mivae_qk_norm_rotary_scratch_floats": [I64],
+    "mivae_qk_norm_rotary_fwd": [P, P],
+    "mivae_qk_norm_rotary_bwd": [P, P],
     "mivae_gather_last": [P, P, P, P, I64, I64, I64, I32, P],
     "mivae_reparam_logq_fwd": [P, P, P, P, P, P, I64, I64, I64, I64, I32, P],
     "mivae_reparam_logq_bwd": [P, P, P, P, P, P, P, I64, I64, I64, I64, I32, P],
@@ -143,6 +171,9 @@ SIGNATURES = {
                            F32, P],
 }
 _RET = {
+    "mivae_biased_attention_codes_ints": I64,
+    "mivae_biased_attention_bwd_floats": I64,
+    "mivae_qk_norm_rotary_scratch_floats": I64,
     "mivae_last_error": ctypes.c_char_p,
     "mivae_col_workspace_floats": I64,
     "mivae_colsum_partial": I64,
@@ -201,6 +232,13 @@ def ptr(t):
 
 def stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(device):
+    """Context in which `device` is the current one: launches go to the operands' device, whatever the caller's is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_gpu(*tensors):

@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmivae.so")
-SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
+INCLUDE = os.path.join(os.path.dirname(HERE), "include")
+SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "biased_attention.hip", "qk_rotary.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
 # packed-fp32-ops off: hipcc -O3 otherwise forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some operand forms
 # of these have been seen to return wrong values now and then.  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
@@ -33,13 +34,16 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(LIBDIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")]
+    abi = os.path.join(INCLUDE, "mivae.h")         # included by the sources whose entry points take its structs
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     objs = [os.path.join(LIBDIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
 
     def compile_one(pair):
         src, obj = pair
-        if force or _newer(obj, [src] + headers):
-            cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        with open(src) as f:
+            deps = [src] + headers + ([abi] if '"mivae.h"' in f.read() else [])
+        if force or _newer(obj, deps):
+            cmd = [hipcc] + FLAGS + ["-I", INCLUDE] + EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             subprocess.check_call(cmd)

@@ -1,0 +1,276 @@
+// Tile machinery of the biased attention kernels (biased_attention.hip, token_attention.hip): operand fragments, the staged
+// LDS tiles and the score arithmetic, for bf16 and fp32 operands on the same 32 x 32 accumulator layout.
+//
+// A fragment is 8 consecutive contraction elements per lane, lane = (hh, r32), elements 8 hh .. 8 hh + 7 of a 16-wide
+// slice.  bf16: one v_mfma_f32_32x32x16_bf16.  fp32: eight v_mfma_f32_32x32x2_f32, the j-th taking element j of both
+// half-waves; a contraction does not care which k an instruction handles as long as A and B agree, so both types share
+// every index below.
+#pragma once
+#include "common.hpp"
+
+namespace mivae {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 att_bf16x4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
+
+constexpr int kChunk = 64;                          // rows of the streamed operands staged per pass
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNoCode = -2;                         // query code that equals no key code
+
+// Kernel arguments; the C struct of include/mivae.h after the host's checks.  Strides are in elements (batch, row, head).
+struct BiasedArgs {
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];
+  void* out;                    // (B, Sq, heads, d) contiguous
+  float* lse;                   // (B, heads, Sq): log2-domain log-sum-exp, +inf for a row that sees no key; may be null
+  const void* dout;             // (B, Sq, heads, d) contiguous
+  float* delta;                 // (B, heads, Sq): sum_d dout * out
+  void *dq, *dk, *dv;           // contiguous, may be null
+  float* dtab;                  // bucket partials (heads, B * q blocks, nb), or null
+  // visibility codes, or null: a pair is seen iff the codes are equal.  Keys: document id (0 without documents), -1 where
+  // hidden.  Queries: document id, kNoCode where it is negative.  tiles: {lowest, highest visible code, any hidden, 0} per 64
+  const int *kcodes, *qcodes;
+  const i32x4 *ktiles, *qtiles;
+  const int *prefix, *q_starts;
+  const float* slopes;          // (heads), or null
+  const float* table;           // (nb, heads), or null
+  const int* buckets;           // (2 R + 1)
+  int B, Sq, Sk, heads, kv, group, d, q_start, causal, nb, R, kpad, qpad;
+  float scale, cap;             // cap = 0: no cap
+};
+
+__device__ __forceinline__ int acc_row(int reg) { return (reg & 3) + 8 * (reg >> 2); }    // + 4 hh
+
+template <typename T>
+struct Frag;
+template <>
+struct Frag<unsigned short> { typedef bf16x8 type; };
+template <>
+struct Frag<float> { typedef f32x8 type; };
+
+__device__ __forceinline__ f32x16 mma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// accumulator registers 8 s .. 8 s + 7 as a fragment (rows 16 s + 4 hh + (j & 3) + 8 (j >> 2))
+__device__ __forceinline__ void pack8(bf16x8& f, const f32x16& x, int s) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (bf16_t)x[8 * s + j];
+}
+__device__ __forceinline__ void pack8(f32x8& f, const f32x16& x, int s) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = x[8 * s + j];
+}
+
+__device__ __forceinline__ float to_f32(unsigned short u) { return bf16_to_f32(u); }
+__device__ __forceinline__ float to_f32(float f) { return f; }
+
+// LDS tile of rows of 32 NDB elements.  bf16: row pitch of 4 or 12 (mod 16) 16-byte granules and an XOR of the granule
+// index with bits 2-3 of the row, so that both the 16-byte row reads and the transposing reads are free of bank
+// conflicts; fp32: an odd number of granules per row.
+template <typename T, int NDB>
+struct Tile;
+
+template <int NDB>
+struct Tile<unsigned short, NDB> {
+  static constexpr int W = 32 * NDB;
+  static constexpr int PITCH = (NDB == 1 || NDB == 3) ? W : W + 32;
+  static constexpr int GE = 8, GPR = W / GE;
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ ((r >> 2) & 3)) << 3); }
+  // f[j] = tile[r][16 s + 8 hh + j]
+  static __device__ __forceinline__ bf16x8 row(const unsigned short* t, int r, int s, int hh) {
+    return *reinterpret_cast<const bf16x8*>(t + at(r, 2 * s + hh));
+  }
+  // f[j] = tile[row0 + 4 hh + (j & 3) + 8 (j >> 2)][32 db + r32].  EXEC must be all ones.
+  static __device__ __forceinline__ bf16x8 col(const unsigned short* t, int row0, int db, int lane) {
+    const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
+    const int r0 = row0 + 4 * (g >> 1) + q, r1 = r0 + 8;
+    const int c = 4 * db + 2 * (g & 1) + (p >> 1), e = 4 * (p & 1);
+    typedef __attribute__((address_space(3))) att_bf16x4* lds_ptr;
+    const att_bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr)(t + at(r0, c) + e));
+    const att_bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr)(t + at(r1, c) + e));
+    return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+template <int NDB>
+struct Tile<float, NDB> {
+  static constexpr int W = 32 * NDB;
+  static constexpr int PITCH = W + 4;
+  static constexpr int GE = 4, GPR = W / GE;
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + 4 * c; }
+  static __device__ __forceinline__ f32x8 row(const float* t, int r, int s, int hh) {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(t + at(r, 4 * s + 2 * hh));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(t + at(r, 4 * s + 2 * hh + 1));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ f32x8 col(const float* t, int row0, int db, int lane) {
+    const float* p = t + (row0 + 4 * (lane >> 5)) * PITCH + 32 * db + (lane & 31);
+    f32x8 f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p[((j & 3) + 8 * (j >> 2)) * PITCH];
+    return f;
+  }
+};
+
+// row `row` of a head from global memory as the NS = 2 NDB fragments of an operand; zero where !ok and beyond d
+template <typename T, int NDB>
+__device__ __forceinline__ void load_row(typename Frag<T>::type (&f)[2 * NDB], const T* p, bool ok, int d, int hh) {
+#pragma unroll
+  for (int s = 0; s < 2 * NDB; ++s) {
+    const int c = 16 * s + 8 * hh;
+    constexpr int NV = sizeof(typename Frag<T>::type) / 16;
+    i32x4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      v[i] = i32x4{0, 0, 0, 0};
+      if (ok && c < d) v[i] = reinterpret_cast<const i32x4*>(p + c)[i];
+    }
+    f[s] = __builtin_bit_cast(typename Frag<T>::type, v);
+  }
+}
+
+// kChunk rows of one head on their way global -> registers -> LDS tile, by 64 NW threads.  Rows at or beyond `rows`, rows
+// whose code is negative (hidden keys: whatever they hold must not meet a product, 0 * NaN is NaN) and columns beyond d
+// arrive as zeros.
+template <typename T, int NDB, int NW>
+struct Stage {
+  using L = Tile<T, NDB>;
+  static constexpr int N = kChunk * L::GPR / (64 * NW);
+  static_assert(kChunk * L::GPR % (64 * NW) == 0, "a whole number of granules per thread");
+  i32x4 r[N];
+  __device__ __forceinline__ void load(const T* src, int64_t sr, int row0, int rows, int d, const int* codes) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = threadIdx.x + i * 64 * NW, row = row0 + idx / L::GPR, c = idx % L::GPR;
+      const i32x4 z = {0, 0, 0, 0};
+      r[i] = z;
+      bool ok = row < rows && c * L::GE < d;
+      if (codes != nullptr) ok = ok && codes[row] >= 0;       // codes are padded to whole chunks
+      if (ok) r[i] = *reinterpret_cast<const i32x4*>(src + (int64_t)row * sr + c * L::GE);
+    }
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = threadIdx.x + i * 64 * NW, row = idx / L::GPR, c = idx % L::GPR;
+      *reinterpret_cast<i32x4*>(tile + L::at(row, c)) = r[i];
+    }
+  }
+};
+
+// rows d = 32 db + 8 a + 4 hh .. + 3 of the transposed accumulators -> one row of a contiguous (.., d) tensor
+__device__ __forceinline__ void store4(unsigned short* p, float a, float b, float c, float e) {
+  const u16x4 o = {f32_to_bf16(a), f32_to_bf16(b), f32_to_bf16(c), f32_to_bf16(e)};
+  *reinterpret_cast<u16x4*>(p) = o;
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float e) {
+  const f32x4 o = {a, b, c, e};
+  *reinterpret_cast<f32x4*>(p) = o;
+}
+template <typename T, int NDB>
+__device__ __forceinline__ void store_row(T* dst, const f32x16 (&x)[NDB], float mul, int d, int hh) {
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int a4 = 0; a4 < 4; ++a4) {
+      const int c = 32 * db + 8 * a4 + 4 * hh;
+      if (c < d)
+        store4(dst + c, x[db][4 * a4] * mul, x[db][4 * a4 + 1] * mul, x[db][4 * a4 + 2] * mul, x[db][4 * a4 + 3] * mul);
+    }
+}
+
+// tanh.  bf16 operands: 1 - 2 / (1 + e^2x), absolute error about 1e-7, i.e. cap * 1e-7 in a score; fp32 operands: the
+// library function, whose relative error near 0 is a last-place one too.
+template <typename T>
+__device__ __forceinline__ float cap_tanh(float x) {
+  if (sizeof(T) == 4) return tanhf(x);
+  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x));
+}
+
+// wave-uniform constants of a block's scores
+struct ScoreParams {
+  float c2;         // scale * log2 e, or cap * log2 e
+  float ci;         // scale / cap
+  float slope2;     // slope * log2 e
+  bool cap, slope, tab;
+  int R;
+};
+
+__device__ __forceinline__ ScoreParams score_params(const BiasedArgs& a, int head) {
+  ScoreParams p;
+  p.cap = a.cap > 0.f;
+  p.c2 = (p.cap ? a.cap : a.scale) * kLog2e;
+  p.ci = p.cap ? a.scale / a.cap : 0.f;
+  p.slope = a.slopes != nullptr;
+  p.slope2 = p.slope ? a.slopes[head] * kLog2e : 0.f;
+  p.tab = a.table != nullptr;
+  p.R = a.R;
+  return p;
+}
+
+// Raw products q.k of a tile -> biased scores in base-2 exponent units.  Register r's relative distance key - query is
+// rel + SIGN * acc_row(r) (SIGN = 1: the lane is a query, -1: the lane is a key); [rel_lo, rel_hi] bounds it over the wave.
+// GRAD: tt holds tanh for the cap's derivative.
+template <typename T, int SIGN, bool GRAD>
+__device__ __forceinline__ void score_tile(f32x16& sc, f32x16& tt, const ScoreParams& p, const float* tab, int rel, int rel_lo,
+                                           int rel_hi) {
+  if (p.cap) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float t = cap_tanh<T>(sc[r] * p.ci);
+      if (GRAD) tt[r] = t;
+      sc[r] = t * p.c2;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] *= p.c2;
+  }
+  if (p.slope) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = fmaf(-p.slope2, fabsf((float)(rel + SIGN * acc_row(r))), sc[r]);
+  }
+  if (p.tab) {
+    if (rel_hi <= -p.R || rel_lo >= p.R) {            // wave-uniform: the whole tile is beyond the last distance
+      const float far = tab[rel_hi <= -p.R ? 0 : 2 * p.R];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] += far;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] += tab[min(max(rel + SIGN * acc_row(r), -p.R), p.R) + p.R];
+    }
+  }
+}
+
+// the bias by relative distance of one head, in base-2 exponent units: tab[R + rel], rel = -R .. R
+__device__ __forceinline__ void stage_table(float* tab, const BiasedArgs& a, int head, int nthreads) {
+  for (int i = threadIdx.x; i <= 2 * a.R; i += nthreads) {
+    const int b = min(max(a.buckets[i], 0), a.nb - 1);
+    tab[i] = a.table[(int64_t)b * a.heads + head] * kLog2e;
+  }
+}
+
+__device__ __forceinline__ int clamp_start(int s) { return min(max(s, -(1 << 30)), 1 << 30); }
+
+// Issue order of a run of N products whose A operands take DS LDS reads each: reads two products ahead of the matrix core
+// (the compiler's own order is read, wait, multiply, which exposes the LDS latency N times).
+template <int N, int DS>
+__device__ __forceinline__ void products_pipelined() {
+  if (N > 2) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * DS, 0);
+#pragma unroll
+    for (int i = 0; i < N - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+  }
+}
+
+}  // namespace mivae

@@ -3,12 +3,14 @@
 PyTorch is plumbing here: it owns device memory, the current HIP stream and autograd bookkeeping.
 Every numeric result on this path comes from a hand-written HIP kernel; inputs must live on the GPU.
 """
+import ctypes
 import math
 from typing import Optional, Sequence, Tuple
 
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -258,6 +260,309 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[
         if mask.shape != q.shape[:2]:
             raise ValueError(f"ops.attention: mask {tuple(mask.shape)} does not match (B, S) = {tuple(q.shape[:2])}")
     return _Attention.apply(q, k, v, mask, int(heads), bool(causal))
+
+
+# Attention sublayer operators over head rows: q / k / v as (B, S, heads * d) (the projections' outputs) or (B, S, heads, d)
+# (any strides with unit feature stride, e.g. a transposed (B, heads, S, d) tensor), fp32 or bf16.
+def _head_rows(t: torch.Tensor, heads: int, what: str) -> torch.Tensor:
+    """(B, S, heads, d) view of `t`"""
+    if t.dim() == 4:
+        if t.size(2) != heads:
+            raise ValueError(f"{what}: {tuple(t.shape)} is not (B, S, {heads}, d)")
+        return t
+    if t.dim() != 3 or heads < 1 or t.size(2) % heads:
+        raise ValueError(f"{what}: {tuple(t.shape)} is neither (B, S, heads * d) nor (B, S, heads, d) with {heads} heads")
+    return t.unflatten(2, (heads, t.size(2) // heads))
+
+
+def _addressable(t: torch.Tensor) -> torch.Tensor:
+    """`t` (.., d) itself where its rows are 16-byte aligned with unit feature stride, else a contiguous copy"""
+    per16 = 16 // t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(st % per16 or st < 0 for n, st in zip(t.shape, t.stride()[:-1]) if n > 1):
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    """batch, row and head strides; a dimension of one element has none"""
+    return tuple(0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _same_device(what: str, ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, the operands are on {ref.device}")
+
+
+def _operand_dtype(what: str, *tensors) -> torch.dtype:
+    dt = tensors[0].dtype
+    if dt not in (torch.float32, torch.bfloat16) or any(t.dtype != dt for t in tensors):
+        raise ValueError(f"{what}: operands are float32 or bfloat16, all alike; got {[str(t.dtype) for t in tensors]}")
+    return dt
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """Turns per position of the rotary_dim / 2 pairs, base^(-2 i / rotary_dim) / 2 pi in float64 (what `qk_norm_rotary`
+    takes as `frequencies`; any float64 vector of that length will do)."""
+    if rotary_dim < 2 or rotary_dim % 2 or not base > 0:
+        raise ValueError(f"rotary_frequencies: rotary_dim {rotary_dim} must be even and positive, base {base} positive")
+    return base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim) / (2 * math.pi)
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def _args(q, k, qw, kw, freqs, positions, opt):
+        heads, kv, start, eps, norm, interleaved = opt
+        B, S, _, d = q.shape
+        pos = (0, 0) if positions is None else tuple(0 if n == 1 else st for n, st in zip(positions.shape, positions.stride()))
+        return L.RotaryArgs(
+            q=L.ptr(q), k=L.ptr(k), q_weight=L.ptr(qw), k_weight=L.ptr(kw), freq=L.ptr(freqs), positions=L.ptr(positions),
+            batch=B, len=S, heads=heads, kv_heads=kv, head_size=d, rotary_dim=0 if freqs is None else 2 * freqs.numel(),
+            q_stride=_strides(q), k_stride=_strides(k), position_stride=pos, start=start, eps=eps, norm=int(norm),
+            interleaved=int(interleaved), dtype=L.dtype_code(q.dtype))
+
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, freqs, positions, opt):
+        heads, kv = opt[:2]
+        q4, k4 = _addressable(_head_rows(q, heads, "q")), _addressable(_head_rows(k, kv, "k"))
+        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q4, k4))
+        if q4.numel():
+            a = _QkNormRotary._args(q4, k4, qw, kw, freqs, positions, opt)
+            a.q_out, a.k_out = L.ptr(yq), L.ptr(yk)
+            with L.on_device(q.device):
+                L.call("mivae_qk_norm_rotary_fwd", ctypes.byref(a), L.stream())
+        norm = opt[4]                   # a rotation alone needs no operands in its backward
+        ctx.save_for_backward(q4 if norm else None, k4 if norm else None, qw, kw, freqs, positions)
+        ctx.opt, ctx.shapes, ctx.meta = opt, (q.shape, k.shape), (q4.shape, k4.shape, q.dtype, q.device)
+        return yq.view(q.shape), yk.view(k.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dyq, dyk):
+        q4, k4, qw, kw, freqs, positions = ctx.saved_tensors
+        qs, ks, dtype, device = ctx.meta
+        dyq, dyk = _addressable(dyq.contiguous()), _addressable(dyk.contiguous())
+        dq, dk = torch.empty(qs, dtype=dtype, device=device), torch.empty(ks, dtype=dtype, device=device)
+        need_qw, need_kw = ctx.needs_input_grad[2:4]
+        dqw = torch.zeros_like(qw) if need_qw else None
+        dkw = torch.zeros_like(kw) if need_kw else None
+        if dq.numel():
+            a = _QkNormRotary._args(q4 if q4 is not None else dq, k4 if k4 is not None else dk, qw, kw, freqs, positions, ctx.opt)
+            scratch = None
+            if need_qw or need_kw:
+                scratch = torch.empty(L.query("mivae_qk_norm_rotary_scratch_floats", qs[3]), dtype=torch.float32, device=device)
+            a.dq_out, a.dk_out, a.q_out, a.k_out = L.ptr(dyq), L.ptr(dyk), L.ptr(dq), L.ptr(dk)
+            a.dq_weight, a.dk_weight, a.scratch = L.ptr(dqw), L.ptr(dkw), L.ptr(scratch)
+            with L.on_device(device):
+                L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(a), L.stream())
+        return dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dqw, dkw, None, None, None
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optional[int] = None, *,
+                   q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   frequencies: Optional[torch.Tensor] = None, positions=None, norm: bool = True,
+                   interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Queries and keys on their way into the attention, in one pass: every head row n = x / sqrt(mean(x^2) + eps) * weight
+    (`norm`; weights (d) fp32 shared by the heads, None: 1), then the position rotation of its first 2 * len(frequencies)
+    elements by 2 pi position * frequencies[i] (frequencies: float64 turns per position, see `rotary_frequencies`; None: no
+    rotation).  Pairs are (i, rotary_dim / 2 + i), or (2 i, 2 i + 1) with `interleaved`.
+
+    q (B, S, heads * d) or (B, S, heads, d), k with kv_heads (default: heads), fp32 or bf16, d even, 2 .. 256.  positions:
+    int64 (S,), (B, S) or (1, S), an int (position of the first token) or None (0).  The angle is reduced in 64 bits: far
+    positions lose nothing.  Outputs have the inputs' shapes, contiguous; gradients flow to q, k and the weights."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    L.require_gpu(q, k, q_weight, k_weight, frequencies)
+    _operand_dtype("qk_norm_rotary", q, k)
+    q4, k4 = _head_rows(q, heads, "qk_norm_rotary: q"), _head_rows(k, kv_heads, "qk_norm_rotary: k")
+    B, S, _, d = q4.shape
+    if k4.shape[:2] != q4.shape[:2] or k4.size(3) != d:
+        raise ValueError(f"qk_norm_rotary: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    if d % 2 or not 2 <= d <= 256:
+        raise ValueError(f"qk_norm_rotary: head size {d} is not an even number in 2 .. 256")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (not norm or w.shape != (d,) or w.dtype != torch.float32):
+            raise ValueError(f"qk_norm_rotary: {name} must be float32 ({d},), and needs the norm")
+    if frequencies is None and not norm:
+        raise ValueError("qk_norm_rotary: neither a norm nor a rotation")
+    if frequencies is not None:
+        if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not 1 <= frequencies.numel() <= d // 2:
+            raise ValueError(f"qk_norm_rotary: frequencies must be float64 with 1 .. {d // 2} values")
+        if frequencies.requires_grad:
+            raise ValueError("qk_norm_rotary: frequencies have no gradient")
+    if not (norm is False or 0 <= eps < math.inf):
+        raise ValueError(f"qk_norm_rotary: eps {eps}")
+    start = 0
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype != torch.int64 or positions.shape not in ((S,), (1, S), (B, S)):
+            raise ValueError(f"qk_norm_rotary: positions must be int64 (S,), (1, S) or (B, S), got {positions.dtype} {tuple(positions.shape)}")
+        L.require_gpu(positions)
+        positions = positions.expand(B, S)
+    elif positions is not None:
+        start, positions = int(positions), None
+    _same_device("qk_norm_rotary", q, k=k, q_weight=q_weight, k_weight=k_weight, frequencies=frequencies, positions=positions)
+    cont = lambda t: None if t is None else t.contiguous()
+    return _QkNormRotary.apply(q, k, cont(q_weight), cont(k_weight), cont(frequencies), positions,
+                               (int(heads), int(kv_heads), start, float(eps), bool(norm), bool(interleaved)))
+
+
+def relative_buckets(num_buckets: int = 32, max_distance: int = 128, both_sides: bool = True, device=None) -> torch.Tensor:
+    """Bucket of every relative distance key - query in -max_distance .. max_distance, int32 (2 max_distance + 1,): the near
+    half of the buckets hold one distance each, the far half widths that grow geometrically up to max_distance, whose
+    bucket also takes everything beyond.  both_sides: keys before and behind the query have half of the buckets each;
+    otherwise (causal attention) keys behind the query share bucket 0.  Any int32 vector of odd length can take its place."""
+    n = num_buckets // 2 if both_sides else num_buckets
+    near = n // 2
+    if near < 1 or (both_sides and num_buckets % 2) or max_distance <= near:
+        raise ValueError(f"relative_buckets: {num_buckets} buckets up to distance {max_distance}")
+    rel = torch.arange(-max_distance, max_distance + 1, dtype=torch.float64)
+    away = rel.abs() if both_sides else (-rel).clamp(min=0)
+    far = near + (away.clamp(min=near) / near).log() / math.log(max_distance / near) * (n - near)
+    b = torch.where(away < near, away, far.floor().clamp(max=n - 1))
+    if both_sides:
+        b = b + torch.where(rel > 0, float(n), 0.0)
+    return b.to(torch.int32).to(device)
+
+
+class _BiasedAttention(torch.autograd.Function):
+    @staticmethod
+    def _args(q, k, v, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, opt):
+        q_start, softcap, scale, causal = opt
+        B, Sq, H, d = q.shape
+        return L.AttentionArgs(
+            q=L.ptr(q), k=L.ptr(k), v=L.ptr(v), out=L.ptr(out), lse=L.ptr(lse), mask=L.ptr(mask), documents=L.ptr(documents),
+            prefix=L.ptr(prefix), q_starts=L.ptr(q_starts), slopes=L.ptr(slopes), table=L.ptr(table), buckets=L.ptr(buckets),
+            codes=L.ptr(codes), batch=B, q_len=Sq, k_len=k.size(1), heads=H, kv_heads=k.size(2), head_size=d,
+            q_stride=_strides(q), k_stride=_strides(k), v_stride=_strides(v), q_start=q_start,
+            num_buckets=0 if table is None else table.size(0), distance=0 if table is None else buckets.numel() // 2,
+            scale=scale, softcap=softcap, causal=int(causal), dtype=L.dtype_code(q.dtype))
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, heads, kv, opt):
+        q4, k4, v4 = (_addressable(_head_rows(t, h, "operand")) for t, h in ((q, heads), (k, kv), (v, kv)))
+        B, Sq, H, d = q4.shape
+        need = any(ctx.needs_input_grad[:4])
+        dev = q.device
+        out = torch.empty(B, Sq, H, d, dtype=q.dtype, device=dev)
+        lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev) if need else None
+        codes = None
+        if mask is not None or documents is not None:
+            n = L.query("mivae_biased_attention_codes_ints", B, Sq, k4.size(1), int(documents is not None))
+            codes = torch.empty(n, dtype=torch.int32, device=dev)
+        a = _BiasedAttention._args(q4, k4, v4, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, opt)
+        with L.on_device(dev), _timed("biased_attention_fwd"):
+            L.call("mivae_biased_attention_fwd", ctypes.byref(a), L.stream())
+        if need:
+            ctx.save_for_backward(q4, k4, v4, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse)
+            ctx.opt, ctx.shapes = opt, (q.shape, k.shape, v.shape)
+        return out.view(q.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q4, k4, v4, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse = ctx.saved_tensors
+        B, Sq, H, d = q4.shape
+        dev = q4.device
+        dout = _addressable(dout.contiguous())
+        need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
+        dq = torch.empty_like(out) if need_q else None
+        dk = dv = None
+        if need_k or need_v:
+            dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (k4, v4))
+        dtable = torch.empty_like(table) if need_t else None
+        scratch = torch.empty(L.query("mivae_biased_attention_bwd_floats", B, Sq, H, table.size(0) if need_t else 0),
+                              dtype=torch.float32, device=dev)
+        a = _BiasedAttention._args(q4, k4, v4, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, ctx.opt)
+        a.dout, a.dq, a.dk, a.dv = L.ptr(dout), L.ptr(dq), L.ptr(dk), L.ptr(dv)
+        a.dtable, a.scratch = L.ptr(dtable), L.ptr(scratch)
+        with L.on_device(dev), _timed("biased_attention_bwd"):
+            L.call("mivae_biased_attention_bwd", ctypes.byref(a), L.stream())
+        qs, ks, vs = ctx.shapes
+        return (dq.view(qs) if need_q else None, dk.view(ks) if need_k else None, dv.view(vs) if need_v else None, dtable,
+                *([None] * 9))
+
+
+ATTENTION_MAX_LEN = 1 << 24
+
+
+def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: Optional[int] = None, *,
+                     mask: Optional[torch.Tensor] = None, causal: bool = False, prefix: Optional[torch.Tensor] = None,
+                     documents: Optional[torch.Tensor] = None, q_start=None, softcap: Optional[float] = None,
+                     slopes: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                     buckets: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(bias(cap(scale q k^T))) v per head, over the keys each query sees; forward and backward on libmivae's kernels.
+
+    q (B, Sq, heads * d) or (B, Sq, heads, d); k, v (B, Sk, kv_heads * d) or 4-D, query head h reading key head
+    h // (heads / kv_heads); fp32 or bf16; d a multiple of 8 up to 128; any lengths (Sq = 1: one new token over a cache).
+    Row i of q stands at position q_start + i of the keys: an int, an int32 (B,) tensor (sequences of unequal length), or
+    None for the last Sq positions.
+
+    scores   softcap * tanh(scale q.k / softcap) (softcap None: scale q.k; scale None: 1 / sqrt(d)), then
+             - slopes[head] * |distance| (fp32 (heads,), no gradient), or
+             + table[buckets[clamp(key - query, -R, R) + R], head] (fp32 (num_buckets, heads), learned; buckets int32
+               (2 R + 1,), see `relative_buckets`; num_buckets <= 256, R <= 1024)
+    seen     key <= query with `causal`, or key < prefix[b] (int32 (B,), needs causal); mask (B, Sk) != 0; documents
+             (int32 (B, Sk)) equal and not negative, the query's taken at its position.
+
+    A query that sees no key gives zeros and has no gradient (`ops.attention` averages such a row instead).  Keys that the
+    mask or a negative document hides may hold anything; all others have to be finite, also where `causal` or documents
+    hide them from some queries."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
+    _operand_dtype("biased_attention", q, k, v)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"biased_attention: {heads} heads over {kv_heads} key heads")
+    q4, k4 = _head_rows(q, heads, "biased_attention: q"), _head_rows(k, kv_heads, "biased_attention: k")
+    v4 = _head_rows(v, kv_heads, "biased_attention: v")
+    B, Sq, _, d = q4.shape
+    Sk = k4.size(1)
+    if k4.shape != v4.shape or k4.size(0) != B or k4.size(3) != d:
+        raise ValueError(f"biased_attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if d % 8 or not 8 <= d <= 128:
+        raise ValueError(f"biased_attention: head size {d} is not a multiple of 8 in 8 .. 128")
+    if B < 1 or not (1 <= Sq <= ATTENTION_MAX_LEN and 1 <= Sk <= ATTENTION_MAX_LEN):
+        raise ValueError(f"biased_attention: batch {B}, lengths {Sq} and {Sk}")
+    if mask is not None:
+        if mask.shape != (B, Sk):
+            raise ValueError(f"biased_attention: mask {tuple(mask.shape)} does not match (B, Sk) = {(B, Sk)}")
+        mask = _mask_i64(mask)
+    for name, t, shape, dtype in (("prefix", prefix, (B,), torch.int32), ("documents", documents, (B, Sk), torch.int32),
+                                  ("slopes", slopes, (heads,), torch.float32)):
+        if t is not None and (t.shape != shape or t.dtype != dtype):
+            raise ValueError(f"biased_attention: {name} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    if prefix is not None and not causal:
+        raise ValueError("biased_attention: a prefix needs causal=True")
+    if slopes is not None and slopes.requires_grad:
+        raise ValueError("biased_attention: slopes have no gradient")
+    if (table is None) != (buckets is None) or (table is not None and slopes is not None):
+        raise ValueError("biased_attention: table and buckets come together, and not with slopes")
+    if table is not None:
+        if table.dim() != 2 or table.dtype != torch.float32 or table.size(1) != heads or not 1 <= table.size(0) <= 256:
+            raise ValueError(f"biased_attention: table must be float32 (1 .. 256, {heads}), got {table.dtype} {tuple(table.shape)}")
+        if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or not 3 <= buckets.numel() <= 2049:
+            raise ValueError("biased_attention: buckets must be int32 of odd length 3 .. 2049")
+    if softcap is not None and not 0 < softcap < 1e30:
+        raise ValueError(f"biased_attention: softcap {softcap}")
+    q_starts = None
+    if isinstance(q_start, torch.Tensor):
+        if q_start.shape != (B,) or q_start.dtype != torch.int32:
+            raise ValueError(f"biased_attention: q_start must be an int or int32 ({B},)")
+        L.require_gpu(q_start)
+        q_starts, q_start = q_start.contiguous(), 0
+    else:
+        q_start = Sk - Sq if q_start is None else int(q_start)
+        if not 0 <= q_start <= ATTENTION_MAX_LEN:
+            raise ValueError(f"biased_attention: queries start at position {q_start}")
+        if documents is not None and q_start + Sq > Sk:
+            raise ValueError(f"biased_attention: documents reach {Sk} positions, the queries {q_start + Sq}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not abs(scale) < 1e30:
+        raise ValueError(f"biased_attention: scale {scale}")
+    _same_device("biased_attention", q, k=k, v=v, mask=mask, prefix=prefix, documents=documents, q_start=q_starts,
+                 slopes=slopes, table=table, buckets=buckets)
+    cont = lambda t: None if t is None else t.contiguous()
+    return _BiasedAttention.apply(q, k, v, cont(table), mask, cont(documents), cont(prefix), q_starts, cont(slopes),
+                                  cont(buckets), int(heads), int(kv_heads),
+                                  (q_start, float(softcap or 0.0), scale, bool(causal)))
 
 
 def segment_sum(tok: torch.Tensor, nseg: int, S: int, add: Optional[torch.Tensor] = None) -> torch.Tensor:
