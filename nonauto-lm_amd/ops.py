@@ -4,6 +4,7 @@ PyTorch is plumbing here: it owns device memory, the current HIP stream and auto
 Every numeric result on this path comes from a hand-written HIP kernel; inputs must live on the GPU.
 """
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -264,28 +265,31 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[
 
 # Attention sublayer operators over head rows: q / k / v as (B, S, heads * d) (the projections' outputs) or (B, S, heads, d)
 # (any strides with unit feature stride, e.g. a transposed (B, heads, S, d) tensor), fp32 or bf16.
-def _head_rows(t: torch.Tensor, heads: int, what: str) -> torch.Tensor:
-    """(B, S, heads, d) view of `t`"""
-    if t.dim() == 4:
-        if t.size(2) != heads:
-            raise ValueError(f"{what}: {tuple(t.shape)} is not (B, S, {heads}, d)")
-        return t
-    if t.dim() != 3 or heads < 1 or t.size(2) % heads:
-        raise ValueError(f"{what}: {tuple(t.shape)} is neither (B, S, heads * d) nor (B, S, heads, d) with {heads} heads")
-    return t.unflatten(2, (heads, t.size(2) // heads))
-
-
-def _addressable(t: torch.Tensor) -> torch.Tensor:
-    """`t` (.., d) itself where its rows are 16-byte aligned with unit feature stride, else a contiguous copy"""
+def _head_rows(t: torch.Tensor, heads: int, what: str):
+    """`t` and its geometry: (tensor, B, S, d, (batch, row, head) strides).  Where the kernels cannot address `t` itself
+    (features not adjacent, rows not 16-byte aligned) the tensor is a contiguous copy."""
+    shape, st = t.shape, t.stride()
+    if len(shape) == 4 and shape[2] == heads:
+        B, S, _, d = shape
+        sb, ss, sh, sf = st
+    elif len(shape) == 3 and heads >= 1 and shape[2] % heads == 0:
+        B, S, d = shape[0], shape[1], shape[2] // heads
+        sb, ss, sf = st
+        sh = d * sf
+    else:
+        raise ValueError(f"{what}: {tuple(shape)} is neither (B, S, heads * d) nor (B, S, heads, d) with {heads} heads")
+    sb, ss, sh = (0 if B == 1 else sb), (0 if S == 1 else ss), (0 if heads == 1 else sh)      # one element: no stride
     per16 = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(st % per16 or st < 0 for n, st in zip(t.shape, t.stride()[:-1]) if n > 1):
-        t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    if (sf != 1 and d > 1) or sb % per16 or ss % per16 or sh % per16 or t.data_ptr() % 16:
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+        sb, ss, sh = S * heads * d, heads * d, d
+    return t, B, S, d, (sb, ss, sh)
 
 
-def _strides(t: torch.Tensor):
-    """batch, row and head strides; a dimension of one element has none"""
-    return tuple(0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()[:3]))
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """contiguous, 16-byte aligned"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _same_device(what: str, ref: torch.Tensor, **tensors) -> None:
@@ -309,53 +313,63 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> t
     return base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim) / (2 * math.pi)
 
 
+@functools.lru_cache(maxsize=1024)
+def _buffer_size(name: str, *args) -> int:
+    """size queries of the library, functions of their integer arguments alone"""
+    return L.query(name, *args)
+
+
+def _refill(args, **tensors):
+    """A copy of a filled argument struct whose pointers are those of `tensors` (saved tensors may have moved)"""
+    args = type(args).from_buffer_copy(args)
+    for name, t in tensors.items():
+        if t is not None:
+            setattr(args, name, t.data_ptr())
+    return args
+
+
+def _learns(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _qk_norm_rotary_fwd(q, k, args):
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    if q.numel():
+        args.q_out, args.k_out = yq.data_ptr(), yk.data_ptr()
+        with L.on_device(q.device):
+            L.call("mivae_qk_norm_rotary_fwd", ctypes.byref(args), L.stream())
+    return yq, yk
+
+
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def _args(q, k, qw, kw, freqs, positions, opt):
-        heads, kv, start, eps, norm, interleaved = opt
-        B, S, _, d = q.shape
-        pos = (0, 0) if positions is None else tuple(0 if n == 1 else st for n, st in zip(positions.shape, positions.stride()))
-        return L.RotaryArgs(
-            q=L.ptr(q), k=L.ptr(k), q_weight=L.ptr(qw), k_weight=L.ptr(kw), freq=L.ptr(freqs), positions=L.ptr(positions),
-            batch=B, len=S, heads=heads, kv_heads=kv, head_size=d, rotary_dim=0 if freqs is None else 2 * freqs.numel(),
-            q_stride=_strides(q), k_stride=_strides(k), position_stride=pos, start=start, eps=eps, norm=int(norm),
-            interleaved=int(interleaved), dtype=L.dtype_code(q.dtype))
-
-    @staticmethod
-    def forward(ctx, q, k, qw, kw, freqs, positions, opt):
-        heads, kv = opt[:2]
-        q4, k4 = _addressable(_head_rows(q, heads, "q")), _addressable(_head_rows(k, kv, "k"))
-        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q4, k4))
-        if q4.numel():
-            a = _QkNormRotary._args(q4, k4, qw, kw, freqs, positions, opt)
-            a.q_out, a.k_out = L.ptr(yq), L.ptr(yk)
-            with L.on_device(q.device):
-                L.call("mivae_qk_norm_rotary_fwd", ctypes.byref(a), L.stream())
-        norm = opt[4]                   # a rotation alone needs no operands in its backward
-        ctx.save_for_backward(q4 if norm else None, k4 if norm else None, qw, kw, freqs, positions)
-        ctx.opt, ctx.shapes, ctx.meta = opt, (q.shape, k.shape), (q4.shape, k4.shape, q.dtype, q.device)
-        return yq.view(q.shape), yk.view(k.shape)
+    def forward(ctx, q, k, qw, kw, freqs, positions, args):
+        yq, yk = _qk_norm_rotary_fwd(q, k, args)
+        ctx.save_for_backward(*((q, k) if args.norm else (None, None)), qw, kw, freqs, positions)
+        ctx.args, ctx.meta = args, (q.shape, k.shape, q.dtype, q.device)      # a rotation alone needs no operands in its backward
+        return yq, yk
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
-        q4, k4, qw, kw, freqs, positions = ctx.saved_tensors
-        qs, ks, dtype, device = ctx.meta
-        dyq, dyk = _addressable(dyq.contiguous()), _addressable(dyk.contiguous())
-        dq, dk = torch.empty(qs, dtype=dtype, device=device), torch.empty(ks, dtype=dtype, device=device)
+        q, k, qw, kw, freqs, positions = ctx.saved_tensors
+        qs, ks, dtype, dev = ctx.meta
+        dyq, dyk = _aligned(dyq), _aligned(dyk)
+        dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
         need_qw, need_kw = ctx.needs_input_grad[2:4]
-        dqw = torch.zeros_like(qw) if need_qw else None
-        dkw = torch.zeros_like(kw) if need_kw else None
+        make = torch.empty_like if dq.numel() else torch.zeros_like
+        dqw, dkw = make(qw) if need_qw else None, make(kw) if need_kw else None
         if dq.numel():
-            a = _QkNormRotary._args(q4 if q4 is not None else dq, k4 if k4 is not None else dk, qw, kw, freqs, positions, ctx.opt)
             scratch = None
             if need_qw or need_kw:
-                scratch = torch.empty(L.query("mivae_qk_norm_rotary_scratch_floats", qs[3]), dtype=torch.float32, device=device)
-            a.dq_out, a.dk_out, a.q_out, a.k_out = L.ptr(dyq), L.ptr(dyk), L.ptr(dq), L.ptr(dk)
-            a.dq_weight, a.dk_weight, a.scratch = L.ptr(dqw), L.ptr(dkw), L.ptr(scratch)
-            with L.on_device(device):
-                L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(a), L.stream())
-        return dq.view(ctx.shapes[0]), dk.view(ctx.shapes[1]), dqw, dkw, None, None, None
+                scratch = torch.empty(_buffer_size("mivae_qk_norm_rotary_scratch_floats", ctx.args.head_size),
+                                      dtype=torch.float32, device=dev)
+            args = _refill(ctx.args, q=q, k=k, q_weight=qw, k_weight=kw, freq=freqs, positions=positions, dq_out=dyq,
+                           dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw, scratch=scratch)
+            with L.on_device(dev):
+                L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream())
+        return dq, dk, dqw, dkw, None, None, None
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optional[int] = None, *,
@@ -373,9 +387,11 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optio
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, q_weight, k_weight, frequencies)
     _operand_dtype("qk_norm_rotary", q, k)
-    q4, k4 = _head_rows(q, heads, "qk_norm_rotary: q"), _head_rows(k, kv_heads, "qk_norm_rotary: k")
-    B, S, _, d = q4.shape
-    if k4.shape[:2] != q4.shape[:2] or k4.size(3) != d:
+    if heads < 1 or kv_heads < 1:
+        raise ValueError(f"qk_norm_rotary: {heads} and {kv_heads} heads")
+    q, B, S, d, qst = _head_rows(q, heads, "qk_norm_rotary: q")
+    k, Bk, Sk, dk, kst = _head_rows(k, kv_heads, "qk_norm_rotary: k")
+    if (Bk, Sk, dk) != (B, S, d):
         raise ValueError(f"qk_norm_rotary: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
     if d % 2 or not 2 <= d <= 256:
         raise ValueError(f"qk_norm_rotary: head size {d} is not an even number in 2 .. 256")
@@ -391,18 +407,24 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optio
             raise ValueError("qk_norm_rotary: frequencies have no gradient")
     if not (norm is False or 0 <= eps < math.inf):
         raise ValueError(f"qk_norm_rotary: eps {eps}")
-    start = 0
+    args = L.RotaryArgs(batch=B, len=S, heads=heads, kv_heads=kv_heads, head_size=d, q_stride=qst, k_stride=kst, eps=eps,
+                        norm=int(norm), interleaved=int(interleaved), dtype=L.dtype_code(q.dtype))
     if isinstance(positions, torch.Tensor):
         if positions.dtype != torch.int64 or positions.shape not in ((S,), (1, S), (B, S)):
             raise ValueError(f"qk_norm_rotary: positions must be int64 (S,), (1, S) or (B, S), got {positions.dtype} {tuple(positions.shape)}")
         L.require_gpu(positions)
-        positions = positions.expand(B, S)
+        st = positions.stride()
+        args.position_stride = (st[0] if positions.shape == (B, S) and B > 1 else 0, st[-1])
     elif positions is not None:
-        start, positions = int(positions), None
+        args.start, positions = int(positions), None
     _same_device("qk_norm_rotary", q, k=k, q_weight=q_weight, k_weight=k_weight, frequencies=frequencies, positions=positions)
-    cont = lambda t: None if t is None else t.contiguous()
-    return _QkNormRotary.apply(q, k, cont(q_weight), cont(k_weight), cont(frequencies), positions,
-                               (int(heads), int(kv_heads), start, float(eps), bool(norm), bool(interleaved)))
+    q_weight, k_weight, frequencies = (None if t is None else t.contiguous() for t in (q_weight, k_weight, frequencies))
+    args.q, args.k, args.q_weight, args.k_weight = L.ptr(q), L.ptr(k), L.ptr(q_weight), L.ptr(k_weight)
+    args.freq, args.positions = L.ptr(frequencies), L.ptr(positions)
+    args.rotary_dim = 0 if frequencies is None else 2 * frequencies.numel()
+    if not _learns(q, k, q_weight, k_weight):
+        return _qk_norm_rotary_fwd(q, k, args)
+    return _QkNormRotary.apply(q, k, q_weight, k_weight, frequencies, positions, args)
 
 
 def relative_buckets(num_buckets: int = 32, max_distance: int = 128, both_sides: bool = True, device=None) -> torch.Tensor:
@@ -423,62 +445,48 @@ def relative_buckets(num_buckets: int = 32, max_distance: int = 128, both_sides:
     return b.to(torch.int32).to(device)
 
 
+def _biased_attention_fwd(q, mask, documents, args, need_lse: bool):
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(args.batch, args.heads, args.q_len, dtype=torch.float32, device=dev) if need_lse else None
+    codes = None
+    if mask is not None or documents is not None:
+        codes = torch.empty(_buffer_size("mivae_biased_attention_codes_ints", args.batch, args.q_len, args.k_len,
+                                         int(documents is not None)), dtype=torch.int32, device=dev)
+    args.out, args.lse, args.codes = out.data_ptr(), L.ptr(lse), L.ptr(codes)
+    with L.on_device(dev), _timed("biased_attention_fwd"):
+        L.call("mivae_biased_attention_fwd", ctypes.byref(args), L.stream())
+    return out, lse, codes
+
+
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
-    def _args(q, k, v, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, opt):
-        q_start, softcap, scale, causal = opt
-        B, Sq, H, d = q.shape
-        return L.AttentionArgs(
-            q=L.ptr(q), k=L.ptr(k), v=L.ptr(v), out=L.ptr(out), lse=L.ptr(lse), mask=L.ptr(mask), documents=L.ptr(documents),
-            prefix=L.ptr(prefix), q_starts=L.ptr(q_starts), slopes=L.ptr(slopes), table=L.ptr(table), buckets=L.ptr(buckets),
-            codes=L.ptr(codes), batch=B, q_len=Sq, k_len=k.size(1), heads=H, kv_heads=k.size(2), head_size=d,
-            q_stride=_strides(q), k_stride=_strides(k), v_stride=_strides(v), q_start=q_start,
-            num_buckets=0 if table is None else table.size(0), distance=0 if table is None else buckets.numel() // 2,
-            scale=scale, softcap=softcap, causal=int(causal), dtype=L.dtype_code(q.dtype))
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, heads, kv, opt):
-        q4, k4, v4 = (_addressable(_head_rows(t, h, "operand")) for t, h in ((q, heads), (k, kv), (v, kv)))
-        B, Sq, H, d = q4.shape
-        need = any(ctx.needs_input_grad[:4])
-        dev = q.device
-        out = torch.empty(B, Sq, H, d, dtype=q.dtype, device=dev)
-        lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev) if need else None
-        codes = None
-        if mask is not None or documents is not None:
-            n = L.query("mivae_biased_attention_codes_ints", B, Sq, k4.size(1), int(documents is not None))
-            codes = torch.empty(n, dtype=torch.int32, device=dev)
-        a = _BiasedAttention._args(q4, k4, v4, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, opt)
-        with L.on_device(dev), _timed("biased_attention_fwd"):
-            L.call("mivae_biased_attention_fwd", ctypes.byref(a), L.stream())
-        if need:
-            ctx.save_for_backward(q4, k4, v4, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse)
-            ctx.opt, ctx.shapes = opt, (q.shape, k.shape, v.shape)
-        return out.view(q.shape)
+    def forward(ctx, q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, args):
+        out, lse, codes = _biased_attention_fwd(q, mask, documents, args, True)
+        ctx.save_for_backward(q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse)
+        ctx.args = args
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q4, k4, v4, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse = ctx.saved_tensors
-        B, Sq, H, d = q4.shape
-        dev = q4.device
-        dout = _addressable(dout.contiguous())
+        q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse = ctx.saved_tensors
+        dev, a = q.device, ctx.args
+        dout = _aligned(dout)
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
-        dq = torch.empty_like(out) if need_q else None
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
         dk = dv = None
         if need_k or need_v:
-            dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (k4, v4))
+            dk, dv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(v.shape, dtype=q.dtype, device=dev)
         dtable = torch.empty_like(table) if need_t else None
-        scratch = torch.empty(L.query("mivae_biased_attention_bwd_floats", B, Sq, H, table.size(0) if need_t else 0),
-                              dtype=torch.float32, device=dev)
-        a = _BiasedAttention._args(q4, k4, v4, out, lse, mask, documents, prefix, q_starts, slopes, table, buckets, codes, ctx.opt)
-        a.dout, a.dq, a.dk, a.dv = L.ptr(dout), L.ptr(dq), L.ptr(dk), L.ptr(dv)
-        a.dtable, a.scratch = L.ptr(dtable), L.ptr(scratch)
+        scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.heads,
+                                           a.num_buckets if need_t else 0), dtype=torch.float32, device=dev)
+        args = _refill(a, q=q, k=k, v=v, table=table, mask=mask, documents=documents, prefix=prefix, q_starts=q_starts,
+                       slopes=slopes, buckets=buckets, codes=codes, out=out, lse=lse, dout=dout, dq=dq, dk=dk, dv=dv,
+                       dtable=dtable, scratch=scratch)
         with L.on_device(dev), _timed("biased_attention_bwd"):
-            L.call("mivae_biased_attention_bwd", ctypes.byref(a), L.stream())
-        qs, ks, vs = ctx.shapes
-        return (dq.view(qs) if need_q else None, dk.view(ks) if need_k else None, dv.view(vs) if need_v else None, dtable,
-                *([None] * 9))
+            L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream())
+        return (dq, dk if need_k else None, dv if need_v else None, dtable) + (None,) * 7
 
 
 ATTENTION_MAX_LEN = 1 << 24
@@ -511,58 +519,75 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     _operand_dtype("biased_attention", q, k, v)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"biased_attention: {heads} heads over {kv_heads} key heads")
-    q4, k4 = _head_rows(q, heads, "biased_attention: q"), _head_rows(k, kv_heads, "biased_attention: k")
-    v4 = _head_rows(v, kv_heads, "biased_attention: v")
-    B, Sq, _, d = q4.shape
-    Sk = k4.size(1)
-    if k4.shape != v4.shape or k4.size(0) != B or k4.size(3) != d:
+    q, B, Sq, d, qst = _head_rows(q, heads, "biased_attention: q")
+    k, Bk, Sk, dk, kst = _head_rows(k, kv_heads, "biased_attention: k")
+    v, Bv, Sv, dv, vst = _head_rows(v, kv_heads, "biased_attention: v")
+    if (Bk, dk) != (B, d) or (Bv, Sv, dv) != (B, Sk, d):
         raise ValueError(f"biased_attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
     if d % 8 or not 8 <= d <= 128:
         raise ValueError(f"biased_attention: head size {d} is not a multiple of 8 in 8 .. 128")
     if B < 1 or not (1 <= Sq <= ATTENTION_MAX_LEN and 1 <= Sk <= ATTENTION_MAX_LEN):
         raise ValueError(f"biased_attention: batch {B}, lengths {Sq} and {Sk}")
+    if prefix is not None and not causal:
+        raise ValueError("biased_attention: a prefix needs causal=True")
+    if (table is None) != (buckets is None) or (table is not None and slopes is not None):
+        raise ValueError("biased_attention: table and buckets come together, and not with slopes")
+    if softcap is not None and not 0 < softcap < 1e30:
+        raise ValueError(f"biased_attention: softcap {softcap}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not abs(scale) < 1e30:
+        raise ValueError(f"biased_attention: scale {scale}")
+    args = L.AttentionArgs(batch=B, q_len=Sq, k_len=Sk, heads=heads, kv_heads=kv_heads, head_size=d, q_stride=qst,
+                           k_stride=kst, v_stride=vst, scale=scale, softcap=softcap or 0.0, causal=int(bool(causal)),
+                           dtype=L.dtype_code(q.dtype))
     if mask is not None:
         if mask.shape != (B, Sk):
             raise ValueError(f"biased_attention: mask {tuple(mask.shape)} does not match (B, Sk) = {(B, Sk)}")
         mask = _mask_i64(mask)
+        args.mask = mask.data_ptr()
     for name, t, shape, dtype in (("prefix", prefix, (B,), torch.int32), ("documents", documents, (B, Sk), torch.int32),
                                   ("slopes", slopes, (heads,), torch.float32)):
         if t is not None and (t.shape != shape or t.dtype != dtype):
             raise ValueError(f"biased_attention: {name} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    if prefix is not None and not causal:
-        raise ValueError("biased_attention: a prefix needs causal=True")
-    if slopes is not None and slopes.requires_grad:
-        raise ValueError("biased_attention: slopes have no gradient")
-    if (table is None) != (buckets is None) or (table is not None and slopes is not None):
-        raise ValueError("biased_attention: table and buckets come together, and not with slopes")
+    if prefix is not None:
+        prefix = prefix.contiguous()
+        args.prefix = prefix.data_ptr()
+    if documents is not None:
+        documents = documents.contiguous()
+        args.documents = documents.data_ptr()
+    if slopes is not None:
+        if slopes.requires_grad:
+            raise ValueError("biased_attention: slopes have no gradient")
+        slopes = slopes.contiguous()
+        args.slopes = slopes.data_ptr()
     if table is not None:
         if table.dim() != 2 or table.dtype != torch.float32 or table.size(1) != heads or not 1 <= table.size(0) <= 256:
             raise ValueError(f"biased_attention: table must be float32 (1 .. 256, {heads}), got {table.dtype} {tuple(table.shape)}")
         if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0 or not 3 <= buckets.numel() <= 2049:
             raise ValueError("biased_attention: buckets must be int32 of odd length 3 .. 2049")
-    if softcap is not None and not 0 < softcap < 1e30:
-        raise ValueError(f"biased_attention: softcap {softcap}")
+        table, buckets = table.contiguous(), buckets.contiguous()
+        args.table, args.buckets = table.data_ptr(), buckets.data_ptr()
+        args.num_buckets, args.distance = table.size(0), buckets.numel() // 2
     q_starts = None
     if isinstance(q_start, torch.Tensor):
         if q_start.shape != (B,) or q_start.dtype != torch.int32:
             raise ValueError(f"biased_attention: q_start must be an int or int32 ({B},)")
         L.require_gpu(q_start)
-        q_starts, q_start = q_start.contiguous(), 0
+        q_starts = q_start.contiguous()
+        args.q_starts = q_starts.data_ptr()
     else:
         q_start = Sk - Sq if q_start is None else int(q_start)
         if not 0 <= q_start <= ATTENTION_MAX_LEN:
             raise ValueError(f"biased_attention: queries start at position {q_start}")
         if documents is not None and q_start + Sq > Sk:
             raise ValueError(f"biased_attention: documents reach {Sk} positions, the queries {q_start + Sq}")
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not abs(scale) < 1e30:
-        raise ValueError(f"biased_attention: scale {scale}")
+        args.q_start = q_start
     _same_device("biased_attention", q, k=k, v=v, mask=mask, prefix=prefix, documents=documents, q_start=q_starts,
                  slopes=slopes, table=table, buckets=buckets)
-    cont = lambda t: None if t is None else t.contiguous()
-    return _BiasedAttention.apply(q, k, v, cont(table), mask, cont(documents), cont(prefix), q_starts, cont(slopes),
-                                  cont(buckets), int(heads), int(kv_heads),
-                                  (q_start, float(softcap or 0.0), scale, bool(causal)))
+    args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not _learns(q, k, v, table):
+        return _biased_attention_fwd(q, mask, documents, args, False)[0]
+    return _BiasedAttention.apply(q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, args)
 
 
 def segment_sum(tok: torch.Tensor, nseg: int, S: int, add: Optional[torch.Tensor] = None) -> torch.Tensor:
