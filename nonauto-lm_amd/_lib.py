@@ -53,7 +53,7 @@ SIGNATURES = {
     "mivae_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, F32,
                             P],
     "mivae_biased_attention_codes_ints": [I64, I64, I64, I32],
-    "mivae_biased_attention_bwd_floats": [I64, I64, I64, I64],
+    "mivae_biased_attention_bwd_floats": [I64, I64, I64, I64, I64, I64, I64],
     "mivae_biased_attention_fwd": [P, P],
     "mivae_biased_attention_bwd": [P, P],
     "mivae_qk_norm_rotary_scratch_floats": [I64],

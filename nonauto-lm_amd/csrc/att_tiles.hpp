@@ -71,18 +71,22 @@ __device__ __forceinline__ void pack8(f32x8& f, const f32x16& x, int s) {
 __device__ __forceinline__ float to_f32(unsigned short u) { return bf16_to_f32(u); }
 __device__ __forceinline__ float to_f32(float f) { return f; }
 
-// LDS tile of rows of 32 NDB elements.  bf16: row pitch of 4 or 12 (mod 16) 16-byte granules and an XOR of the granule
-// index with bits 2-3 of the row, so that both the 16-byte row reads and the transposing reads are free of bank
-// conflicts; fp32: an odd number of granules per row.
+// LDS tile of rows of 32 NDB elements, without padding for bf16: the 16-byte granule index is XORed with bits of the row so
+// that both the 16-byte row reads (16 rows, one granule) and the transposing reads (4 rows, 4 granules) touch all 64 banks
+// once.  4 or 12 granules per row: bits 2-3 of the row; 8: rows of one parity share the banks, bit 1 picks the half;
+// 16: bits 0-1 pick the quarter.  fp32: an odd number of granules per row.
 template <typename T, int NDB>
 struct Tile;
 
 template <int NDB>
 struct Tile<unsigned short, NDB> {
   static constexpr int W = 32 * NDB;
-  static constexpr int PITCH = (NDB == 1 || NDB == 3) ? W : W + 32;
+  static constexpr int PITCH = W;
   static constexpr int GE = 8, GPR = W / GE;
-  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ ((r >> 2) & 3)) << 3); }
+  static __device__ __forceinline__ int at(int r, int c) {
+    const int x = NDB == 4 ? (r & 3) << 2 | ((r >> 2) & 3) : NDB == 2 ? (r & 2) << 1 | ((r >> 2) & 3) : (r >> 2) & 3;
+    return r * PITCH + ((c ^ x) << 3);
+  }
   // f[j] = tile[r][16 s + 8 hh + j]
   static __device__ __forceinline__ bf16x8 row(const unsigned short* t, int r, int s, int hh) {
     return *reinterpret_cast<const bf16x8*>(t + at(r, 2 * s + hh));
@@ -186,64 +190,66 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&x)[NDB], float 
     }
 }
 
-// tanh.  bf16 operands: 1 - 2 / (1 + e^2x), absolute error about 1e-7, i.e. cap * 1e-7 in a score; fp32 operands: the
-// library function, whose relative error near 0 is a last-place one too.
-template <typename T>
-__device__ __forceinline__ float cap_tanh(float x) {
-  if (sizeof(T) == 4) return tanhf(x);
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x));
-}
-
-// wave-uniform constants of a block's scores
-struct ScoreParams {
-  float c2;         // scale * log2 e, or cap * log2 e
-  float ci;         // scale / cap
-  float slope2;     // slope * log2 e
-  bool cap, slope, tab;
-  int R;
+// Scores of a block in base-2 exponent units.  The raw product x of a pair becomes u = x, or with a cap
+// u = 1 / (1 + e^(-2 y)), y = scale x / cap, tanh y = 2 u - 1 (bf16 operands: absolute error about 1e-7, i.e. cap * 1e-7 in
+// a score; fp32 operands: u from the library's tanhf, a last-place error near 0 too).  The score is then A u + C, A >= 0,
+// plus the bias: linear, so that where the bias is constant over a tile everything folds into the exponential's one fma.
+struct Score {
+  float A, C, k;      // k: factor of x in the cap's exponent
+  float slope;        // slope * log2 e
+  bool cap, slopes, tab;
 };
 
-__device__ __forceinline__ ScoreParams score_params(const BiasedArgs& a, int head) {
-  ScoreParams p;
+__device__ __forceinline__ Score score_of(const BiasedArgs& a, int head, bool fp32) {
+  Score p;
   p.cap = a.cap > 0.f;
-  p.c2 = (p.cap ? a.cap : a.scale) * kLog2e;
-  p.ci = p.cap ? a.scale / a.cap : 0.f;
-  p.slope = a.slopes != nullptr;
-  p.slope2 = p.slope ? a.slopes[head] * kLog2e : 0.f;
+  p.A = p.cap ? 2.f * a.cap * kLog2e : a.scale * kLog2e;
+  p.C = p.cap ? -a.cap * kLog2e : 0.f;
+  p.k = p.cap ? (fp32 ? a.scale / a.cap : -2.f * kLog2e * a.scale / a.cap) : 0.f;
+  if (p.cap && fp32) { p.A = a.cap * kLog2e; p.C = 0.f; }       // fp32: u = tanh y
+  p.slopes = a.slopes != nullptr;
+  p.slope = p.slopes ? a.slopes[head] * kLog2e : 0.f;
   p.tab = a.table != nullptr;
-  p.R = a.R;
   return p;
 }
 
-// Raw products q.k of a tile -> biased scores in base-2 exponent units.  Register r's relative distance key - query is
-// rel + SIGN * acc_row(r) (SIGN = 1: the lane is a query, -1: the lane is a key); [rel_lo, rel_hi] bounds it over the wave.
-// GRAD: tt holds tanh for the cap's derivative.
-template <typename T, int SIGN, bool GRAD>
-__device__ __forceinline__ void score_tile(f32x16& sc, f32x16& tt, const ScoreParams& p, const float* tab, int rel, int rel_lo,
-                                           int rel_hi) {
-  if (p.cap) {
+template <typename T>
+__device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float t = cap_tanh<T>(sc[r] * p.ci);
-      if (GRAD) tt[r] = t;
-      sc[r] = t * p.c2;
-    }
-  } else {
+  for (int r = 0; r < 16; ++r)
+    u[r] = sizeof(T) == 4 ? tanhf(p.k * u[r]) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p.k * u[r]));
+}
+// d score / d x = scale * kCapSlope<T> * cap_slope(u)
+template <typename T>
+__device__ __forceinline__ float cap_slope(float u) { return sizeof(T) == 4 ? fmaf(-u, u, 1.f) : fmaf(-u, u, u); }
+template <typename T>
+__device__ __forceinline__ float cap_slope_factor() { return sizeof(T) == 4 ? 1.f : 4.f; }
+
+// Element-wise part: u <- A u + C + bias.  Register r's relative distance key - query is rel + SIGN * acc_row(r) (SIGN = 1: the
+// lane is a query, -1: the lane is a key); rel0 is that of the wave's first lane's row to the tile's first.
+template <int SIGN>
+__device__ __forceinline__ void bias_tile(f32x16& u, const Score& p, const float* tab, int R, int rel, int rel0) {
+  const bool behind = rel0 + 31 <= 0, inside = rel0 - 31 >= -R && rel0 + 31 <= R;        // wave-uniform
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] *= p.c2;
-  }
-  if (p.slope) {
+  for (int r = 0; r < 16; ++r) u[r] = fmaf(p.A, u[r], p.C);
+  if (p.slopes) {
+    if (behind) {                       // every key at or behind its query: -slope |rel| is linear in the register's row
+      const float base = p.slope * (float)rel;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] = fmaf(-p.slope2, fabsf((float)(rel + SIGN * acc_row(r))), sc[r]);
-  }
-  if (p.tab) {
-    if (rel_hi <= -p.R || rel_lo >= p.R) {            // wave-uniform: the whole tile is beyond the last distance
-      const float far = tab[rel_hi <= -p.R ? 0 : 2 * p.R];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] += far;
+      for (int r = 0; r < 16; ++r) u[r] += fmaf(p.slope, (float)(SIGN * acc_row(r)), base);
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] += tab[min(max(rel + SIGN * acc_row(r), -p.R), p.R) + p.R];
+      for (int r = 0; r < 16; ++r) u[r] = fmaf(-p.slope, fabsf((float)(rel + SIGN * acc_row(r))), u[r]);
+    }
+  }
+  if (p.tab) {
+    const float* t = tab + R + rel;
+    if (inside) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) u[r] += t[SIGN * acc_row(r)];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) u[r] += tab[min(max(rel + SIGN * acc_row(r), -R), R) + R];
     }
   }
 }
@@ -258,19 +264,11 @@ __device__ __forceinline__ void stage_table(float* tab, const BiasedArgs& a, int
 
 __device__ __forceinline__ int clamp_start(int s) { return min(max(s, -(1 << 30)), 1 << 30); }
 
-// Issue order of a run of N products whose A operands take DS LDS reads each: reads two products ahead of the matrix core
-// (the compiler's own order is read, wait, multiply, which exposes the LDS latency N times).
-template <int N, int DS>
-__device__ __forceinline__ void products_pipelined() {
-  if (N > 2) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * DS, 0);
-#pragma unroll
-    for (int i = 0; i < N - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-  }
+// the other half-wave's value, without a trip through LDS
+__device__ __forceinline__ float max_halves(float x) {
+  const unsigned b = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);        // {both low halves, both high halves}
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 }  // namespace mivae

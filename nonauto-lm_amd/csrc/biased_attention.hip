@@ -13,6 +13,8 @@
 // The backward recomputes the scores in both kernels (7 products, not 5): every output is written once, without atomics.
 // Softmax statistics, sums and all score arithmetic are fp32; P and dS are rounded to the operands' type for the second
 // products, which is what lets them run on the bf16 matrix instruction.
+#include <type_traits>
+
 #include "att_tiles.hpp"
 #include "mivae.h"
 
@@ -22,8 +24,14 @@ namespace {
 
 static inline hipStream_t S_(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+typedef __attribute__((address_space(3))) float lds_float;
+
 constexpr float kSlack = 8.f;       // exponent slack before the accumulators are rescaled
 constexpr int kWaves = 4, kRows = 32 * kWaves;      // rows (queries or keys) of a block
+// LDS buffers of the streamed tiles: two overlap the stores with the products; fp32 tiles are twice as large, the products
+// eight times as slow, and one buffer leaves room for the table gradient's arrays (141 of 160 KiB at d = 128, R = 1024)
+template <typename T>
+constexpr int buffers() { return sizeof(T) == 4 ? 1 : 2; }
 constexpr int kMaxDistance = 1024, kMaxBuckets = 256;
 
 // ---- visibility codes ------------------------------------------------------------------------------------------------
@@ -91,23 +99,28 @@ __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, f
   }
 }
 
-// What a block of 32 NW rows knows about visibility
+// ---- what a block knows about visibility -------------------------------------------------------------------------------
+// Causal mask and prefix are one limit per query, non-decreasing in the row: it sees the keys below limit(i).
 struct View {
-  int start, prefix;      // position of query 0, length of the beginning that everybody sees
+  int start, prefix, Sk;
   bool causal, codes, docs;
+  __device__ __forceinline__ int limit(int row) const { return causal ? min(Sk, max(start + row + 1, prefix)) : Sk; }
+  // first query row that sees key j
+  __device__ __forceinline__ int first_row(int key) const { return !causal || key < prefix ? 0 : max(0, key - start); }
 };
 
 __device__ __forceinline__ View view_of(const BiasedArgs& a, int64_t b) {
   View v;
   v.start = clamp_start(a.q_starts ? a.q_starts[b] : a.q_start);
   v.prefix = a.prefix ? a.prefix[b] : 0;
+  v.Sk = a.Sk;
   v.causal = a.causal != 0;
   v.codes = a.kcodes != nullptr;
   v.docs = a.qcodes != nullptr;
   return v;
 }
 
-// lowest / highest value of `code` over the wave, over lanes with code >= 0
+// lowest / highest value of `code` over the wave's lanes with code >= 0
 __device__ __forceinline__ void wave_range(int code, int& lo, int& hi) {
   lo = code >= 0 ? code : INT32_MAX;
   hi = code >= 0 ? code : -1;
@@ -142,8 +155,7 @@ struct KeyWalk {
 
 __device__ __forceinline__ KeyWalk key_walk(const BiasedArgs& a, const View& v, int64_t b, int row0) {
   KeyWalk w;
-  w.end = a.Sk;
-  if (v.causal) w.end = min(a.Sk, max(v.start + min(row0 + kRows, a.Sq), v.prefix));
+  w.end = v.limit(min(row0 + kRows, a.Sq) - 1);
   w.lo = w.hi = 0;
   w.tiles = v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr;
   if (v.docs) {
@@ -156,18 +168,53 @@ __device__ __forceinline__ KeyWalk key_walk(const BiasedArgs& a, const View& v, 
   return w;
 }
 
-// A tile of 32 queries (the lanes) x 32 keys (the registers): -inf where a pair is not seen
-__device__ __forceinline__ void hide_keys(f32x16& sc, const View& v, int key, int rel, int Sk, const int* kc, int qcode) {
+// What a wave of 32 queries (one per lane, both half-waves the same) sees of a chunk
+struct QueryWave {
+  int row, limit;               // the lane's query
+  int first, last;              // limits of the wave's first and last query
+  int code, lo, hi;             // the lane's code and the wave's range
+  bool none;                    // some lane's query sees nothing
+  // 0: nothing of the chunk, 1: some of its pairs, 2: all of them
+  __device__ __forceinline__ int sees(const KeyWalk& w, int kc) const {
+    if (kc >= last) return 0;
+    bool all = kc + kChunk <= first;
+    if (w.tiles != nullptr) {
+      const i32x4 t = w.tiles[kc / kChunk];
+      if (t[1] < lo || t[0] > hi) return 0;
+      all = all && !t[2] && !none && lo == hi && t[0] == lo && t[1] == lo;
+    }
+    return all ? 2 : 1;
+  }
+};
+
+__device__ __forceinline__ QueryWave query_wave(const BiasedArgs& a, const View& v, int64_t b, int q0, int r32) {
+  QueryWave w;
+  w.row = q0 + r32;
+  w.limit = v.limit(w.row);
+  w.first = v.limit(q0);
+  w.last = q0 < a.Sq ? v.limit(min(q0 + 32, a.Sq) - 1) : 0;
+  w.code = w.lo = w.hi = 0;
+  w.none = false;
+  if (v.docs) {
+    w.code = w.row < a.qpad ? a.qcodes[b * a.qpad + w.row] : kNoCode;
+    wave_range(w.code, w.lo, w.hi);
+    w.none = __builtin_amdgcn_ballot_w64(w.code < 0) != 0;
+  }
+  return w;
+}
+
+// lane: query, registers: keys key0 + 4 hh + acc_row(r)
+__device__ __forceinline__ void hide_keys(f32x16& u, const QueryWave& w, bool codes, int key, const int* kc) {
+  const int lim = w.limit - key;
+  if (!codes) {
 #pragma unroll
-  for (int a4 = 0; a4 < 4; ++a4) {
-    const i32x4 code = v.codes ? *reinterpret_cast<const i32x4*>(kc + 8 * a4) : i32x4{0, 0, 0, 0};
+    for (int r = 0; r < 16; ++r) u[r] = acc_row(r) < lim ? u[r] : -INFINITY;
+  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int o = 8 * a4 + i;
-      bool see = key + o < Sk;
-      if (v.causal) see = see && (rel + o <= 0 || key + o < v.prefix);
-      if (v.codes) see = see && code[i] == qcode;
-      if (!see) sc[4 * a4 + i] = -INFINITY;
+    for (int a4 = 0; a4 < 4; ++a4) {
+      const i32x4 code = *reinterpret_cast<const i32x4*>(kc + 8 * a4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[4 * a4 + i] = 8 * a4 + i < lim && code[i] == w.code ? u[4 * a4 + i] : -INFINITY;
     }
   }
 }
@@ -176,50 +223,46 @@ struct Ids {
   int64_t b;
   int head, blk;
 };
-// block id -> (batch row, head, block of rows).  Blocks of one head follow one another; with a causal mask the long ones
-// (many keys to walk) come first.
-__device__ __forceinline__ Ids ids_of(int heads, int nblk, bool last_first) {
+// Block id -> (batch row, head, block of rows): all heads' blocks of one position before the next position.  Ids go round the
+// eight XCDs, so with a multiple of eight (batch row, head) pairs all blocks of a pair share one L2; and the blocks with the
+// longest walks (last queries, first keys under a causal mask) start first.
+__device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool last_first) {
   Ids r;
-  const int64_t id = blockIdx.x;
-  r.blk = (int)(id % nblk);
+  const unsigned bhs = (unsigned)B * (unsigned)heads, id = blockIdx.x;
+  r.blk = (int)(id / bhs);
   if (last_first) r.blk = nblk - 1 - r.blk;
-  const int64_t bh = id / nblk;
-  r.head = (int)(bh % heads);
-  r.b = bh / heads;
+  const unsigned bh = id % bhs;
+  r.head = (int)(bh % (unsigned)heads);
+  r.b = bh / (unsigned)heads;
   return r;
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
+// Chunks go through two LDS buffers: the next one is stored and the one after it is on its way while a chunk is multiplied,
+// one barrier per chunk.
 template <typename T, int NDB>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(BiasedArgs a) {
   using L = Tile<T, NDB>;
+  constexpr int TW = kChunk / 32, TILE = kChunk * L::PITCH, NBUF = buffers<T>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* kt = reinterpret_cast<T*>(smem);
-  T* vt = kt + kChunk * L::PITCH;
-  int* kc_lds = reinterpret_cast<int*>(vt + kChunk * L::PITCH);
-  float* tab = reinterpret_cast<float*>(kc_lds + kChunk);
+  T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][K, V]
+  int* kc_lds = reinterpret_cast<int*>(tiles + 2 * NBUF * TILE);          // [NBUF][kChunk]
+  float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const int nblk = (a.Sq + kRows - 1) / kRows;
-  const Ids id = ids_of(a.heads, nblk, a.causal);
+  const Ids id = ids_of(a.B, a.heads, (a.Sq + kRows - 1) / kRows, true);
   const int64_t b = id.b;
-  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave, row = q0 + r32;
+  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
   const KeyWalk walk = key_walk(a, v, b, row0);
-  const ScoreParams sp = score_params(a, head);
+  const QueryWave qw = query_wave(a, v, b, q0, r32);
+  const Score sp = score_of(a, head, sizeof(T) == 4);
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
-  const int qpos = v.start + row;
-  const int qcode = !v.docs ? 0 : row < a.qpad ? a.qcodes[b * a.qpad + row] : kNoCode;
-  int qlo = 0, qhi = 0;
-  bool qneg = false;                    // some row of the wave sees nothing
-  if (v.docs) {
-    wave_range(qcode, qlo, qhi);
-    qneg = __builtin_amdgcn_ballot_w64(qcode < 0) != 0;
-  }
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
+  const bool live = qw.row < a.Sq;
   typename Frag<T>::type qf[2 * NDB];
-  load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)row * a.qs[1] + head * a.qs[2], row < a.Sq, a.d, hh);
+  load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)qw.row * a.qs[1] + head * a.qs[2], live, a.d, hh);
   f32x16 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
@@ -227,85 +270,110 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   float m = -__FLT_MAX__, l = 0.f;
   Stage<T, NDB, kWaves> sk, sv;
-  int pc = 0;
+  int pc = 0, buf = 0;
   auto load = [&](int kc) {
     sk.load(kbase, a.ks[1], kc, a.Sk, a.d, codes);
     sv.load(vbase, a.vs[1], kc, a.Sk, a.d, codes);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0);
+  auto store = [&](int n) {
+    sk.store(tiles + 2 * n * TILE);
+    sv.store(tiles + (2 * n + 1) * TILE);
+    if (v.codes && threadIdx.x < kChunk) kc_lds[n * kChunk + threadIdx.x] = pc;
+  };
+  int kc = walk.next(0), kn = kc;       // the chunk to multiply, the chunk in the registers
   if (kc < walk.end) load(kc);
-  while (kc < walk.end) {
-    __syncthreads();                    // the previous chunk has been consumed
-    sk.store(kt);
-    sv.store(vt);
-    if (v.codes && threadIdx.x < kChunk) kc_lds[threadIdx.x] = pc;
-    __syncthreads();
-    const int kn = walk.next(kc + kChunk);
-    if (kn < walk.end) load(kn);        // travels while this chunk is multiplied
-    if (q0 < a.Sq) {                    // wave-uniform, like every branch below
+  if (NBUF == 2 && kc < walk.end) {
+    store(0);
+    kn = walk.next(kc + kChunk);
+    if (kn < walk.end) load(kn);
+  }
+  for (; kc < walk.end; buf ^= NBUF - 1) {
+    __syncthreads();                    // this chunk is stored, the previous one consumed
+    const int at = kc;
+    if (NBUF == 1) {
+      store(0);
+      __syncthreads();
+    } else if (kn < walk.end) {
+      store(buf ^ 1);
+    }
+    const int ahead = kn < walk.end ? walk.next(kn + kChunk) : kn;
+    if (ahead < walk.end) load(ahead);
+    kc = NBUF == 1 ? ahead : kn;
+    kn = ahead;
+    const int sees = qw.sees(walk, at); // wave-uniform, like every branch below
+    if (sees == 0) continue;
+    const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
+    const int rel0 = at - (v.start + q0);                       // the wave's first query to the chunk's first key
+    f32x16 u[TW];
 #pragma unroll
-      for (int t = 0; t < kChunk / 32; ++t) {
-        const int key0 = kc + 32 * t;
-        if (key0 >= walk.end) break;
-        const int rel0 = key0 - (v.start + q0);                       // query 0 of the wave to key 0 of the tile
-        const bool beyond = v.causal && rel0 > 31 && key0 >= v.prefix;
-        bool clean = key0 + 32 <= a.Sk && (!v.causal || rel0 + 31 <= 0 || key0 + 32 <= v.prefix);
-        bool other = false;
-        if (v.codes) {
-          const i32x4 ts = walk.tiles[kc / kChunk];
-          other = ts[1] < qlo || ts[0] > qhi;
-          clean = clean && !ts[2] && ts[0] == ts[1] && !qneg && qlo == qhi && ts[0] == qlo;
-        }
-        if (beyond || other) continue;
-        f32x16 sc, tt;
+    for (int t = 0; t < TW; ++t) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+      for (int r = 0; r < 16; ++r) u[t][r] = 0.f;
 #pragma unroll
-        for (int s = 0; s < 2 * NDB; ++s) sc = mma(L::row(kt, 32 * t + r32, s, hh), qf[s], sc);
-        score_tile<T, 1, false>(sc, tt, sp, tab, key0 + 4 * hh - qpos, rel0 - 31, rel0 + 31);
-        if (!clean) hide_keys(sc, v, key0 + 4 * hh, key0 + 4 * hh - qpos, a.Sk, kc_lds + 32 * t + 4 * hh, qcode);
-        float tmax = sc[0];
+      for (int s = 0; s < 2 * NDB; ++s) u[t] = mma(L::row(kt, 32 * t + r32, s, hh), qf[s], u[t]);
+    }
+    if (sp.cap) {
 #pragma unroll
-        for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, sc[r]);
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
-        // m follows the running maximum only when that has grown by more than 2^kSlack: most tiles skip the rescaling
-        if (__builtin_amdgcn_ballot_w64(tmax > m + kSlack) != 0) {
-          const float mn = tmax > m + kSlack ? tmax : m;
-          const float alpha = __builtin_amdgcn_exp2f(m - mn);
-          l *= alpha;
-          m = mn;
+      for (int t = 0; t < TW; ++t) cap_tile<T>(u[t], sp);
+    }
+    float A = sp.A, C = sp.C;
+    const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
+    if (sees == 1 || sp.slopes || near) {
 #pragma unroll
-          for (int db = 0; db < NDB; ++db)
+      for (int t = 0; t < TW; ++t) {
+        const int key = at + 32 * t + 4 * hh;
+        bias_tile<1>(u[t], sp, tab, a.R, key - (v.start + qw.row), rel0 + 32 * t);
+        if (sees == 1) hide_keys(u[t], qw, v.codes, key, kc_lds + buf * kChunk + 32 * t + 4 * hh);
+      }
+      A = 1.f;
+      C = 0.f;
+    } else if (sp.tab) {
+      C += tab[rel0 < 0 ? 0 : 2 * a.R];
+    }
+    float top = u[0][0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-        }
-        float ps = 0.f;
+    for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sc[r] = __builtin_amdgcn_exp2f(sc[r] - m);
-          ps += sc[r];
-        }
-        l += ps;
-        typename Frag<T>::type p0, p1;
-        pack8(p0, sc, 0);
-        pack8(p1, sc, 1);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, u[t][r]);
+    top = fmaf(A, max_halves(top), C);
+    // m follows the running maximum only when that has grown by more than 2^kSlack: most chunks skip the rescaling
+    if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
+      const float mn = top > m + kSlack ? top : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+      m = mn;
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          o[db] = mma(L::col(vt, 32 * t, db, lane), p0, o[db]);
-          o[db] = mma(L::col(vt, 32 * t + 16, db, lane), p1, o[db]);
-        }
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+    }
+    const float cm = C - m;
+    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < TW; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        u[t][r] = __builtin_amdgcn_exp2f(fmaf(A, u[t][r], cm));
+        ps[r & 3] += u[t][r];
+      }
+      typename Frag<T>::type p0, p1;
+      pack8(p0, u[t], 0);
+      pack8(p1, u[t], 1);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        o[db] = mma(L::col(vt, 32 * t, db, lane), p0, o[db]);
+        o[db] = mma(L::col(vt, 32 * t + 16, db, lane), p1, o[db]);
       }
     }
-    kc = kn;
+    l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   }
   l += __shfl_xor(l, 32, 64);           // the half-waves hold disjoint keys of the same query
-  if (row < a.Sq) {
+  if (live) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t at = ((b * a.Sq + row) * a.heads + head) * a.d;
-    store_row<T, NDB>(static_cast<T*>(a.out) + at, o, inv, a.d, hh);
+    store_row<T, NDB>(static_cast<T*>(a.out) + ((b * a.Sq + qw.row) * a.heads + head) * a.d, o, inv, a.d, hh);
     if (a.lse && hh == 0)
-      a.lse[(b * a.heads + head) * a.Sq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+      a.lse[(b * a.heads + head) * a.Sq + qw.row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
 }
 
@@ -321,19 +389,20 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 template <typename T, int NDB, bool DELTA>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a) {
   using L = Tile<T, NDB>;
+  constexpr int TILE = kChunk * L::PITCH, NBUF = buffers<T>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* kt = reinterpret_cast<T*>(smem);
-  T* vt = kt + kChunk * L::PITCH;
-  int* kc_lds = reinterpret_cast<int*>(vt + kChunk * L::PITCH);
-  float* tab = reinterpret_cast<float*>(kc_lds + kChunk);
+  T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][K, V]
+  int* kc_lds = reinterpret_cast<int*>(tiles + 2 * NBUF * TILE);          // [NBUF][kChunk]
+  float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
   const int nblk = (a.Sq + kRows - 1) / kRows;
-  const Ids id = ids_of(a.heads, nblk, a.causal);
+  const Ids id = ids_of(a.B, a.heads, nblk, true);
   const int64_t b = id.b;
-  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave, row = q0 + r32;
+  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
   const KeyWalk walk = key_walk(a, v, b, row0);
-  const ScoreParams sp = score_params(a, head);
+  const QueryWave qw = query_wave(a, v, b, q0, r32);
+  const Score sp = score_of(a, head, sizeof(T) == 4);
   const int TW = 2 * a.R + 1;
   float* hist = tab + TW;                            // [2 kWaves][TW]
   float* mine = hist + (2 * wave + hh) * TW;
@@ -341,22 +410,15 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
   if (grad_tab)
     for (int i = threadIdx.x; i < 2 * kWaves * TW; i += 64 * kWaves) hist[i] = 0.f;
-  const int qpos = v.start + row;
-  const int qcode = !v.docs ? 0 : row < a.qpad ? a.qcodes[b * a.qpad + row] : kNoCode;
-  int qlo = 0, qhi = 0;
-  bool qneg = false;                    // some row of the wave sees nothing
-  if (v.docs) {
-    wave_range(qcode, qlo, qhi);
-    qneg = __builtin_amdgcn_ballot_w64(qcode < 0) != 0;
-  }
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
-  const int64_t at = ((b * a.Sq + row) * a.heads + head) * a.d, at1 = (b * a.heads + head) * a.Sq + row;
+  const bool live = qw.row < a.Sq;
+  const int64_t at_q = ((b * a.Sq + qw.row) * a.heads + head) * a.d, at_l = (b * a.heads + head) * a.Sq + qw.row;
   typename Frag<T>::type qf[2 * NDB], dof[2 * NDB];
-  load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)row * a.qs[1] + head * a.qs[2], row < a.Sq, a.d, hh);
-  load_row<T, NDB>(dof, static_cast<const T*>(a.dout) + at, row < a.Sq, a.d, hh);
-  const float lse = row < a.Sq ? a.lse[at1] : INFINITY, delta = !DELTA && row < a.Sq ? a.delta[at1] : 0.f;
+  load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)qw.row * a.qs[1] + head * a.qs[2], live, a.d, hh);
+  load_row<T, NDB>(dof, static_cast<const T*>(a.dout) + at_q, live, a.d, hh);
+  const float lse = live ? a.lse[at_l] : INFINITY, delta = !DELTA && live ? a.delta[at_l] : 0.f;
   float dsum = 0.f;
   f32x16 dq[NDB];
 #pragma unroll
@@ -365,95 +427,120 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     for (int r = 0; r < 16; ++r) dq[db][r] = 0.f;
   float far_lo = 0.f, far_hi = 0.f;
   Stage<T, NDB, kWaves> sk, sv;
-  int pc = 0;
+  int pc = 0, buf = 0;
   auto load = [&](int kc) {
     sk.load(kbase, a.ks[1], kc, a.Sk, a.d, codes);
     sv.load(vbase, a.vs[1], kc, a.Sk, a.d, codes);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0);
+  auto store = [&](int n) {
+    sk.store(tiles + 2 * n * TILE);
+    sv.store(tiles + (2 * n + 1) * TILE);
+    if (v.codes && threadIdx.x < kChunk) kc_lds[n * kChunk + threadIdx.x] = pc;
+  };
+  int kc = walk.next(0), kn = kc;       // the chunk to multiply, the chunk in the registers
   if (kc < walk.end) load(kc);
-  while (kc < walk.end) {
-    __syncthreads();
-    sk.store(kt);
-    sv.store(vt);
-    if (v.codes && threadIdx.x < kChunk) kc_lds[threadIdx.x] = pc;
-    __syncthreads();
-    const int kn = walk.next(kc + kChunk);
+  if (NBUF == 2 && kc < walk.end) {
+    store(0);
+    kn = walk.next(kc + kChunk);
     if (kn < walk.end) load(kn);
-    if (q0 < a.Sq) {
+  }
+  for (; kc < walk.end; buf ^= NBUF - 1) {
+    __syncthreads();
+    const int at = kc;
+    if (NBUF == 1) {
+      store(0);
+      __syncthreads();
+    } else if (kn < walk.end) {
+      store(buf ^ 1);
+    }
+    const int ahead = kn < walk.end ? walk.next(kn + kChunk) : kn;
+    if (ahead < walk.end) load(ahead);
+    kc = NBUF == 1 ? ahead : kn;
+    kn = ahead;
+    const int sees = qw.sees(walk, at);
+    if (sees == 0) continue;
+    const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
 #pragma unroll
-      for (int t = 0; t < kChunk / 32; ++t) {
-        const int key0 = kc + 32 * t;
-        if (key0 >= walk.end) break;
-        const int rel0 = key0 - (v.start + q0);
-        const bool beyond = v.causal && rel0 > 31 && key0 >= v.prefix;
-        bool clean = key0 + 32 <= a.Sk && (!v.causal || rel0 + 31 <= 0 || key0 + 32 <= v.prefix);
-        bool other = false;
-        if (v.codes) {
-          const i32x4 ts = walk.tiles[kc / kChunk];
-          other = ts[1] < qlo || ts[0] > qhi;
-          clean = clean && !ts[2] && ts[0] == ts[1] && !qneg && qlo == qhi && ts[0] == qlo;
-        }
-        if (beyond || other) continue;
-        f32x16 sc, dp, tt;
+    for (int t = 0; t < kChunk / 32; ++t) {
+      const int key0 = at + 32 * t, rel0 = key0 - (v.start + q0);
+      if (key0 >= qw.last) break;
+      f32x16 u, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { sc[r] = 0.f; dp[r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { u[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
-        for (int s = 0; s < 2 * NDB; ++s) {
-          sc = mma(L::row(kt, 32 * t + r32, s, hh), qf[s], sc);
-          dp = mma(L::row(vt, 32 * t + r32, s, hh), dof[s], dp);
-        }
-        const int rel = key0 + 4 * hh - qpos;
-        score_tile<T, 1, !DELTA>(sc, tt, sp, tab, rel, rel0 - 31, rel0 + 31);
-        if (!clean) hide_keys(sc, v, key0 + 4 * hh, rel, a.Sk, kc_lds + 32 * t + 4 * hh, qcode);
-        if (DELTA) {
+      for (int s = 0; s < 2 * NDB; ++s) {
+        u = mma(L::row(kt, 32 * t + r32, s, hh), qf[s], u);
+        dp = mma(L::row(vt, 32 * t + r32, s, hh), dof[s], dp);
+      }
+      f32x16 g;                          // the cap's slope
+      if (sp.cap) {
+        cap_tile<T>(u, sp);
+        if (!DELTA)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dsum = fmaf(__builtin_amdgcn_exp2f(sc[r] - lse), dp[r], dsum);
-          continue;
-        }
+          for (int r = 0; r < 16; ++r) g[r] = cap_slope<T>(u[r]);
+      }
+      float A = sp.A, C = sp.C;
+      const int rel = key0 + 4 * hh - (v.start + qw.row);
+      const bool far = sp.tab && (rel0 + 31 <= -a.R || rel0 - 31 >= a.R);
+      if (sees == 1 || sp.slopes || (sp.tab && !far)) {
+        bias_tile<1>(u, sp, tab, a.R, rel, rel0);
+        if (sees == 1) hide_keys(u, qw, v.codes, key0 + 4 * hh, kc_lds + buf * kChunk + 32 * t + 4 * hh);
+        A = 1.f;
+        C = 0.f;
+      } else if (sp.tab) {
+        C += tab[rel0 < 0 ? 0 : 2 * a.R];
+      }
+      const float cm = C - lse;
+      if (DELTA) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(sc[r] - lse) * (dp[r] - delta);     // ds
-        if (grad_tab) {
-          const int lo = rel0 - 31, hi = rel0 + 31;
-          if (hi <= -a.R || lo >= a.R) {
-            float s = 0.f;
+        for (int r = 0; r < 16; ++r) dsum = fmaf(__builtin_amdgcn_exp2f(fmaf(A, u[r], cm)), dp[r], dsum);
+        continue;
+      }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s += sc[r];
-            if (hi <= -a.R) far_lo += s;
-            else far_hi += s;
-          } else {
+      for (int r = 0; r < 16; ++r) u[r] = __builtin_amdgcn_exp2f(fmaf(A, u[r], cm)) * (dp[r] - delta);     // ds
+      if (grad_tab) {
+        if (far) {
+          float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int x = rel + acc_row(r);
-              if (x <= -a.R) far_lo += sc[r];
-              else if (x >= a.R) far_hi += sc[r];
-              else __builtin_amdgcn_ds_faddf((__attribute__((address_space(3))) float*)(mine + x + a.R), sc[r], 0, 0, false);
-            }
+          for (int r = 0; r < 16; ++r) s += u[r];
+          if (rel0 < 0) far_lo += s;
+          else far_hi += s;
+        } else if (rel0 - 31 > -a.R && rel0 + 31 < a.R) {
+          lds_float* h = (lds_float*)(mine + rel + a.R);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) __builtin_amdgcn_ds_faddf(h + acc_row(r), u[r], 0, 0, false);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int x = rel + acc_row(r);
+            if (x <= -a.R) far_lo += u[r];
+            else if (x >= a.R) far_hi += u[r];
+            else __builtin_amdgcn_ds_faddf((lds_float*)(mine + x + a.R), u[r], 0, 0, false);
           }
         }
-        if (sp.cap) {
+      }
+      if (sp.cap) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[r] *= 1.f - tt[r] * tt[r];
-        }
-        typename Frag<T>::type d0, d1;
-        pack8(d0, sc, 0);
-        pack8(d1, sc, 1);
+        for (int r = 0; r < 16; ++r) u[r] *= g[r];
+      }
+      typename Frag<T>::type d0, d1;
+      pack8(d0, u, 0);
+      pack8(d1, u, 1);
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          dq[db] = mma(L::col(kt, 32 * t, db, lane), d0, dq[db]);
-          dq[db] = mma(L::col(kt, 32 * t + 16, db, lane), d1, dq[db]);
-        }
+      for (int db = 0; db < NDB; ++db) {
+        dq[db] = mma(L::col(kt, 32 * t, db, lane), d0, dq[db]);
+        dq[db] = mma(L::col(kt, 32 * t + 16, db, lane), d1, dq[db]);
       }
     }
-    kc = kn;
   }
   if (DELTA) {
     dsum += __shfl_xor(dsum, 32, 64);
-    if (row < a.Sq && hh == 0) a.delta[at1] = dsum;
+    if (live && hh == 0) a.delta[at_l] = dsum;
     return;
   }
-  if (row < a.Sq && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at, dq, a.scale, a.d, hh);
+  const float out_scale = a.scale * (sp.cap ? cap_slope_factor<T>() : 1.f);
+  if (live && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, out_scale, a.d, hh);
   if (grad_tab) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -474,10 +561,15 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       ids[i] = min(max(a.buckets[i], 0), a.nb - 1);
     }
     __syncthreads();
-    for (int n = threadIdx.x; n < a.nb; n += 64 * kWaves) {
+    int lanes = 64;                      // lanes per bucket, a power of two
+    while (lanes > 1 && lanes * a.nb > 64 * kWaves) lanes >>= 1;
+    for (int n0 = 0; n0 < a.nb; n0 += 64 * kWaves / lanes) {
+      const int n = n0 + (int)threadIdx.x / lanes;
       float s = 0.f;
-      for (int i = 0; i < TW; ++i) s += ids[i] == n ? hist[i] : 0.f;
-      a.dtab[((int64_t)head * a.B * nblk + b * nblk + id.blk) * a.nb + n] = s;
+      for (int i = threadIdx.x % lanes; i < TW; i += lanes) s += ids[i] == n ? hist[i] : 0.f;
+      s = group_sum(s, lanes);
+      if (threadIdx.x % lanes == 0 && n < a.nb)
+        a.dtab[((int64_t)head * a.B * nblk + b * nblk + id.blk) * a.nb + n] = s;
     }
   }
 }
@@ -493,21 +585,22 @@ __global__ __launch_bounds__(64) void k_ba_dtable(const float* part, float* dtab
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------
+// A block's walk over the queries of all heads of a group.  Where key heads are few, `split` blocks share a group's heads
+// and leave fp32 partials that k_ba_fold sums in order.
 template <typename T, int NDB>
-__global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, float* part) {
   using L = Tile<T, NDB>;
+  constexpr int TILE = kChunk * L::PITCH, NBUF = buffers<T>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* qt = reinterpret_cast<T*>(smem);
-  T* dt = qt + kChunk * L::PITCH;
-  float* lses = reinterpret_cast<float*>(dt + kChunk * L::PITCH);
-  float* dels = lses + kChunk;
-  int* qc_lds = reinterpret_cast<int*>(dels + kChunk);
-  float* tab = reinterpret_cast<float*>(qc_lds + kChunk);
+  T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][Q, dO]
+  float* lses = reinterpret_cast<float*>(tiles + 2 * NBUF * TILE);        // [NBUF][kChunk] each
+  float* dels = lses + NBUF * kChunk;
+  int* qc_lds = reinterpret_cast<int*>(dels + NBUF * kChunk);
+  float* tab = reinterpret_cast<float*>(qc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const int nblk = (a.Sk + kRows - 1) / kRows;
-  const Ids id = ids_of(a.kv, nblk, false);
+  const Ids id = ids_of(a.B, a.kv * split, (a.Sk + kRows - 1) / kRows, false);
   const int64_t b = id.b;
-  const int kvh = id.head, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
+  const int kvh = id.head / split, share = id.head % split, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
   const View v = view_of(a, b);
   const bool ok = key < a.Sk;
   const int kcode = !ok ? -1 : v.codes ? a.kcodes[b * a.kpad + key] : 0;
@@ -517,9 +610,9 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
     wave_range(kcode, klo, khi);
     khid = __builtin_amdgcn_ballot_w64(kcode < 0) != 0;
   }
-  // the block's first query chunk and range of key codes
-  int qfirst = 0;
-  if (v.causal && row0 >= v.prefix) qfirst = max(0, row0 - v.start) / kChunk * kChunk;
+  const int first = v.first_row(key);                                     // the lane's key is seen from this row on
+  const int wfirst = v.first_row(k0), wall = v.first_row(min(k0 + 31, a.Sk - 1));        // some / every key of the wave
+  const int qfirst = v.first_row(row0) / kChunk * kChunk;
   i32x4 br = {0, 0, 0, 0};
   if (v.codes) {
     const i32x4* t = a.ktiles + b * (a.kpad / 64);
@@ -527,15 +620,22 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
     if (row0 + 64 < a.Sk) br = merge(br, t[row0 / 64 + 1]);
   }
   const i32x4* qtiles = v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr;
-  auto next = [&](int qc) {
-    if (v.codes && !v.docs && br[1] < 0) return a.Sq;              // every key of the block is hidden
-    if (qtiles != nullptr)
-      while (qc < a.Sq) {
-        const i32x4 t = qtiles[qc / kChunk];
+  // next chunk of queries of the group's heads that the block's keys may be seen from
+  const int glast = (share + 1) * a.group / split;
+  struct Pos { int g, qc; };
+  auto settle = [&](Pos p) {
+    while (p.g < glast) {
+      if (br[1] < 0) { p.g = glast; break; }                             // every key of the block is hidden
+      while (qtiles != nullptr && p.qc < a.Sq) {
+        const i32x4 t = qtiles[p.qc / kChunk];
         if (t[1] >= br[0] && t[0] <= br[1]) break;
-        qc += kChunk;
+        p.qc += kChunk;
       }
-    return qc;
+      if (p.qc < a.Sq) break;
+      p.g += 1;
+      p.qc = qfirst;
+    }
+    return p;
   };
   typename Frag<T>::type kf[2 * NDB], vf[2 * NDB];
   load_row<T, NDB>(kf, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + kvh * a.ks[2], kcode >= 0, a.d, hh);
@@ -547,141 +647,204 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
     for (int r = 0; r < 16; ++r) { dk[db][r] = 0.f; dv[db][r] = 0.f; }
   Stage<T, NDB, kWaves> sq, sd;
   float pl = 0.f, pd = 0.f;
-  int pq = 0;
-  auto load = [&](int head, int qc) {
-    sq.load(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], qc, a.Sq, a.d, nullptr);
-    sd.load(static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d, (int64_t)a.heads * a.d, qc, a.Sq, a.d, nullptr);
-    const int i = qc + (int)threadIdx.x;
+  int pq = 0, buf = 0;
+  auto load = [&](Pos p) {
+    const int head = kvh * a.group + p.g;
+    sq.load(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, a.Sq, a.d, nullptr);
+    sd.load(static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d, (int64_t)a.heads * a.d, p.qc, a.Sq, a.d, nullptr);
+    const int i = p.qc + (int)threadIdx.x;
     const bool in = threadIdx.x < kChunk && i < a.Sq;
     pl = in ? a.lse[(b * a.heads + head) * a.Sq + i] : INFINITY;    // rows beyond Sq: p = exp2(. - inf) = 0
     pd = in ? a.delta[(b * a.heads + head) * a.Sq + i] : 0.f;
     if (v.docs && threadIdx.x < kChunk) pq = a.qcodes[b * a.qpad + i];
   };
-  for (int g = 0; g < a.group; ++g) {
-    const int head = kvh * a.group + g;
-    const ScoreParams sp = score_params(a, head);
-    __syncthreads();                    // the last chunk of the previous head has been consumed
-    if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
-    int qc = next(qfirst);
-    if (qc < a.Sq) load(head, qc);
-    while (qc < a.Sq) {
-      __syncthreads();
-      sq.store(qt);
-      sd.store(dt);
-      if (threadIdx.x < kChunk) {
-        lses[threadIdx.x] = pl;
-        dels[threadIdx.x] = pd;
-        qc_lds[threadIdx.x] = pq;
+  auto store = [&](int n) {
+    sq.store(tiles + 2 * n * TILE);
+    sd.store(tiles + (2 * n + 1) * TILE);
+    if (threadIdx.x < kChunk) {
+      lses[n * kChunk + threadIdx.x] = pl;
+      dels[n * kChunk + threadIdx.x] = pd;
+      qc_lds[n * kChunk + threadIdx.x] = pq;
+    }
+  };
+  Pos p = settle(Pos{share * a.group / split, qfirst}), pn = p;          // to multiply, in the registers
+  if (p.g < glast) load(p);
+  if (NBUF == 2 && p.g < glast) {
+    store(0);
+    pn = settle(Pos{p.g, p.qc + kChunk});
+    if (pn.g < glast) load(pn);
+  }
+  int tab_head = -1;
+  Score sp = score_of(a, kvh * a.group, sizeof(T) == 4);
+  for (; p.g < glast; buf ^= NBUF - 1) {
+    const Pos at = p;
+    const int head = kvh * a.group + at.g;
+    __syncthreads();
+    if (head != tab_head) {             // block-uniform: another head's bias
+      sp = score_of(a, head, sizeof(T) == 4);
+      tab_head = head;
+      if (sp.tab) {
+        stage_table(tab, a, head, 64 * kWaves);
+        __syncthreads();
       }
+    }
+    if (NBUF == 1) {
+      store(0);
       __syncthreads();
-      const int qn = next(qc + kChunk);
-      if (qn < a.Sq) load(head, qn);
-      if (k0 < a.Sk) {
+    } else if (pn.g < glast) {
+      store(buf ^ 1);
+    }
+    const Pos ahead = pn.g < glast ? settle(Pos{pn.g, pn.qc + kChunk}) : pn;
+    if (ahead.g < glast) load(ahead);
+    p = NBUF == 1 ? ahead : pn;
+    pn = ahead;
+    if (k0 >= a.Sk || at.qc + kChunk <= wfirst) continue;
+    bool clean = !khid && at.qc >= wall;
+    if (v.docs) {
+      const i32x4 ts = qtiles[at.qc / kChunk];
+      if (ts[1] < klo || ts[0] > khi) continue;
+      clean = clean && !ts[2] && ts[0] == ts[1] && klo == khi && ts[0] == klo;
+    } else if (v.codes && khi < 0) {
+      continue;
+    }
+    const T *qt = tiles + 2 * buf * TILE, *dt = qt + TILE;
+    const float *ls = lses + buf * kChunk, *de = dels + buf * kChunk;
+    const int* qcs = qc_lds + buf * kChunk;
 #pragma unroll
-        for (int t = 0; t < kChunk / 32; ++t) {
-          const int q0 = qc + 32 * t;
-          if (q0 >= a.Sq) break;
-          const int rel0 = k0 - (v.start + q0);             // query 0 of the tile to key 0 of the wave
-          const bool beyond = v.causal && rel0 > 31 && k0 >= v.prefix;
-          bool clean = !khid && (!v.causal || rel0 + 31 <= 0 || k0 + 32 <= v.prefix);
-          bool other = v.codes && khi < 0;
-          if (v.docs) {
-            const i32x4 ts = qtiles[qc / kChunk];
-            other = ts[1] < klo || ts[0] > khi;
-            clean = clean && !ts[2] && ts[0] == ts[1] && klo == khi && ts[0] == klo;
-          } else if (v.codes) {
-            clean = clean && klo == khi;
-          }
-          if (beyond || other) continue;
-          f32x16 sc, dp, tt;
+    for (int t = 0; t < kChunk / 32; ++t) {
+      const int q0 = at.qc + 32 * t;
+      if (q0 >= a.Sq) break;
+      if (q0 + 32 <= wfirst) continue;
+      f32x16 u, dp;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) { sc[r] = 0.f; dp[r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { u[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
-          for (int s = 0; s < 2 * NDB; ++s) {
-            sc = mma(L::row(qt, 32 * t + r32, s, hh), kf[s], sc);
-            dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
-          }
-          const int rel = key - (v.start + q0 + 4 * hh);    // register r: rel - acc_row(r)
-          score_tile<T, -1, true>(sc, tt, sp, tab, rel, rel0 - 31, rel0 + 31);
-          if (!clean) {
+      for (int s = 0; s < 2 * NDB; ++s) {
+        u = mma(L::row(qt, 32 * t + r32, s, hh), kf[s], u);
+        dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
+      }
+      f32x16 g;
+      if (sp.cap) {
+        cap_tile<T>(u, sp);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              bool see = kcode >= 0;
-              if (v.causal) see = see && (rel - acc_row(r) <= 0 || key < v.prefix);
-              if (v.docs) see = see && qc_lds[32 * t + 4 * hh + acc_row(r)] == kcode;
-              if (!see) sc[r] = -INFINITY;
-            }
-          }
+        for (int r = 0; r < 16; ++r) g[r] = cap_slope<T>(u[r]);
+      }
+      float A = sp.A, C = sp.C;
+      const int rel0 = k0 - (v.start + q0), rel = key - (v.start + q0 + 4 * hh);        // register r: rel - acc_row(r)
+      const bool near = sp.tab && rel0 + 31 > -a.R && rel0 - 31 < a.R;
+      if (!clean || sp.slopes || near) {
+        bias_tile<-1>(u, sp, tab, a.R, rel, rel0);
+        if (!clean) {
+          const int from = kcode >= 0 ? first - (q0 + 4 * hh) : INT32_MAX;
 #pragma unroll
-          for (int a4 = 0; a4 < 4; ++a4) {
-            const f32x4 ls = *reinterpret_cast<const f32x4*>(lses + 32 * t + 8 * a4 + 4 * hh);
-            const f32x4 de = *reinterpret_cast<const f32x4*>(dels + 32 * t + 8 * a4 + 4 * hh);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 4 * a4 + i;
-              sc[r] = __builtin_amdgcn_exp2f(sc[r] - ls[i]);
-              dp[r] = sc[r] * (dp[r] - de[i]);
-              if (sp.cap) dp[r] *= 1.f - tt[r] * tt[r];
-            }
-          }
-          typename Frag<T>::type p0, p1, d0, d1;
-          pack8(p0, sc, 0);
-          pack8(p1, sc, 1);
-          pack8(d0, dp, 0);
-          pack8(d1, dp, 1);
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) {
-            dv[db] = mma(L::col(dt, 32 * t, db, lane), p0, dv[db]);
-            dv[db] = mma(L::col(dt, 32 * t + 16, db, lane), p1, dv[db]);
-            dk[db] = mma(L::col(qt, 32 * t, db, lane), d0, dk[db]);
-            dk[db] = mma(L::col(qt, 32 * t + 16, db, lane), d1, dk[db]);
+          for (int r = 0; r < 16; ++r) {
+            bool see = acc_row(r) >= from;
+            if (v.docs) see = see && qcs[32 * t + 4 * hh + acc_row(r)] == kcode;
+            u[r] = see ? u[r] : -INFINITY;
           }
         }
+        A = 1.f;
+        C = 0.f;
+      } else if (sp.tab) {
+        C += tab[rel0 < 0 ? 0 : 2 * a.R];
       }
-      qc = qn;
+#pragma unroll
+      for (int a4 = 0; a4 < 4; ++a4) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * t + 8 * a4 + 4 * hh);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(de + 32 * t + 8 * a4 + 4 * hh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * a4 + i;
+          u[r] = __builtin_amdgcn_exp2f(fmaf(A, u[r], C - l4[i]));
+          dp[r] = u[r] * (dp[r] - d4[i]);
+        }
+      }
+      if (sp.cap) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= g[r];
+      }
+      typename Frag<T>::type p0, p1, d0, d1;
+      pack8(p0, u, 0);
+      pack8(p1, u, 1);
+      pack8(d0, dp, 0);
+      pack8(d1, dp, 1);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        dv[db] = mma(L::col(dt, 32 * t, db, lane), p0, dv[db]);
+        dv[db] = mma(L::col(dt, 32 * t + 16, db, lane), p1, dv[db]);
+        dk[db] = mma(L::col(qt, 32 * t, db, lane), d0, dk[db]);
+        dk[db] = mma(L::col(qt, 32 * t + 16, db, lane), d1, dk[db]);
+      }
     }
   }
-  if (ok) {
-    const int64_t at = ((b * a.Sk + key) * a.kv + kvh) * a.d;
-    store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, hh);
+  if (!ok) return;
+  const float out_scale = a.scale * (sp.cap ? cap_slope_factor<T>() : 1.f);
+  const int64_t at = ((b * a.Sk + key) * a.kv + kvh) * a.d;
+  if (part == nullptr) {
+    store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, out_scale, a.d, hh);
     store_row<T, NDB>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, hh);
+  } else {                              // [split][dk, dv][(B, Sk, kv, d)]
+    const int64_t n = (int64_t)a.B * a.Sk * a.kv * a.d;
+    store_row<float, NDB>(part + 2 * share * n + at, dk, out_scale, a.d, hh);
+    store_row<float, NDB>(part + (2 * share + 1) * n + at, dv, 1.f, a.d, hh);
   }
+}
+
+// dk and dv = the shares' partials in order; n4 groups of four values each
+template <typename T>
+__global__ __launch_bounds__(256) void k_ba_fold(const float* part, T* dk, T* dv, int64_t n4, int split) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * n4) return;
+  const bool second = i >= n4;
+  const int64_t e = 4 * (second ? i - n4 : i);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < split; ++k) s += *reinterpret_cast<const f32x4*>(part + (2 * k + (second ? 1 : 0)) * 4 * n4 + e);
+  store4((second ? dv : dk) + e, s[0], s[1], s[2], s[3]);
+}
+
+// Heads of a group on separate blocks until there are four blocks per CU (1024): below that the chip is not filled, or (causal)
+// the longest walks are waited for.  The partials cost 8 bytes per value and share each way.
+int dkv_split(int64_t B, int64_t Sk, int64_t kv, int64_t group) {
+  const int64_t blocks = B * kv * ((Sk + kRows - 1) / kRows);
+  int64_t split = 1;
+  for (int64_t s = 1; s <= group; ++s)
+    if (group % s == 0) {
+      split = s;
+      if (blocks * s >= 1024) break;
+    }
+  return (int)split;
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
-size_t tile_bytes(int es, int ndb) {
-  const int pitch = es == 4 ? 32 * ndb + 4 : (ndb == 1 || ndb == 3 ? 32 * ndb : 32 * ndb + 32);
-  return (size_t)2 * kChunk * pitch * es;
+// LDS of the buffers: two tiles and `words` 4-byte values per row of a chunk
+size_t tile_bytes(int dtype, int d, int words) {
+  const int ndb = (d + 31) / 32, w = 32 * ndb;
+  const int row = dtype == MIVAE_F32 ? (w + 4) * 4 : w * 2;
+  return (size_t)(dtype == MIVAE_F32 ? buffers<float>() : buffers<unsigned short>()) * kChunk * (2 * row + 4 * words);
 }
 
-enum Which { kFwd, kDelta, kDq, kDkv };
-
-template <typename T, int NDB>
-void launch(Which which, const BiasedArgs& a, dim3 grid, size_t lds, hipStream_t st) {
-  void (*fn)(BiasedArgs) = which == kFwd   ? k_ba_fwd<T, NDB>
-                           : which == kDq  ? k_ba_dq<T, NDB, false>
-                           : which == kDkv ? k_ba_dkv<T, NDB>
-                                           : k_ba_dq<unsigned short, NDB, true>;
-  if (lds > 64 * 1024)        // at most 141 KiB: fp32 heads of 128, a table gradient over 2049 distances
-    (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL(fn, grid, dim3(64 * kWaves), lds, st, a);
+template <typename... A>
+void start(void (*fn)(A...), dim3 grid, size_t lds, hipStream_t st, A... args) {
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL(fn, grid, dim3(64 * kWaves), lds, st, args...);
 }
 
-void dispatch(Which which, int dtype, const BiasedArgs& a, dim3 grid, size_t lds, hipStream_t st) {
-  const int ndb = (a.d + 31) / 32;
-  if (dtype == MIVAE_F32) switch (ndb) {
-      case 1: return launch<float, 1>(which, a, grid, lds, st);
-      case 2: return launch<float, 2>(which, a, grid, lds, st);
-      case 3: return launch<float, 3>(which, a, grid, lds, st);
-      default: return launch<float, 4>(which, a, grid, lds, st);
+// f(type tag, std::integral_constant NDB)
+template <typename F>
+void by_shape(int dtype, int d, F f) {
+  using std::integral_constant;
+  const int ndb = (d + 31) / 32;
+  auto by_width = [&](auto tag) {
+    switch (ndb) {
+      case 1: return f(tag, integral_constant<int, 1>());
+      case 2: return f(tag, integral_constant<int, 2>());
+      case 3: return f(tag, integral_constant<int, 3>());
+      default: return f(tag, integral_constant<int, 4>());
     }
-  switch (ndb) {
-    case 1: return launch<unsigned short, 1>(which, a, grid, lds, st);
-    case 2: return launch<unsigned short, 2>(which, a, grid, lds, st);
-    case 3: return launch<unsigned short, 3>(which, a, grid, lds, st);
-    default: return launch<unsigned short, 4>(which, a, grid, lds, st);
-  }
+  };
+  if (dtype == MIVAE_F32) by_width(float());
+  else by_width((unsigned short)0);
 }
 
 int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
@@ -703,7 +866,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
   MIVAE_REQUIRE(x->q && x->k && x->v, "%s: null operand", name);
   MIVAE_REQUIRE(aligned16(x->q) && aligned16(x->k) && aligned16(x->v), "%s: q / k / v must be 16-byte aligned", name);
   MIVAE_REQUIRE(!(x->prefix && !x->causal), "%s: a prefix needs the causal mask", name);
-  MIVAE_REQUIRE(x->softcap >= 0.f && x->softcap < 1e30f && x->scale > -1e30f && x->scale < 1e30f,
+  MIVAE_REQUIRE(x->softcap >= 0.f && x->softcap < 1e30f && x->scale >= 0.f && x->scale < 1e30f,
                 "%s: softcap or scale out of range", name);
   MIVAE_REQUIRE(!(x->slopes && x->table), "%s: slopes and a table are alternatives", name);
   if (x->table)
@@ -722,7 +885,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
   a.nb = (int)x->num_buckets; a.R = x->table ? (int)x->distance : 0;
   a.scale = x->scale; a.cap = x->softcap;
   a.kpad = (int)pad64(a.Sk); a.qpad = (int)pad64(a.Sq);
-  const int64_t nq = (x->batch * x->heads) * ((a.Sq + kRows - 1) / kRows), nk = (x->batch * x->kv_heads) * ((a.Sk + kRows - 1) / kRows);
+  const int64_t nq = (x->batch * x->heads) * ((a.Sq + kRows - 1) / kRows), nk = (x->batch * x->heads) * ((a.Sk + kRows - 1) / kRows);
   MIVAE_REQUIRE(x->batch <= (1 << 24) && nq < (1ll << 31) && nk < (1ll << 31) && x->batch * (a.kpad + a.qpad) / 256 < (1ll << 31),
                 "%s: too many blocks", name);
   if (x->mask || x->documents) {          // [codes][key tiles], and with documents the same of the queries
@@ -748,9 +911,11 @@ int64_t mivae_biased_attention_codes_ints(int64_t batch, int64_t q_len, int64_t 
   return batch * (pad64(k_len) + (documents ? pad64(q_len) : 0)) / 16 * 17;
 }
 
-int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t heads, int64_t num_buckets) {
-  const int64_t nblk = (q_len + kRows - 1) / kRows;
-  return batch * heads * q_len + batch * heads * nblk * num_buckets;
+int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
+                                          int64_t head_size, int64_t num_buckets) {
+  const int64_t nblk = (q_len + kRows - 1) / kRows, split = dkv_split(batch, k_len, kv_heads, heads / kv_heads);
+  return (batch * heads * q_len + 3) / 4 * 4 + (batch * heads * nblk * num_buckets + 3) / 4 * 4 +
+         (split > 1 ? 2 * split * batch * k_len * kv_heads * head_size : 0);
 }
 
 int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
@@ -765,10 +930,9 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
                        const_cast<int*>(a.qcodes), const_cast<i32x4*>(a.ktiles), const_cast<i32x4*>(a.qtiles));
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (codes)");
   }
-  const int ndb = (a.d + 31) / 32, es = x->dtype == MIVAE_F32 ? 4 : 2;
-  const size_t lds = tile_bytes(es, ndb) + kChunk * 4 + (a.table ? (2 * a.R + 1) * 4 : 0);
+  const size_t lds = tile_bytes(x->dtype, a.d, 1) + (a.table ? (2 * a.R + 1) * 4 : 0);
   const dim3 grid((unsigned)((int64_t)a.B * a.heads * ((a.Sq + kRows - 1) / kRows)));
-  dispatch(kFwd, x->dtype, a, grid, lds, S_(stream));
+  by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_fwd<decltype(t), n()>, grid, lds, S_(stream), a); });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd");
   return MIVAE_OK;
 }
@@ -786,25 +950,27 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   MIVAE_REQUIRE(rows / 16 < (1ll << 31), "mivae_biased_attention_bwd: too many rows");
   a.dout = x->dout;
   a.dq = x->dq; a.dk = x->dk; a.dv = x->dv;
-  a.delta = x->scratch;
-  a.dtab = x->dtable ? x->scratch + rows : nullptr;
-  hipStream_t st = S_(stream);
-  const int ndb = (a.d + 31) / 32, es = x->dtype == MIVAE_F32 ? 4 : 2;
-  const size_t tiles = tile_bytes(es, ndb), tw = a.table ? 2 * a.R + 1 : 0;
+  MIVAE_REQUIRE(aligned16(x->scratch), "mivae_biased_attention_bwd: scratch must be 16-byte aligned");
   const int nblk = (a.Sq + kRows - 1) / kRows;
+  a.delta = x->scratch;
+  float* dtab = x->scratch + (rows + 3) / 4 * 4;
+  a.dtab = x->dtable ? dtab : nullptr;
+  float* part = dtab + (x->dtable ? ((int64_t)a.B * a.heads * nblk * a.nb + 3) / 4 * 4 : 0);
+  hipStream_t st = S_(stream);
+  const size_t tw = a.table ? 2 * a.R + 1 : 0, lds = tile_bytes(x->dtype, a.d, 1) + tw * 4;
   const dim3 grid((unsigned)((int64_t)a.B * a.heads * nblk)), dgrid((unsigned)((rows + 15) / 16));
-  if (es == 4)
+  if (x->dtype == MIVAE_F32)
     hipLaunchKernelGGL((k_ba_delta<float>), dgrid, dim3(256), 0, st, static_cast<const float*>(x->dout),
                        static_cast<const float*>(x->out), a.delta, rows, a.Sq, a.heads, a.d);
   else if (!a.dtab)
     hipLaunchKernelGGL((k_ba_delta<unsigned short>), dgrid, dim3(256), 0, st, static_cast<const unsigned short*>(x->dout),
                        static_cast<const unsigned short*>(x->out), a.delta, rows, a.Sq, a.heads, a.d);
   else
-    dispatch(kDelta, x->dtype, a, grid, tiles + (kChunk + tw) * 4, st);
+    by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a); });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (delta)");
   if (a.dq || a.dtab) {
-    const size_t lds = tiles + kChunk * 4 + (tw + (a.dtab ? 2 * kWaves * tw : 0)) * 4;
-    dispatch(kDq, x->dtype, a, grid, lds, st);
+    const size_t more = a.dtab ? 2 * kWaves * tw * 4 : 0;
+    by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_dq<decltype(t), n(), false>, grid, lds + more, st, a); });
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dq)");
     if (a.dtab) {
       hipLaunchKernelGGL(k_ba_dtable, dim3((unsigned)(a.heads * a.nb)), dim3(64), 0, st, a.dtab, x->dtable, (int64_t)a.B * nblk,
@@ -813,10 +979,22 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     }
   }
   if (a.dk) {
-    const size_t lds = tiles + 3 * kChunk * 4 + tw * 4;
-    const dim3 grid((unsigned)((int64_t)a.B * a.kv * ((a.Sk + kRows - 1) / kRows)));
-    dispatch(kDkv, x->dtype, a, grid, lds, st);
+    const int split = dkv_split(a.B, a.Sk, a.kv, a.group);
+    const dim3 kgrid((unsigned)((int64_t)a.B * a.kv * split * ((a.Sk + kRows - 1) / kRows)));
+    float* shares = split > 1 ? part : nullptr;
+    by_shape(x->dtype, a.d,
+             [&](auto t, auto n) { start(k_ba_dkv<decltype(t), n()>, kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, split, shares); });
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dk, dv)");
+    if (shares) {
+      const int64_t n4 = (int64_t)a.B * a.Sk * a.kv * a.d / 4;
+      const dim3 fgrid((unsigned)((2 * n4 + 255) / 256));
+      if (x->dtype == MIVAE_F32)
+        hipLaunchKernelGGL((k_ba_fold<float>), fgrid, dim3(256), 0, st, shares, static_cast<float*>(a.dk), static_cast<float*>(a.dv), n4, split);
+      else
+        hipLaunchKernelGGL((k_ba_fold<unsigned short>), fgrid, dim3(256), 0, st, shares, static_cast<unsigned short*>(a.dk),
+                           static_cast<unsigned short*>(a.dv), n4, split);
+      MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (fold)");
+    }
   }
   return MIVAE_OK;
 }

@@ -479,8 +479,8 @@ class _BiasedAttention(torch.autograd.Function):
         if need_k or need_v:
             dk, dv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(v.shape, dtype=q.dtype, device=dev)
         dtable = torch.empty_like(table) if need_t else None
-        scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.heads,
-                                           a.num_buckets if need_t else 0), dtype=torch.float32, device=dev)
+        scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.k_len, a.heads,
+                                           a.kv_heads, a.head_size, a.num_buckets if need_t else 0), dtype=torch.float32, device=dev)
         args = _refill(a, q=q, k=k, v=v, table=table, mask=mask, documents=documents, prefix=prefix, q_starts=q_starts,
                        slopes=slopes, buckets=buckets, codes=codes, out=out, lse=lse, dout=dout, dq=dq, dk=dk, dv=dv,
                        dtable=dtable, scratch=scratch)
@@ -535,7 +535,7 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     if softcap is not None and not 0 < softcap < 1e30:
         raise ValueError(f"biased_attention: softcap {softcap}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not abs(scale) < 1e30:
+    if not 0 <= scale < 1e30:
         raise ValueError(f"biased_attention: scale {scale}")
     args = L.AttentionArgs(batch=B, q_len=Sq, k_len=Sk, heads=heads, kv_heads=kv_heads, head_size=d, q_stride=qst,
                            k_stride=kst, v_stride=vst, scale=scale, softcap=softcap or 0.0, causal=int(bool(causal)),

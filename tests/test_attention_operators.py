@@ -467,7 +467,7 @@ def test_attention_refusals(monkeypatch):
         (dict(table=z(8, 4), buckets=i32(4)), "odd length"), (dict(table=z(8, 4), buckets=i32(2051)), "odd length"),
         (dict(table=z(8, 4), buckets=z(5)), "odd length"),
         (dict(softcap=0.0), "softcap"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
-        (dict(softcap=float("inf")), "softcap"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+        (dict(softcap=float("inf")), "softcap"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=-0.5), "scale"),
         (dict(q=z(2, 10, 64)), "start at position -1"), (dict(q_start=-1), "start at position"),
         (dict(q_start=4, documents=i32(2, 9)), "documents reach"), (dict(q_start=z(2)), "q_start must be"),
         (dict(q_start=i32(3)), "q_start must be"),
