@@ -29,7 +29,7 @@ struct BiasedArgs {
   void *dq, *dk, *dv;           // contiguous, may be null
   float* dtab;                  // bucket partials (heads, B * q blocks, nb), or null
   // visibility codes, or null: a pair is seen iff the codes are equal.  Keys: document id (0 without documents), -1 where
-  // hidden.  Queries: document id, kNoCode where it is negative.  tiles: {lowest, highest visible code, any hidden, 0} per 64
+  // hidden.  Queries: document id, kNoCode where it is negative.  tiles: {lowest, highest visible code, visible rows} per 64
   const int *kcodes, *qcodes;
   const i32x4 *ktiles, *qtiles;
   const int *prefix, *q_starts;
@@ -83,10 +83,10 @@ struct Tile<unsigned short, NDB> {
   static constexpr int W = 32 * NDB;
   static constexpr int PITCH = W;
   static constexpr int GE = 8, GPR = W / GE;
-  static __device__ __forceinline__ int at(int r, int c) {
-    const int x = NDB == 4 ? (r & 3) << 2 | ((r >> 2) & 3) : NDB == 2 ? (r & 2) << 1 | ((r >> 2) & 3) : (r >> 2) & 3;
-    return r * PITCH + ((c ^ x) << 3);
+  static __device__ __forceinline__ int swizzle(int r) {
+    return NDB == 4 ? (r & 3) << 2 | ((r >> 2) & 3) : NDB == 2 ? (r & 2) << 1 | ((r >> 2) & 3) : (r >> 2) & 3;
   }
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ swizzle(r)) << 3); }
   // f[j] = tile[r][16 s + 8 hh + j]
   static __device__ __forceinline__ bf16x8 row(const unsigned short* t, int r, int s, int hh) {
     return *reinterpret_cast<const bf16x8*>(t + at(r, 2 * s + hh));
@@ -140,27 +140,52 @@ __device__ __forceinline__ void load_row(typename Frag<T>::type (&f)[2 * NDB], c
   }
 }
 
-// kChunk rows of one head on their way global -> registers -> LDS tile, by 64 NW threads.  Rows at or beyond `rows`, rows
-// whose code is negative (hidden keys: whatever they hold must not meet a product, 0 * NaN is NaN) and columns beyond d
-// arrive as zeros.
+// kChunk rows of one head on their way into an LDS tile, by 64 NW threads.  Rows whose bit of `rows` is 0 (beyond the end, or
+// hidden keys: whatever they hold must not meet a product, 0 * NaN is NaN) and columns beyond d arrive as zeros.
+//   bf16: global_load_lds, 16 bytes per lane into 64 consecutive granules of the tile.  The swizzle is on the global side (the
+//         lane at position `pos` of row r fetches granule pos ^ x(r)), a zero granule is fetched from kZero16, no registers
+//         are held while the loads travel.  land() waits for them; a barrier has to follow.
+//   fp32: through registers (the padded tile is not linear); land() needs the tile consumed by everybody.
+static __device__ const i32x4 kZero16[1] = {{0, 0, 0, 0}};
+
+__device__ __forceinline__ uint64_t low_rows(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
 template <typename T, int NDB, int NW>
-struct Stage {
-  using L = Tile<T, NDB>;
-  static constexpr int N = kChunk * L::GPR / (64 * NW);
-  static_assert(kChunk * L::GPR % (64 * NW) == 0, "a whole number of granules per thread");
-  i32x4 r[N];
-  __device__ __forceinline__ void load(const T* src, int64_t sr, int row0, int rows, int d, const int* codes) {
+struct Stage;
+
+template <int NDB, int NW>
+struct Stage<unsigned short, NDB, NW> {
+  using L = Tile<unsigned short, NDB>;
+  static constexpr int NBUF = 2, N = L::GPR / NW;
+  static_assert(L::GPR % NW == 0, "whole waves of granules");
+  __device__ __forceinline__ void issue(unsigned short* tile, const unsigned short* src, int64_t sr, int row0, uint64_t rows, int d) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = threadIdx.x + i * 64 * NW, row = row0 + idx / L::GPR, c = idx % L::GPR;
-      const i32x4 z = {0, 0, 0, 0};
-      r[i] = z;
-      bool ok = row < rows && c * L::GE < d;
-      if (codes != nullptr) ok = ok && codes[row] >= 0;       // codes are padded to whole chunks
-      if (ok) r[i] = *reinterpret_cast<const i32x4*>(src + (int64_t)row * sr + c * L::GE);
+      const int first = (i * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64, g = first + (threadIdx.x & 63);
+      const int row = g / L::GPR, c = (g % L::GPR) ^ L::swizzle(row);
+      const bool ok = ((rows >> row) & 1) && c * L::GE < d;
+      const void* p = ok ? (const void*)(src + (int64_t)(row0 + row) * sr + c * L::GE) : (const void*)kZero16;
+      const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned short*)(tile + first * L::GE);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory", "m0");
     }
   }
-  __device__ __forceinline__ void store(T* tile) const {
+  __device__ __forceinline__ void land(unsigned short*) { __builtin_amdgcn_s_waitcnt(0x0f70); }       // vmcnt(0)
+};
+
+template <int NDB, int NW>
+struct Stage<float, NDB, NW> {
+  using L = Tile<float, NDB>;
+  static constexpr int NBUF = 1, N = kChunk * L::GPR / (64 * NW);
+  i32x4 r[N];
+  __device__ __forceinline__ void issue(float*, const float* src, int64_t sr, int row0, uint64_t rows, int d) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = threadIdx.x + i * 64 * NW, row = idx / L::GPR, c = idx % L::GPR;
+      r[i] = i32x4{0, 0, 0, 0};
+      if (((rows >> row) & 1) && c * L::GE < d) r[i] = *reinterpret_cast<const i32x4*>(src + (int64_t)(row0 + row) * sr + c * L::GE);
+    }
+  }
+  __device__ __forceinline__ void land(float* tile) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int idx = threadIdx.x + i * 64 * NW, row = idx / L::GPR, c = idx % L::GPR;

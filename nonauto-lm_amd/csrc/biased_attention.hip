@@ -24,18 +24,12 @@ namespace {
 
 static inline hipStream_t S_(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-typedef __attribute__((address_space(3))) float lds_float;
-
 constexpr float kSlack = 8.f;       // exponent slack before the accumulators are rescaled
 constexpr int kWaves = 4, kRows = 32 * kWaves;      // rows (queries or keys) of a block
-// LDS buffers of the streamed tiles: two overlap the stores with the products; fp32 tiles are twice as large, the products
-// eight times as slow, and one buffer leaves room for the table gradient's arrays (141 of 160 KiB at d = 128, R = 1024)
-template <typename T>
-constexpr int buffers() { return sizeof(T) == 4 ? 1 : 2; }
 constexpr int kMaxDistance = 1024, kMaxBuckets = 256;
 
 // ---- visibility codes ------------------------------------------------------------------------------------------------
-// One wave per 64 keys (or queries): code per row and {lowest, highest visible code, any hidden} per 64 rows.
+// One wave per 64 keys (or queries): code per row and {lowest, highest visible code, visible rows as 64 bits} per 64 rows.
 __global__ __launch_bounds__(256) void k_ba_codes(const int64_t* mask, const int* documents, const int* q_starts, int q_start,
                                                   int B, int Sq, int Sk, int kpad, int qpad, int* kcodes, int* qcodes,
                                                   i32x4* ktiles, i32x4* qtiles) {
@@ -68,9 +62,9 @@ __global__ __launch_bounds__(256) void k_ba_codes(const int64_t* mask, const int
     lo = min(lo, __shfl_xor(lo, off, 64));
     hi = max(hi, __shfl_xor(hi, off, 64));
   }
-  const bool hidden = __builtin_amdgcn_ballot_w64(!seen) != 0;
+  const uint64_t rows = __builtin_amdgcn_ballot_w64(seen);
   if (lane == 0) {
-    const i32x4 s = {lo, hi, hidden ? 1 : 0, 0};
+    const i32x4 s = {lo, hi, (int)(unsigned)rows, (int)(unsigned)(rows >> 32)};
     if (keys) ktiles[b * nkt + t] = s;
     else qtiles[b * nqt + (t - nkt)] = s;
   }
@@ -134,8 +128,9 @@ __device__ __forceinline__ void wave_range(int code, int& lo, int& hi) {
 }
 
 __device__ __forceinline__ i32x4 merge(const i32x4& a, const i32x4& b) {
-  return i32x4{min(a[0], b[0]), max(a[1], b[1]), a[2] | b[2], 0};
+  return i32x4{min(a[0], b[0]), max(a[1], b[1]), 0, 0};
 }
+__device__ __forceinline__ uint64_t rows_of(const i32x4& t) { return (uint64_t)(unsigned)t[3] << 32 | (unsigned)t[2]; }
 
 // The walk of a block of queries over the keys in chunks of kChunk, shared by the forward and the dq kernel.
 struct KeyWalk {
@@ -150,6 +145,9 @@ struct KeyWalk {
         kc += kChunk;
       }
     return kc;
+  }
+  __device__ __forceinline__ uint64_t rows(int kc, int Sk) const {       // the keys of a chunk that are not hidden
+    return tiles != nullptr ? rows_of(tiles[kc / kChunk]) : low_rows(Sk - kc);
   }
 };
 
@@ -181,7 +179,7 @@ struct QueryWave {
     if (w.tiles != nullptr) {
       const i32x4 t = w.tiles[kc / kChunk];
       if (t[1] < lo || t[0] > hi) return 0;
-      all = all && !t[2] && !none && lo == hi && t[0] == lo && t[1] == lo;
+      all = all && rows_of(t) == ~0ull && !none && lo == hi && t[0] == lo && t[1] == lo;
     }
     return all ? 2 : 1;
   }
@@ -222,34 +220,60 @@ __device__ __forceinline__ void hide_keys(f32x16& u, const QueryWave& w, bool co
 struct Ids {
   int64_t b;
   int head, blk;
+  bool none;
 };
-// Block id -> (batch row, head, block of rows): all heads' blocks of one position before the next position.  Ids go round the
-// eight XCDs, so with a multiple of eight (batch row, head) pairs all blocks of a pair share one L2; and the blocks with the
-// longest walks (last queries, first keys under a causal mask) start first.
-__device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool last_first) {
+// Block id -> (batch row, head, block of rows).  Blocks go round the eight XCDs, each with an L2 of its own.
+//   From 32 (batch row, head) pairs, or a multiple of 8, on: an XCD takes a contiguous run of pairs, so that the blocks of a
+//   pair (and the heads of a group) read their keys through one L2.  The grid is rounded up to a multiple of 8; ids beyond
+//   the last pair do nothing.  (64 x 512 tokens, 4 heads of 128: 69 instead of 133 us forward.)
+//   Fewer pairs, or a causal mask over pairs that do not divide by 8: the position is the slow index, which spreads every
+//   pair over the XCDs.
+// A causal mask makes the blocks' walks unequal: the longest (last queries, first keys) start first, over as many pairs at a
+// time as keep an XCD's 32 CUs busy four times over, and the short ones fill the end.  (4 x 16 x 4096 queries: 263
+// instead of 317 us forward with pair after pair.)
+__host__ __device__ __forceinline__ bool by_xcd(int64_t pairs, bool causal) { return pairs % 8 == 0 || (!causal && pairs >= 32); }
+int64_t grid_of(int64_t pairs, int64_t nblk, bool causal) { return by_xcd(pairs, causal) ? (pairs * nblk + 7) / 8 * 8 : pairs * nblk; }
+
+__device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool causal, bool last_first) {
   Ids r;
-  const unsigned bhs = (unsigned)B * (unsigned)heads, id = blockIdx.x;
-  r.blk = (int)(id / bhs);
+  const unsigned pairs = (unsigned)B * (unsigned)heads, n = (unsigned)nblk;
+  unsigned bh;
+  r.none = false;
+  if (by_xcd(pairs, causal)) {
+    const unsigned x = blockIdx.x & 7, i = blockIdx.x >> 3, each = gridDim.x >> 3;
+    if (causal) {
+      const unsigned mine = pairs / 8, most = min(mine, (255 + n) / n), g = i / (most * n), j = i % (most * n);
+      const unsigned size = min(most, mine - g * most);
+      bh = x * mine + g * most + j % size;
+      r.blk = (int)(j / size);
+    } else {
+      const unsigned w = x * each + i;
+      bh = w / n;
+      r.blk = (int)(w % n);
+      r.none = bh >= pairs;
+    }
+  } else {
+    r.blk = (int)(blockIdx.x / pairs);
+    bh = blockIdx.x % pairs;
+  }
   if (last_first) r.blk = nblk - 1 - r.blk;
-  const unsigned bh = id % bhs;
   r.head = (int)(bh % (unsigned)heads);
   r.b = bh / (unsigned)heads;
   return r;
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-// Chunks go through two LDS buffers: the next one is stored and the one after it is on its way while a chunk is multiplied,
-// one barrier per chunk.
 template <typename T, int NDB>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(BiasedArgs a) {
   using L = Tile<T, NDB>;
-  constexpr int TW = kChunk / 32, TILE = kChunk * L::PITCH, NBUF = buffers<T>();
+  constexpr int TW = kChunk / 32, TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][K, V]
   int* kc_lds = reinterpret_cast<int*>(tiles + 2 * NBUF * TILE);          // [NBUF][kChunk]
   float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const Ids id = ids_of(a.B, a.heads, (a.Sq + kRows - 1) / kRows, true);
+  const Ids id = ids_of(a.B, a.heads, (a.Sq + kRows - 1) / kRows, a.causal != 0, true);
+  if (id.none) return;
   const int64_t b = id.b;
   const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
@@ -269,38 +293,26 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   float m = -__FLT_MAX__, l = 0.f;
+  // Two LDS buffers with bf16: the next chunk is on its way while one is multiplied, one barrier per chunk.
   Stage<T, NDB, kWaves> sk, sv;
   int pc = 0, buf = 0;
-  auto load = [&](int kc) {
-    sk.load(kbase, a.ks[1], kc, a.Sk, a.d, codes);
-    sv.load(vbase, a.vs[1], kc, a.Sk, a.d, codes);
+  auto issue = [&](int n, int kc) {
+    const uint64_t rows = walk.rows(kc, a.Sk);
+    sk.issue(tiles + 2 * n * TILE, kbase, a.ks[1], kc, rows, a.d);
+    sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  auto store = [&](int n) {
-    sk.store(tiles + 2 * n * TILE);
-    sv.store(tiles + (2 * n + 1) * TILE);
-    if (v.codes && threadIdx.x < kChunk) kc_lds[n * kChunk + threadIdx.x] = pc;
-  };
-  int kc = walk.next(0), kn = kc;       // the chunk to multiply, the chunk in the registers
-  if (kc < walk.end) load(kc);
-  if (NBUF == 2 && kc < walk.end) {
-    store(0);
-    kn = walk.next(kc + kChunk);
-    if (kn < walk.end) load(kn);
-  }
+  int kc = walk.next(0);
+  if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
-    __syncthreads();                    // this chunk is stored, the previous one consumed
+    if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
+    sk.land(tiles + 2 * buf * TILE);
+    sv.land(tiles + (2 * buf + 1) * TILE);
+    if (v.codes && threadIdx.x < kChunk) kc_lds[buf * kChunk + threadIdx.x] = pc;
+    __syncthreads();
     const int at = kc;
-    if (NBUF == 1) {
-      store(0);
-      __syncthreads();
-    } else if (kn < walk.end) {
-      store(buf ^ 1);
-    }
-    const int ahead = kn < walk.end ? walk.next(kn + kChunk) : kn;
-    if (ahead < walk.end) load(ahead);
-    kc = NBUF == 1 ? ahead : kn;
-    kn = ahead;
+    kc = walk.next(kc + kChunk);
+    if (kc < walk.end) issue(buf ^ (NBUF - 1), kc);
     const int sees = qw.sees(walk, at); // wave-uniform, like every branch below
     if (sees == 0) continue;
     const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
@@ -378,10 +390,11 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 }
 
 // ---- backward: dq and the table's gradient ---------------------------------------------------------------------------
-// The table's gradient sums ds along diagonals.  Every wave has two LDS arrays by relative distance, one per half-wave, and
-// adds with ds_add_f32: the lanes of a half-wave hold 32 queries, so within one instruction they hit 32 different
-// distances, and a wave's LDS instructions keep their order -- the sums have one order, from run to run.  Distances at or
-// beyond R go to two registers instead.  The block then folds its eight arrays by bucket into one partial row.
+// The table's gradient sums ds along the diagonals of the tiles.  A wave writes its tile into LDS skewed, query q's value at
+// distance x into column x + 31 of row q (64 columns; the corners keep their zeros), lane c sums column c and adds it to the
+// wave's array by relative distance: every sum has one order, from run to run.  (LDS float atomics, 16 per tile, took
+// 190 cycles each: 686 us instead of the SKEW_US at 4 x 16 x 4096^2.)  Tiles at or beyond distance R go to two
+// registers instead.  The block then folds its four arrays by bucket into one partial row.
 //
 // DELTA: the first half of the same walk, delta_i = sum_j p_ij (do_i . v_j), instead of dout . out.  Needed by the table's
 // gradient on bf16 operands: the o of the forward carries the rounding of P (2^-9 of it, as does its own), which averages
@@ -389,14 +402,15 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 template <typename T, int NDB, bool DELTA>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a) {
   using L = Tile<T, NDB>;
-  constexpr int TILE = kChunk * L::PITCH, NBUF = buffers<T>();
+  constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][K, V]
   int* kc_lds = reinterpret_cast<int*>(tiles + 2 * NBUF * TILE);          // [NBUF][kChunk]
   float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
   const int nblk = (a.Sq + kRows - 1) / kRows;
-  const Ids id = ids_of(a.B, a.heads, nblk, true);
+  const Ids id = ids_of(a.B, a.heads, nblk, a.causal != 0, true);
+  if (id.none) return;
   const int64_t b = id.b;
   const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
@@ -404,12 +418,15 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   const QueryWave qw = query_wave(a, v, b, q0, r32);
   const Score sp = score_of(a, head, sizeof(T) == 4);
   const int TW = 2 * a.R + 1;
-  float* hist = tab + TW;                            // [2 kWaves][TW]
-  float* mine = hist + (2 * wave + hh) * TW;
+  float* hist = tab + TW;                                                 // [kWaves][TW]
+  float* mine = hist + wave * TW;
+  float* skew = hist + kWaves * TW + wave * 32 * 64;                      // [kWaves][32][64]
   const bool grad_tab = !DELTA && a.dtab != nullptr;
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
-  if (grad_tab)
-    for (int i = threadIdx.x; i < 2 * kWaves * TW; i += 64 * kWaves) hist[i] = 0.f;
+  if (grad_tab) {
+    for (int i = threadIdx.x; i < kWaves * TW; i += 64 * kWaves) hist[i] = 0.f;
+    for (int i = lane; i < 32 * 64; i += 64) skew[i] = 0.f;
+  }
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
@@ -428,36 +445,23 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   float far_lo = 0.f, far_hi = 0.f;
   Stage<T, NDB, kWaves> sk, sv;
   int pc = 0, buf = 0;
-  auto load = [&](int kc) {
-    sk.load(kbase, a.ks[1], kc, a.Sk, a.d, codes);
-    sv.load(vbase, a.vs[1], kc, a.Sk, a.d, codes);
+  auto issue = [&](int n, int kc) {
+    const uint64_t rows = walk.rows(kc, a.Sk);
+    sk.issue(tiles + 2 * n * TILE, kbase, a.ks[1], kc, rows, a.d);
+    sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  auto store = [&](int n) {
-    sk.store(tiles + 2 * n * TILE);
-    sv.store(tiles + (2 * n + 1) * TILE);
-    if (v.codes && threadIdx.x < kChunk) kc_lds[n * kChunk + threadIdx.x] = pc;
-  };
-  int kc = walk.next(0), kn = kc;       // the chunk to multiply, the chunk in the registers
-  if (kc < walk.end) load(kc);
-  if (NBUF == 2 && kc < walk.end) {
-    store(0);
-    kn = walk.next(kc + kChunk);
-    if (kn < walk.end) load(kn);
-  }
+  int kc = walk.next(0);
+  if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
+    if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
+    sk.land(tiles + 2 * buf * TILE);
+    sv.land(tiles + (2 * buf + 1) * TILE);
+    if (v.codes && threadIdx.x < kChunk) kc_lds[buf * kChunk + threadIdx.x] = pc;
     __syncthreads();
     const int at = kc;
-    if (NBUF == 1) {
-      store(0);
-      __syncthreads();
-    } else if (kn < walk.end) {
-      store(buf ^ 1);
-    }
-    const int ahead = kn < walk.end ? walk.next(kn + kChunk) : kn;
-    if (ahead < walk.end) load(ahead);
-    kc = NBUF == 1 ? ahead : kn;
-    kn = ahead;
+    kc = walk.next(kc + kChunk);
+    if (kc < walk.end) issue(buf ^ (NBUF - 1), kc);
     const int sees = qw.sees(walk, at);
     if (sees == 0) continue;
     const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
@@ -506,18 +510,18 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
           for (int r = 0; r < 16; ++r) s += u[r];
           if (rel0 < 0) far_lo += s;
           else far_hi += s;
-        } else if (rel0 - 31 > -a.R && rel0 + 31 < a.R) {
-          lds_float* h = (lds_float*)(mine + rel + a.R);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) __builtin_amdgcn_ds_faddf(h + acc_row(r), u[r], 0, 0, false);
         } else {
+          float* w = skew + r32 * 63 + 4 * hh + 31;                       // row r32, column key - query + 31
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int x = rel + acc_row(r);
-            if (x <= -a.R) far_lo += u[r];
-            else if (x >= a.R) far_hi += u[r];
-            else __builtin_amdgcn_ds_faddf((lds_float*)(mine + x + a.R), u[r], 0, 0, false);
-          }
+          for (int r = 0; r < 16; ++r) w[acc_row(r)] = u[r];
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 32; ++q) s[q & 3] += skew[q * 64 + lane];
+          const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+          const int x = rel0 - 31 + lane;
+          if (x <= -a.R) far_lo += sum;
+          else if (x >= a.R) far_hi += sum;
+          else mine[x + a.R] += sum;
         }
       }
       if (sp.cap) {
@@ -542,13 +546,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   const float out_scale = a.scale * (sp.cap ? cap_slope_factor<T>() : 1.f);
   if (live && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, out_scale, a.d, hh);
   if (grad_tab) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      far_lo += __shfl_xor(far_lo, off, 64);
-      far_hi += __shfl_xor(far_hi, off, 64);
-    }
+    far_lo = group_sum(far_lo, 64);
+    far_hi = group_sum(far_hi, 64);
     __syncthreads();          // the arrays are zeroed also where no chunk was walked
-    if (r32 == 0) {
+    if (lane == 0) {
       mine[0] = far_lo;
       mine[2 * a.R] = far_hi;
     }
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     int* ids = reinterpret_cast<int*>(tab);
     for (int i = threadIdx.x; i < TW; i += 64 * kWaves) {
       float s = 0.f;
-      for (int w = 0; w < 2 * kWaves; ++w) s += hist[w * TW + i];
+      for (int w = 0; w < kWaves; ++w) s += hist[w * TW + i];
       hist[i] = s;
       ids[i] = min(max(a.buckets[i], 0), a.nb - 1);
     }
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(64) void k_ba_dtable(const float* part, float* dtab
 template <typename T, int NDB>
 __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, float* part) {
   using L = Tile<T, NDB>;
-  constexpr int TILE = kChunk * L::PITCH, NBUF = buffers<T>();
+  constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][Q, dO]
   float* lses = reinterpret_cast<float*>(tiles + 2 * NBUF * TILE);        // [NBUF][kChunk] each
@@ -598,7 +599,8 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   int* qc_lds = reinterpret_cast<int*>(dels + NBUF * kChunk);
   float* tab = reinterpret_cast<float*>(qc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const Ids id = ids_of(a.B, a.kv * split, (a.Sk + kRows - 1) / kRows, false);
+  const Ids id = ids_of(a.B, a.kv * split, (a.Sk + kRows - 1) / kRows, a.causal != 0, false);
+  if (id.none) return;
   const int64_t b = id.b;
   const int kvh = id.head / split, share = id.head % split, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
   const View v = view_of(a, b);
@@ -648,62 +650,48 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   Stage<T, NDB, kWaves> sq, sd;
   float pl = 0.f, pd = 0.f;
   int pq = 0, buf = 0;
-  auto load = [&](Pos p) {
+  auto issue = [&](int n, Pos p) {
     const int head = kvh * a.group + p.g;
-    sq.load(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, a.Sq, a.d, nullptr);
-    sd.load(static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d, (int64_t)a.heads * a.d, p.qc, a.Sq, a.d, nullptr);
+    const uint64_t rows = low_rows(a.Sq - p.qc);
+    sq.issue(tiles + 2 * n * TILE, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, rows, a.d);
+    sd.issue(tiles + (2 * n + 1) * TILE, static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d,
+             (int64_t)a.heads * a.d, p.qc, rows, a.d);
     const int i = p.qc + (int)threadIdx.x;
     const bool in = threadIdx.x < kChunk && i < a.Sq;
     pl = in ? a.lse[(b * a.heads + head) * a.Sq + i] : INFINITY;    // rows beyond Sq: p = exp2(. - inf) = 0
     pd = in ? a.delta[(b * a.heads + head) * a.Sq + i] : 0.f;
     if (v.docs && threadIdx.x < kChunk) pq = a.qcodes[b * a.qpad + i];
   };
-  auto store = [&](int n) {
-    sq.store(tiles + 2 * n * TILE);
-    sd.store(tiles + (2 * n + 1) * TILE);
-    if (threadIdx.x < kChunk) {
-      lses[n * kChunk + threadIdx.x] = pl;
-      dels[n * kChunk + threadIdx.x] = pd;
-      qc_lds[n * kChunk + threadIdx.x] = pq;
-    }
-  };
-  Pos p = settle(Pos{share * a.group / split, qfirst}), pn = p;          // to multiply, in the registers
-  if (p.g < glast) load(p);
-  if (NBUF == 2 && p.g < glast) {
-    store(0);
-    pn = settle(Pos{p.g, p.qc + kChunk});
-    if (pn.g < glast) load(pn);
-  }
+  Pos p = settle(Pos{share * a.group / split, qfirst});
+  if (p.g < glast) issue(0, p);
   int tab_head = -1;
   Score sp = score_of(a, kvh * a.group, sizeof(T) == 4);
   for (; p.g < glast; buf ^= NBUF - 1) {
     const Pos at = p;
     const int head = kvh * a.group + at.g;
-    __syncthreads();
-    if (head != tab_head) {             // block-uniform: another head's bias
+    const bool other_head = head != tab_head;                             // block-uniform: another head's bias
+    if (NBUF == 1 || (other_head && sp.tab)) __syncthreads();             // the previous chunk has been consumed
+    sq.land(tiles + 2 * buf * TILE);
+    sd.land(tiles + (2 * buf + 1) * TILE);
+    if (threadIdx.x < kChunk) {
+      lses[buf * kChunk + threadIdx.x] = pl;
+      dels[buf * kChunk + threadIdx.x] = pd;
+      qc_lds[buf * kChunk + threadIdx.x] = pq;
+    }
+    if (other_head) {
       sp = score_of(a, head, sizeof(T) == 4);
       tab_head = head;
-      if (sp.tab) {
-        stage_table(tab, a, head, 64 * kWaves);
-        __syncthreads();
-      }
+      if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
     }
-    if (NBUF == 1) {
-      store(0);
-      __syncthreads();
-    } else if (pn.g < glast) {
-      store(buf ^ 1);
-    }
-    const Pos ahead = pn.g < glast ? settle(Pos{pn.g, pn.qc + kChunk}) : pn;
-    if (ahead.g < glast) load(ahead);
-    p = NBUF == 1 ? ahead : pn;
-    pn = ahead;
+    __syncthreads();
+    p = settle(Pos{p.g, p.qc + kChunk});
+    if (p.g < glast) issue(buf ^ (NBUF - 1), p);
     if (k0 >= a.Sk || at.qc + kChunk <= wfirst) continue;
     bool clean = !khid && at.qc >= wall;
     if (v.docs) {
       const i32x4 ts = qtiles[at.qc / kChunk];
       if (ts[1] < klo || ts[0] > khi) continue;
-      clean = clean && !ts[2] && ts[0] == ts[1] && klo == khi && ts[0] == klo;
+      clean = clean && rows_of(ts) == ~0ull && ts[0] == ts[1] && klo == khi && ts[0] == klo;
     } else if (v.codes && khi < 0) {
       continue;
     }
@@ -817,11 +805,11 @@ int dkv_split(int64_t B, int64_t Sk, int64_t kv, int64_t group) {
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
-// LDS of the buffers: two tiles and `words` 4-byte values per row of a chunk
+// LDS of the buffers (two with bf16, one with fp32): two tiles and `words` 4-byte values per row of a chunk
 size_t tile_bytes(int dtype, int d, int words) {
   const int ndb = (d + 31) / 32, w = 32 * ndb;
   const int row = dtype == MIVAE_F32 ? (w + 4) * 4 : w * 2;
-  return (size_t)(dtype == MIVAE_F32 ? buffers<float>() : buffers<unsigned short>()) * kChunk * (2 * row + 4 * words);
+  return (size_t)(dtype == MIVAE_F32 ? 1 : 2) * kChunk * (2 * row + 4 * words);
 }
 
 template <typename... A>
@@ -886,7 +874,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
   a.scale = x->scale; a.cap = x->softcap;
   a.kpad = (int)pad64(a.Sk); a.qpad = (int)pad64(a.Sq);
   const int64_t nq = (x->batch * x->heads) * ((a.Sq + kRows - 1) / kRows), nk = (x->batch * x->heads) * ((a.Sk + kRows - 1) / kRows);
-  MIVAE_REQUIRE(x->batch <= (1 << 24) && nq < (1ll << 31) && nk < (1ll << 31) && x->batch * (a.kpad + a.qpad) / 256 < (1ll << 31),
+  MIVAE_REQUIRE(x->batch <= (1 << 24) && nq < (1ll << 31) - 8 && nk < (1ll << 31) - 8 && x->batch * (a.kpad + a.qpad) / 256 < (1ll << 31),
                 "%s: too many blocks", name);
   if (x->mask || x->documents) {          // [codes][key tiles], and with documents the same of the queries
     int* p = static_cast<int*>(x->codes);
@@ -931,7 +919,7 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (codes)");
   }
   const size_t lds = tile_bytes(x->dtype, a.d, 1) + (a.table ? (2 * a.R + 1) * 4 : 0);
-  const dim3 grid((unsigned)((int64_t)a.B * a.heads * ((a.Sq + kRows - 1) / kRows)));
+  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, (a.Sq + kRows - 1) / kRows, a.causal));
   by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_fwd<decltype(t), n()>, grid, lds, S_(stream), a); });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd");
   return MIVAE_OK;
@@ -958,7 +946,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   float* part = dtab + (x->dtable ? ((int64_t)a.B * a.heads * nblk * a.nb + 3) / 4 * 4 : 0);
   hipStream_t st = S_(stream);
   const size_t tw = a.table ? 2 * a.R + 1 : 0, lds = tile_bytes(x->dtype, a.d, 1) + tw * 4;
-  const dim3 grid((unsigned)((int64_t)a.B * a.heads * nblk)), dgrid((unsigned)((rows + 15) / 16));
+  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, nblk, a.causal)), dgrid((unsigned)((rows + 15) / 16));
   if (x->dtype == MIVAE_F32)
     hipLaunchKernelGGL((k_ba_delta<float>), dgrid, dim3(256), 0, st, static_cast<const float*>(x->dout),
                        static_cast<const float*>(x->out), a.delta, rows, a.Sq, a.heads, a.d);
@@ -969,7 +957,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a); });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (delta)");
   if (a.dq || a.dtab) {
-    const size_t more = a.dtab ? 2 * kWaves * tw * 4 : 0;
+    const size_t more = a.dtab ? kWaves * (tw + 32 * 64) * 4 : 0;
     by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_dq<decltype(t), n(), false>, grid, lds + more, st, a); });
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dq)");
     if (a.dtab) {
@@ -980,7 +968,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   }
   if (a.dk) {
     const int split = dkv_split(a.B, a.Sk, a.kv, a.group);
-    const dim3 kgrid((unsigned)((int64_t)a.B * a.kv * split * ((a.Sk + kRows - 1) / kRows)));
+    const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * split, (a.Sk + kRows - 1) / kRows, a.causal));
     float* shares = split > 1 ? part : nullptr;
     by_shape(x->dtype, a.d,
              [&](auto t, auto n) { start(k_ba_dkv<decltype(t), n()>, kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, split, shares); });
