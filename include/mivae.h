@@ -113,10 +113,10 @@ typedef struct mivae_attention_args {
   const int32_t* buckets;     /* (2 distance + 1) */
   int32_t* codes;             /* mivae_biased_attention_codes_ints values, 16-byte aligned; with mask or documents: written
                                  forward, read backward */
-  const void* dout;           /* backward only from here on */
+  const void* dout;           /* backward only, to dtable */
   void *dq, *dk, *dv;         /* dq may be NULL, dk and dv together */
   float* dtable;              /* (num_buckets, heads), or NULL */
-  float* scratch;             /* mivae_biased_attention_bwd_floats values, 16-byte aligned */
+  float* scratch;             /* mivae_biased_attention_fwd_floats (0: NULL will do) / .._bwd_floats values, 16-byte aligned */
   int64_t batch, q_len, k_len, heads, kv_heads, head_size;
   int64_t q_stride[3], k_stride[3], v_stride[3];
   int64_t q_start, num_buckets, distance;
@@ -124,6 +124,8 @@ typedef struct mivae_attention_args {
   int causal, dtype;
 } mivae_attention_args;
 int64_t mivae_biased_attention_codes_ints(int64_t batch, int64_t q_len, int64_t k_len, int documents);
+int64_t mivae_biased_attention_fwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
+                                          int64_t head_size);
 int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
                                           int64_t head_size, int64_t num_buckets);
 int mivae_biased_attention_fwd(const mivae_attention_args* args, void* stream);

@@ -53,6 +53,7 @@ SIGNATURES = {
     "mivae_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, F32,
                             P],
     "mivae_biased_attention_codes_ints": [I64, I64, I64, I32],
+    "mivae_biased_attention_fwd_floats": [I64, I64, I64, I64, I64, I64],
     "mivae_biased_attention_bwd_floats": [I64, I64, I64, I64, I64, I64, I64],
     "mivae_biased_attention_fwd": [P, P],
     "mivae_biased_attention_bwd": [P, P],
@@ -172,6 +173,7 @@ SIGNATURES = {
 }
 _RET = {
     "mivae_biased_attention_codes_ints": I64,
+    "mivae_biased_attention_fwd_floats": I64,
     "mivae_biased_attention_bwd_floats": I64,
     "mivae_qk_norm_rotary_scratch_floats": I64,
     "mivae_last_error": ctypes.c_char_p,

@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmivae.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
-SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "biased_attention.hip", "qk_rotary.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
+SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "biased_attention.hip", "token_attention.hip", "qk_rotary.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
 # packed-fp32-ops off: hipcc -O3 otherwise forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some operand forms
 # of these have been seen to return wrong values now and then.  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",

@@ -289,6 +289,45 @@ __device__ __forceinline__ void stage_table(float* tab, const BiasedArgs& a, int
 
 __device__ __forceinline__ int clamp_start(int s) { return min(max(s, -(1 << 30)), 1 << 30); }
 
+// ---- visibility ---------------------------------------------------------------------------------------------------------
+// Causal mask and prefix are one limit per query, non-decreasing in the row: it sees the keys below limit(i).
+struct View {
+  int start, prefix, Sk;
+  bool causal, codes, docs;
+  __device__ __forceinline__ int limit(int row) const { return causal ? min(Sk, max(start + row + 1, prefix)) : Sk; }
+  // first query row that sees key j
+  __device__ __forceinline__ int first_row(int key) const { return !causal || key < prefix ? 0 : max(0, key - start); }
+};
+
+__device__ __forceinline__ View view_of(const BiasedArgs& a, int64_t b) {
+  View v;
+  v.start = clamp_start(a.q_starts ? a.q_starts[b] : a.q_start);
+  v.prefix = a.prefix ? a.prefix[b] : 0;
+  v.Sk = a.Sk;
+  v.causal = a.causal != 0;
+  v.codes = a.kcodes != nullptr;
+  v.docs = a.qcodes != nullptr;
+  return v;
+}
+
+// lowest / highest value of `code` over the wave's lanes with code >= 0
+__device__ __forceinline__ void wave_range(int code, int& lo, int& hi) {
+  lo = code >= 0 ? code : INT32_MAX;
+  hi = code >= 0 ? code : -1;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    lo = min(lo, __shfl_xor(lo, off, 64));
+    hi = max(hi, __shfl_xor(hi, off, 64));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+}
+
+__device__ __forceinline__ i32x4 merge(const i32x4& a, const i32x4& b) {
+  return i32x4{min(a[0], b[0]), max(a[1], b[1]), 0, 0};
+}
+__device__ __forceinline__ uint64_t rows_of(const i32x4& t) { return (uint64_t)(unsigned)t[3] << 32 | (unsigned)t[2]; }
+
 // the other half-wave's value, without a trip through LDS
 __device__ __forceinline__ float max_halves(float x) {
   const unsigned b = __float_as_uint(x);

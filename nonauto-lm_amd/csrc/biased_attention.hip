@@ -17,6 +17,7 @@
 
 #include "att_tiles.hpp"
 #include "mivae.h"
+#include "token_attention.hpp"
 
 using namespace mivae;
 
@@ -94,44 +95,6 @@ __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, f
 }
 
 // ---- what a block knows about visibility -------------------------------------------------------------------------------
-// Causal mask and prefix are one limit per query, non-decreasing in the row: it sees the keys below limit(i).
-struct View {
-  int start, prefix, Sk;
-  bool causal, codes, docs;
-  __device__ __forceinline__ int limit(int row) const { return causal ? min(Sk, max(start + row + 1, prefix)) : Sk; }
-  // first query row that sees key j
-  __device__ __forceinline__ int first_row(int key) const { return !causal || key < prefix ? 0 : max(0, key - start); }
-};
-
-__device__ __forceinline__ View view_of(const BiasedArgs& a, int64_t b) {
-  View v;
-  v.start = clamp_start(a.q_starts ? a.q_starts[b] : a.q_start);
-  v.prefix = a.prefix ? a.prefix[b] : 0;
-  v.Sk = a.Sk;
-  v.causal = a.causal != 0;
-  v.codes = a.kcodes != nullptr;
-  v.docs = a.qcodes != nullptr;
-  return v;
-}
-
-// lowest / highest value of `code` over the wave's lanes with code >= 0
-__device__ __forceinline__ void wave_range(int code, int& lo, int& hi) {
-  lo = code >= 0 ? code : INT32_MAX;
-  hi = code >= 0 ? code : -1;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    lo = min(lo, __shfl_xor(lo, off, 64));
-    hi = max(hi, __shfl_xor(hi, off, 64));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
-}
-
-__device__ __forceinline__ i32x4 merge(const i32x4& a, const i32x4& b) {
-  return i32x4{min(a[0], b[0]), max(a[1], b[1]), 0, 0};
-}
-__device__ __forceinline__ uint64_t rows_of(const i32x4& t) { return (uint64_t)(unsigned)t[3] << 32 | (unsigned)t[2]; }
-
 // The walk of a block of queries over the keys in chunks of kChunk, shared by the forward and the dq kernel.
 struct KeyWalk {
   int end;                // no query of the block sees a key at or beyond it
@@ -804,6 +767,9 @@ int dkv_split(int64_t B, int64_t Sk, int64_t kv, int64_t group) {
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
+// Few queries take the split form.
+bool few_queries(int64_t Sq) { return Sq <= 16; }
+
 int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
 // LDS of the buffers (two with bf16, one with fp32): two tiles and `words` 4-byte values per row of a chunk
 size_t tile_bytes(int dtype, int d, int words) {
@@ -899,6 +865,11 @@ int64_t mivae_biased_attention_codes_ints(int64_t batch, int64_t q_len, int64_t 
   return batch * (pad64(k_len) + (documents ? pad64(q_len) : 0)) / 16 * 17;
 }
 
+int64_t mivae_biased_attention_fwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
+                                          int64_t head_size) {
+  return few_queries(q_len) ? token_attention_floats(batch, q_len, k_len, heads, kv_heads, head_size) : 0;
+}
+
 int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
                                           int64_t head_size, int64_t num_buckets) {
   const int64_t nblk = (q_len + kRows - 1) / kRows, split = dkv_split(batch, k_len, kv_heads, heads / kv_heads);
@@ -917,6 +888,13 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
                        a.q_starts, a.q_start, a.B, a.Sq, a.Sk, a.kpad, a.qpad, const_cast<int*>(a.kcodes),
                        const_cast<int*>(a.qcodes), const_cast<i32x4*>(a.ktiles), const_cast<i32x4*>(a.qtiles));
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (codes)");
+  }
+  if (few_queries(a.Sq)) {
+    const int64_t need = token_attention_floats(a.B, a.Sq, a.Sk, a.heads, a.kv, a.d);
+    MIVAE_REQUIRE(need == 0 || (x->scratch && aligned16(x->scratch)), "mivae_biased_attention_fwd: the keys are split and need the scratch buffer");
+    token_attention(a, x->scratch, x->dtype, stream);
+    MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (few queries)");
+    return MIVAE_OK;
   }
   const size_t lds = tile_bytes(x->dtype, a.d, 1) + (a.table ? (2 * a.R + 1) * 4 : 0);
   const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, (a.Sq + kRows - 1) / kRows, a.causal));

@@ -453,7 +453,10 @@ def _biased_attention_fwd(q, mask, documents, args, need_lse: bool):
     if mask is not None or documents is not None:
         codes = torch.empty(_buffer_size("mivae_biased_attention_codes_ints", args.batch, args.q_len, args.k_len,
                                          int(documents is not None)), dtype=torch.int32, device=dev)
-    args.out, args.lse, args.codes = out.data_ptr(), L.ptr(lse), L.ptr(codes)
+    n = _buffer_size("mivae_biased_attention_fwd_floats", args.batch, args.q_len, args.k_len, args.heads, args.kv_heads,
+                     args.head_size)
+    scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    args.out, args.lse, args.codes, args.scratch = out.data_ptr(), L.ptr(lse), L.ptr(codes), L.ptr(scratch)
     with L.on_device(dev), _timed("biased_attention_fwd"):
         L.call("mivae_biased_attention_fwd", ctypes.byref(args), L.stream())
     return out, lse, codes
