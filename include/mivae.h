@@ -138,7 +138,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* args, void* stream);
  * q (batch, len, heads, head_size) and k (.., kv_heads, ..) of one dtype, element (b, s, h, c) at b stride[0] + s stride[1] +
  * h stride[2] + c; q_out / k_out / dq_out / dk_out contiguous.  Backward: q_out / k_out receive dq / dk (q, k may be NULL
  * without a norm), dq_weight / dk_weight (head_size) may be NULL, scratch holds mivae_qk_norm_rotary_scratch_floats.
- * head_size even, 2 .. 256.  16-byte accesses where alignment, strides and rotary_dim allow, else element by element. */
+ * head_size even, 2 .. 256, at most 4095 heads in all, batch len < 2^31 - 2^16.  16-byte accesses where alignment, strides and rotary_dim allow, else element by element. */
 typedef struct mivae_rotary_args {
   const void *q, *k;
   void *q_out, *k_out;

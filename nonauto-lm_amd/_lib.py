@@ -236,11 +236,24 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+_NO_SWITCH = contextlib.nullcontext()
+_DEVICES = 0
+
+
 def on_device(device):
     """Context in which `device` is the current one: launches go to the operands' device, whatever the caller's is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    global _DEVICES
+    if _DEVICES == 0:
+        _DEVICES = torch.cuda.device_count()
+    if _DEVICES == 1 or device.index is None or device.index == torch.cuda.current_device():
+        return _NO_SWITCH
     return torch.cuda.device(device)
+
+
+def stream_of(device):
+    """Handle of the current stream of `device`.  (torch.cuda.current_stream() builds a Stream object: 13 us a call from
+    autograd's thread.)"""
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def require_gpu(*tensors):

@@ -22,10 +22,22 @@ struct RotArgs {
   float* part;                          // backward: (blocks, 2, d) weight-gradient partials, or null
   const double* freq;                   // (rot / 2) turns per position, or null: no rotation
   const int64_t* pos;                   // element (b, s) at pos[b * pos_b + s * pos_s], or null: start + s
-  int64_t qs[3], ks[3], pos_b, pos_s, start, tokens;
-  int S, H, G, d, half, rest, lpr, tpb, inter;      // half = rot / 2, rest = (d - rot) / 2; lpr lanes per row, tpb tokens per block
+  int64_t qs[3], ks[3], pos_b, pos_s, start;
+  unsigned tokens, S, rows_magic, half_magic;       // x / (H + G) = umulhi(x, rows_magic) and x / half likewise, x < 2^16
+  int H, G, d, half, rest, lpr, tpb, inter;         // half = rot / 2, rest = (d - rot) / 2; lpr lanes per row, tpb tokens at a time
   float eps;
 };
+
+// (batch row, position) of token t behind token (b0, s0)
+__device__ __forceinline__ void token_at(unsigned S, unsigned b0, unsigned s0, unsigned t, int64_t& b, int64_t& s) {
+  unsigned x = s0 + t, y = b0;
+  while (x >= S) {
+    x -= S;
+    ++y;
+  }
+  b = y;
+  s = x;
+}
 
 constexpr int kThreads = 256;
 
@@ -82,12 +94,14 @@ __device__ __forceinline__ void join_pairs(bool inter, const float (&a)[VEC], co
   }
 }
 
-// cosines and sines of the block's tokens: cs[token][pair] = {cos, sin}
-__device__ __forceinline__ void stage_angles(float2* cs, const RotArgs& a, int64_t tok0, int ntok) {
+// cosines and sines of ntok tokens from (b0, s0) on: cs[token][pair] = {cos, sin}
+__device__ __forceinline__ void stage_angles(float2* cs, const RotArgs& a, unsigned b0, unsigned s0, int ntok) {
   for (int i = threadIdx.x; i < ntok * a.half; i += kThreads) {
-    const int64_t tok = tok0 + i / a.half, b = tok / a.S, s = tok % a.S;
+    const unsigned t = a.half == 1 ? i : __umulhi(i, a.half_magic);
+    int64_t b, s;
+    token_at(a.S, b0, s0, t, b, s);
     const int64_t p = a.pos ? a.pos[b * a.pos_b + s * a.pos_s] : a.start + s;
-    const double turns = (double)p * a.freq[i % a.half];
+    const double turns = (double)p * a.freq[i - t * a.half];
     float sn, cn;
     sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
     cs[i] = make_float2(cn, sn);
@@ -98,7 +112,7 @@ __device__ __forceinline__ void stage_angles(float2* cs, const RotArgs& a, int64
 template <typename T, int VEC, int CPL, bool NORM, bool BWD>
 __global__ __launch_bounds__(kThreads) void k_qk(RotArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float2* cs = reinterpret_cast<float2*>(smem);
+  float2* cs = reinterpret_cast<float2*>(smem);       // [2][tpb][half]: written for the next tokens while these are read
   const int HG = a.H + a.G, lane_c = threadIdx.x % a.lpr, slot = threadIdx.x / a.lpr, slots = kThreads / a.lpr;
   const int chunks = (a.half + a.rest) / VEC;
   const float inv_d = 1.f / (float)a.d;
@@ -123,11 +137,13 @@ __global__ __launch_bounds__(kThreads) void k_qk(RotArgs a) {
       }
     }
   }
-  for (int64_t tok0 = (int64_t)blockIdx.x * a.tpb; tok0 < a.tokens; tok0 += (int64_t)gridDim.x * a.tpb) {
-    const int ntok = (int)min((int64_t)a.tpb, a.tokens - tok0);
+  unsigned odd = 0;
+  for (unsigned tok0 = blockIdx.x * a.tpb; tok0 < a.tokens; tok0 += gridDim.x * a.tpb, odd ^= 1) {
+    const int ntok = (int)min((unsigned)a.tpb, a.tokens - tok0);
+    const unsigned b0 = tok0 / a.S, s0 = tok0 % a.S;
+    const float2* now = cs + odd * a.tpb * a.half;
     if (a.freq) {
-      __syncthreads();                  // the previous tokens' angles have been read
-      stage_angles(cs, a, tok0, ntok);
+      stage_angles(cs + odd * a.tpb * a.half, a, b0, s0, ntok);
       __syncthreads();
     }
     const int rows = ntok * HG;
@@ -135,9 +151,11 @@ __global__ __launch_bounds__(kThreads) void k_qk(RotArgs a) {
     for (int r0 = 0; r0 < rows; r0 += slots) {
       const int r = r0 + slot;
       const bool live = r < rows;
-      const int t = live ? r / HG : 0, hd = live ? r % HG : 0;
+      const int t = live ? (int)__umulhi(r, a.rows_magic) : 0, hd = live ? r - t * HG : 0;
       const bool isq = hd < a.H;
-      const int64_t tok = tok0 + t, b = tok / a.S, s = tok % a.S;
+      const int64_t tok = (int64_t)tok0 + t;
+      int64_t b, s;
+      token_at(a.S, b0, s0, t, b, s);
       const T* x = isq ? static_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[1] + hd * a.qs[2]
                        : static_cast<const T*>(a.k) + b * a.ks[0] + s * a.ks[1] + (hd - a.H) * a.ks[2];
       const int64_t o = isq ? (tok * a.H + hd) * a.d : (tok * a.G + hd - a.H) * a.d;
@@ -165,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void k_qk(RotArgs a) {
       }
       float inv = 1.f;
       if (NORM) inv = 1.f / sqrtf(fmaf(group_sum(sum, a.lpr), inv_d, a.eps));
-      const float2* c0 = cs + t * a.half;
+      const float2* c0 = now + t * a.half;
       float dot = 0.f;
 #pragma unroll
       for (int n = 0; n < CPL; ++n) {
@@ -253,17 +271,23 @@ __global__ __launch_bounds__(kThreads) void k_qk(RotArgs a) {
   }
 }
 
-// dqw / dkw = the blocks' partials summed in a fixed order, one wave per element
-__global__ __launch_bounds__(64) void k_qk_dw(const float* part, float* dqw, float* dkw, int blocks, int d) {
-  const int e = blockIdx.x;
+// dqw / dkw = the blocks' partials summed in a fixed order: 16 columns per block, 64 rows at a time
+__global__ __launch_bounds__(1024) void k_qk_dw(const float* part, float* dqw, float* dkw, int blocks, int d) {
+  __shared__ float red[64][17];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
   float s = 0.f;
-  for (int i = threadIdx.x; i < blocks; i += 64) s += part[(int64_t)i * 2 * d + e];
-  s = group_sum(s, 64);
+  if (e < 2 * d)
+    for (int i = g; i < blocks; i += 64) s += part[(int64_t)i * 2 * d + e];
+  red[g][c] = s;
+  for (int n = 32; n > 0; n >>= 1) {
+    __syncthreads();
+    if (g < n) red[g][c] += red[g + n][c];
+  }
   float* dst = e < d ? dqw : dkw;
-  if (threadIdx.x == 0 && dst) dst[e < d ? e : e - d] = s;
+  if (g == 0 && e < 2 * d && dst) dst[e < d ? e : e - d] = red[0][c];
 }
 
-constexpr int kMaxBlocks = 2048;        // of the backward: one row of partials each
+constexpr int kMaxBlocks = 1024;        // four per CU; the backward leaves a row of partials for each
 
 struct Geometry {
   bool vec;
@@ -307,8 +331,8 @@ void launch(const RotArgs& a, const Geometry& g, int64_t blocks, size_t lds, boo
 int run(const mivae_rotary_args* x, bool bwd, const char* name, void* stream) {
   MIVAE_REQUIRE(x != nullptr, "%s: null arguments", name);
   MIVAE_REQUIRE(x->dtype == MIVAE_F32 || x->dtype == MIVAE_BF16, "%s: dtype %d is neither float32 nor bfloat16", name, x->dtype);
-  MIVAE_REQUIRE(x->batch >= 1 && x->len >= 1 && x->heads >= 1 && x->kv_heads >= 1 && x->heads <= 65535 && x->kv_heads <= 65535 &&
-                    x->batch <= (1ll << 31) && x->len <= (1ll << 31) && x->batch * x->len < (1ll << 40),
+  MIVAE_REQUIRE(x->batch >= 1 && x->len >= 1 && x->heads >= 1 && x->kv_heads >= 1 && x->heads + x->kv_heads <= 4095 &&
+                    x->batch < (1ll << 31) && x->len < (1ll << 31) && x->batch * x->len < (1ll << 31) - (1 << 16),
                 "%s: batch %lld, length %lld, heads %lld + %lld out of range", name, (long long)x->batch, (long long)x->len,
                 (long long)x->heads, (long long)x->kv_heads);
   MIVAE_REQUIRE(x->head_size >= 2 && x->head_size <= 256 && x->head_size % 2 == 0, "%s: head size %lld is not an even number in 2 .. 256",
@@ -328,8 +352,8 @@ int run(const mivae_rotary_args* x, bool bwd, const char* name, void* stream) {
   a.freq = x->freq; a.pos = x->positions;
   for (int i = 0; i < 3; ++i) { a.qs[i] = x->q_stride[i]; a.ks[i] = x->k_stride[i]; }
   a.pos_b = x->position_stride[0]; a.pos_s = x->position_stride[1]; a.start = x->start;
-  a.tokens = x->batch * x->len;
-  a.S = (int)x->len; a.H = (int)x->heads; a.G = (int)x->kv_heads; a.d = (int)x->head_size;
+  a.tokens = (unsigned)(x->batch * x->len);
+  a.S = (unsigned)x->len; a.H = (int)x->heads; a.G = (int)x->kv_heads; a.d = (int)x->head_size;
   a.half = x->freq ? (int)x->rotary_dim / 2 : 0;
   a.rest = a.d / 2 - a.half;
   a.inter = x->interleaved ? 1 : 0;
@@ -338,17 +362,17 @@ int run(const mivae_rotary_args* x, bool bwd, const char* name, void* stream) {
   a.lpr = g.lpr; a.tpb = g.tpb;
   const bool dw = x->dq_weight || x->dk_weight;
   a.part = dw ? x->scratch : nullptr;
-  size_t lds = (size_t)a.tpb * a.half * sizeof(float2);
+  size_t lds = (size_t)2 * a.tpb * a.half * sizeof(float2);
   if (dw && lds < (size_t)kThreads / 64 * 2 * a.d * 4) lds = (size_t)kThreads / 64 * 2 * a.d * 4;
-  int64_t blocks = (a.tokens + a.tpb - 1) / a.tpb;
-  if (bwd) blocks = g.blocks;
-  if (blocks > (1ll << 30)) blocks = 1ll << 30;
+  const int64_t blocks = g.blocks;
+  a.rows_magic = (unsigned)(((1ull << 32) + a.H + a.G - 1) / (a.H + a.G));
+  a.half_magic = a.half > 1 ? (unsigned)(((1ull << 32) + a.half - 1) / a.half) : 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (x->dtype == MIVAE_F32) launch<float, 4>(a, g, blocks, lds, x->norm != 0, bwd, st);
   else launch<unsigned short, 8>(a, g, blocks, lds, x->norm != 0, bwd, st);
   MIVAE_CHECK_LAUNCH(name);
   if (dw) {
-    hipLaunchKernelGGL(k_qk_dw, dim3((unsigned)(2 * a.d)), dim3(64), 0, st, x->scratch, x->dq_weight, x->dk_weight, (int)blocks, a.d);
+    hipLaunchKernelGGL(k_qk_dw, dim3((unsigned)((2 * a.d + 15) / 16)), dim3(1024), 0, st, x->scratch, x->dq_weight, x->dk_weight, (int)blocks, a.d);
     MIVAE_CHECK_LAUNCH(name);
   }
   return MIVAE_OK;

@@ -17,7 +17,7 @@ using namespace mivae;
 
 namespace {
 
-constexpr int kWaves = 4, kKeys = 32;          // keys of a tile
+constexpr int kWaves = 2, kKeys = 32;          // keys of a tile
 constexpr int kSpan = kWaves * kKeys;          // keys of a block's turn
 
 // 32 rows of a head on their way into a wave's own tile; rows whose bit is 0 and columns beyond d arrive as zeros
@@ -89,10 +89,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
   T* tiles = reinterpret_cast<T*>(smem) + wave * 2 * NBUF * TILE;         // [NBUF][K, V]
   const unsigned id = blockIdx.x;
-  const int split = (int)(id % (unsigned)t.splits), rt = (int)(id / (unsigned)t.splits % (unsigned)t.tiles);
-  const unsigned pair = id / (unsigned)(t.splits * t.tiles);
-  const int64_t b = pair / (unsigned)a.kv;
-  const int kvh = (int)(pair % (unsigned)a.kv);
+  // the key heads of a row are neighbours in memory and in the grid
+  const int kvh = (int)(id % (unsigned)a.kv), split = (int)(id / (unsigned)a.kv % (unsigned)t.splits);
+  const unsigned rest = id / (unsigned)(a.kv * t.splits);
+  const int rt = (int)(rest % (unsigned)t.tiles);
+  const int64_t b = rest / (unsigned)t.tiles, pair = b * a.kv + kvh;
   const View v = view_of(a, b);
   // the lane's row
   const int row = rt * 32 + r32, pos = row / a.group, head = kvh * a.group + row % a.group;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     }
   }
   l += __shfl_xor(l, 32, 64);
-  // join the four waves: [wave][row][W + 4] floats of O, max, sum (the pitch keeps 16-byte stores aligned)
+  // join the waves: [wave][row][W + 4] floats of O, max, sum (the pitch keeps 16-byte stores aligned)
   constexpr int P = W + 4;
   float* join = reinterpret_cast<float*>(smem);
   __syncthreads();
@@ -292,32 +293,42 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   }
 }
 
-// out = the splits' partials joined in order: one group of d / 4 lanes per packed row
+// out = the splits' partials joined in order, one wave per packed row: lanes take splits for the maximum and the sum, then
+// stripes of splits for groups of four columns
 template <typename T>
-__global__ __launch_bounds__(256) void k_token_join(TokenArgs t, int64_t n) {
+__global__ __launch_bounds__(64) void k_token_join(TokenArgs t) {
   const BiasedArgs& a = t.a;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int q4 = a.d / 4;
-  if (i >= n * q4) return;
-  const int64_t pr = i / q4;
-  const int c = (int)(i % q4) * 4;
-  const float* p = t.part + pr * t.splits * (a.d + 4);
-  float top = -__FLT_MAX__, sum = 0.f;
-  for (int s = 0; s < t.splits; ++s) top = fmaxf(top, p[s * (a.d + 4) + a.d]);
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < t.splits; ++s) {
-    const float* e = p + s * (a.d + 4);
-    const float f = __builtin_amdgcn_exp2f(e[a.d] - top);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(e + c);
-    sum = fmaf(f, e[a.d + 1], sum);
+  const int64_t pr = blockIdx.x;
+  const int lane = threadIdx.x, pitch = a.d + 4;
+  const float* p = t.part + pr * t.splits * pitch;
+  float top = -__FLT_MAX__;
+  for (int s = lane; s < t.splits; s += 64) top = fmaxf(top, p[s * pitch + a.d]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = fmaf(f, y[j], x[j]);
-  }
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  float sum = 0.f;
+  for (int s = lane; s < t.splits; s += 64) sum = fmaf(__builtin_amdgcn_exp2f(p[s * pitch + a.d] - top), p[s * pitch + a.d + 1], sum);
+  sum = group_sum(sum, 64);
+  int lpg = 1;                           // lanes per row of d / 4 groups, a power of two
+  while (lpg < a.d / 4) lpg <<= 1;
+  const int c = (lane % lpg) * 4, stripes = 64 / lpg;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (c < a.d)
+#pragma unroll 4
+    for (int s = lane / lpg; s < t.splits; s += stripes) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * pitch + c);
+      const float f = __builtin_amdgcn_exp2f(p[s * pitch + a.d] - top);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = fmaf(f, y[j], x[j]);
+    }
+  for (int off = 32; off >= lpg; off >>= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], off, 64);
   const int64_t pair = pr / t.rows, row = pr % t.rows, b = pair / a.kv;
   const int64_t pos = row / a.group, head = pair % a.kv * a.group + row % a.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  store4(static_cast<T*>(a.out) + ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-  if (a.lse && c == 0) a.lse[(b * a.heads + head) * a.Sq + pos] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+  if (lane < lpg && c < a.d)
+    store4(static_cast<T*>(a.out) + ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  if (a.lse && lane == 0) a.lse[(b * a.heads + head) * a.Sq + pos] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 template <typename T, int NDB>
@@ -330,8 +341,8 @@ void start(const TokenArgs& t, unsigned grid, hipStream_t st) {
   hipLaunchKernelGGL((k_token<T, NDB>), dim3(grid), dim3(64 * kWaves), lds, st, t);
 }
 
-// Splits: enough blocks for four turns of 256 CUs, each of at least one turn of its four waves (128 keys).  More only add
-// partials to join; fewer leave CUs idle or wait for the longest row.
+// Splits: 1024 blocks, two turns of two blocks per CU, each of at least one turn of its waves (64 keys).  More pay for more
+// starts and partials (2048: 178 us at the size above), fewer wait for the longest row (512: 165 us there, 56 % to 100 % full).
 int splits_of(int64_t blocks, int64_t Sk) {
   int64_t s = (1024 + blocks - 1) / blocks;
   const int64_t most = (Sk + kSpan - 1) / kSpan;
@@ -372,10 +383,9 @@ void token_attention(const BiasedArgs& a, float* scratch, int dtype, void* strea
     else start<unsigned short, 4>(t, grid, st);
   }
   if (t.part) {
-    const int64_t n = (int64_t)a.B * a.kv * t.rows;
-    const dim3 jgrid((unsigned)((n * (a.d / 4) + 255) / 256));
-    if (dtype == MIVAE_F32) hipLaunchKernelGGL((k_token_join<float>), jgrid, dim3(256), 0, st, t, n);
-    else hipLaunchKernelGGL((k_token_join<unsigned short>), jgrid, dim3(256), 0, st, t, n);
+    const dim3 rows((unsigned)((int64_t)a.B * a.kv * t.rows));
+    if (dtype == MIVAE_F32) hipLaunchKernelGGL((k_token_join<float>), rows, dim3(64), 0, st, t);
+    else hipLaunchKernelGGL((k_token_join<unsigned short>), rows, dim3(64), 0, st, t);
   }
 }
 

@@ -338,7 +338,7 @@ def _qk_norm_rotary_fwd(q, k, args):
     if q.numel():
         args.q_out, args.k_out = yq.data_ptr(), yk.data_ptr()
         with L.on_device(q.device):
-            L.call("mivae_qk_norm_rotary_fwd", ctypes.byref(args), L.stream())
+            L.call("mivae_qk_norm_rotary_fwd", ctypes.byref(args), L.stream_of(q.device))
     return yq, yk
 
 
@@ -368,7 +368,7 @@ class _QkNormRotary(torch.autograd.Function):
             args = _refill(ctx.args, q=q, k=k, q_weight=qw, k_weight=kw, freq=freqs, positions=positions, dq_out=dyq,
                            dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw, scratch=scratch)
             with L.on_device(dev):
-                L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream())
+                L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream_of(dev))
         return dq, dk, dqw, dkw, None, None, None
 
 
@@ -458,7 +458,7 @@ def _biased_attention_fwd(q, mask, documents, args, need_lse: bool):
     scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
     args.out, args.lse, args.codes, args.scratch = out.data_ptr(), L.ptr(lse), L.ptr(codes), L.ptr(scratch)
     with L.on_device(dev), _timed("biased_attention_fwd"):
-        L.call("mivae_biased_attention_fwd", ctypes.byref(args), L.stream())
+        L.call("mivae_biased_attention_fwd", ctypes.byref(args), L.stream_of(dev))
     return out, lse, codes
 
 
@@ -488,7 +488,7 @@ class _BiasedAttention(torch.autograd.Function):
                        slopes=slopes, buckets=buckets, codes=codes, out=out, lse=lse, dout=dout, dq=dq, dk=dk, dv=dv,
                        dtable=dtable, scratch=scratch)
         with L.on_device(dev), _timed("biased_attention_bwd"):
-            L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream())
+            L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream_of(dev))
         return (dq, dk if need_k else None, dv if need_v else None, dtable) + (None,) * 7
 
 
