@@ -104,8 +104,8 @@ typedef struct mivae_attention_args {
   const void *q, *k, *v;
   void* out;
   float* lse;                 /* (batch, heads, q_len): written forward (or NULL), read backward */
-  const int64_t* mask;        /* (batch, k_len), or NULL */
-  const int32_t* documents;   /* (batch, k_len), or NULL */
+  const int64_t* mask;        /* (batch, k_len), or NULL.  The backward reads codes instead and only looks whether these */
+  const int32_t* documents;   /* (batch, k_len), or NULL   two are NULL */
   const int32_t* prefix;      /* (batch), or NULL; needs causal */
   const int32_t* q_starts;    /* (batch), or NULL: q_start for every batch row */
   const float* slopes;        /* (heads), or NULL */

@@ -466,22 +466,85 @@ USE_MIVAE_ATTENTION = os.environ.get("MIVAE_LIB_ATTENTION", "0") != "1"
 
 class MultiHeadAttention(torch.nn.Module):
     """nn/transformer.py:7-117: separate q/k/v projections, masked_fill(-1e13) on padded keys,
-    optional causal (tril) mask.  Scores are materialised like the reference (S <= 512 here)."""
+    optional causal (tril) mask.  Scores are materialised like the reference (S <= 512 here).
+
+    Options beyond the reference, any of which moves the layer onto `ops.qk_norm_rotary` / `ops.biased_attention` (fp32 or
+    bf16, any length, head sizes that are multiples of 8 up to 128, GPU only, no attention dropout):
+      kv_heads        key / value heads, each shared by num_heads / kv_heads query heads
+      softcap         scores capped to softcap * tanh(score / softcap)
+      relative_bias   dict(num_buckets=32, max_distance=128): learned bias by bucketed relative position, `_relative_bias`
+                      (num_buckets, num_heads), zero at first
+      distance_slopes scores lowered by 2^(-8 (h + 1) / num_heads) per position of distance (not with relative_bias)
+      qk_norm         root-mean-square norm of every query and key head with learned scales `_query_norm`, `_key_norm`
+      rotary          position rotation of the heads' first `rotary` elements (True: all of them)
+    With them a query that sees no key gets zeros instead of the mean of all values, and `forward` takes `documents` and
+    `prefix` (see ops.biased_attention) and keys that are longer than the queries (the queries are the last positions)."""
 
     def __init__(self, num_heads, hidden_size, bias=True, dropout=0.1, output_size=None,
-                 attention_fill_value=-1e13, mask_tril=False):
+                 attention_fill_value=-1e13, mask_tril=False, kv_heads=None, softcap=None, relative_bias=None,
+                 distance_slopes=False, qk_norm=False, rotary=None, rotary_base=10000.0):
         super().__init__()
         assert hidden_size % num_heads == 0
         self._attn_size = hidden_size // num_heads
         self._num_heads = num_heads
+        self._kv_heads = kv_heads or num_heads
+        self._softcap, self._slopes, self._qk_norm = softcap, bool(distance_slopes), bool(qk_norm)
+        self._rotary, self._rotary_base = (self._attn_size if rotary is True else rotary or None), rotary_base
+        self._scored = bool(self._kv_heads != num_heads or softcap is not None or relative_bias is not None or distance_slopes
+                            or qk_norm or self._rotary)
+        if self._scored:
+            if num_heads % self._kv_heads:
+                raise ValueError(f"{num_heads} heads cannot share {self._kv_heads} key heads")
+            if dropout and dropout > 0:
+                raise ValueError("kv_heads, softcap, relative_bias, distance_slopes, qk_norm and rotary need dropout=0 in the "
+                                 "attention (a transformer layer's own dropout may differ: attention=dict(dropout=0.0, ...))")
+            if relative_bias is not None and distance_slopes:
+                raise ValueError("relative_bias and distance_slopes are alternatives")
         self._projections = torch.nn.ModuleDict({
             "query": Linear(hidden_size, hidden_size, bias=bias),
-            "key": Linear(hidden_size, hidden_size, bias=bias),
-            "value": Linear(hidden_size, hidden_size, bias=bias)})
+            "key": Linear(hidden_size, self._kv_heads * self._attn_size, bias=bias),
+            "value": Linear(hidden_size, self._kv_heads * self._attn_size, bias=bias)})
         self._output = Linear(hidden_size, output_size or hidden_size)
         self._fill = attention_fill_value
         self._mask_tril = mask_tril
         self._dropout = _maybe_dropout(dropout)
+        self._relative_bias = None
+        if relative_bias is not None:
+            count = relative_bias.get("num_buckets", 32)
+            self._relative_bias = torch.nn.Parameter(torch.zeros(count, num_heads))
+            self.register_buffer("_buckets", ops.relative_buckets(count, relative_bias.get("max_distance", 128),
+                                                                  not mask_tril), persistent=False)
+        if self._qk_norm:
+            self._query_norm = torch.nn.Parameter(torch.ones(self._attn_size))
+            self._key_norm = torch.nn.Parameter(torch.ones(self._attn_size))
+        self._constants = {}            # device -> (frequencies, slopes): float64 / fp32 whatever the module is cast to
+
+    def _scored_constants(self, device):
+        made = self._constants.get(device)
+        if made is None:
+            freqs = ops.rotary_frequencies(self._rotary, self._rotary_base, device) if self._rotary else None
+            h = torch.arange(1, self._num_heads + 1, dtype=torch.float32, device=device)
+            made = (freqs, 2.0 ** (-8.0 * h / self._num_heads) if self._slopes else None)
+            if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():     # else: values of that graph alone
+                self._constants[device] = made
+        return made
+
+    def _scored_attention(self, q, k, v, mask, documents, prefix):
+        """(B, Sq, heads * d), (B, Sk, kv_heads * d) projections -> (B, Sq, heads * d)"""
+        freqs, slopes = self._scored_constants(q.device)
+        if self._qk_norm or self._rotary:
+            norm = dict(norm=self._qk_norm, q_weight=self._query_norm if self._qk_norm else None,
+                        k_weight=self._key_norm if self._qk_norm else None, frequencies=freqs)
+            if q.size(1) == k.size(1):
+                q, k = ops.qk_norm_rotary(q, k, self._num_heads, self._kv_heads, **norm)
+            else:                       # the queries are the last positions of the keys: two passes, one half of each kept
+                back = k.size(1) - q.size(1)
+                q_, k_ = q, k
+                q = ops.qk_norm_rotary(q_, k_[:, back:], self._num_heads, self._kv_heads, positions=back, **norm)[0]
+                k = ops.qk_norm_rotary(k_, k_, self._kv_heads, self._kv_heads, **norm)[1]
+        return ops.biased_attention(q, k, v, self._num_heads, self._kv_heads, mask=mask, causal=self._mask_tril, prefix=prefix,
+                                    documents=documents, softcap=self._softcap, slopes=slopes, table=self._relative_bias,
+                                    buckets=None if self._relative_bias is None else self._buckets)
 
     def _split(self, x):
         b, s, _ = x.shape
@@ -503,14 +566,18 @@ class MultiHeadAttention(torch.nn.Module):
     def _project_out(self, t, residual):
         return self._output(t) if residual is None else self._output.forward_residual(t, residual)
 
-    def forward(self, query, key, value, mask=None, attn_bias=None, residual=None):
+    def forward(self, query, key, value, mask=None, attn_bias=None, residual=None, documents=None, prefix=None):
         """`residual` (optional): returns residual + attention(...), the add folded into the output projection"""
-        if query is key and key is value:        # self-attention: the three projections share their input
+        if not self._scored and (documents is not None or prefix is not None):
+            raise ValueError("documents and prefix need one of MultiHeadAttention's score options")
+        if query is key and key is value and self._kv_heads == self._num_heads:   # the three projections share their input
             q, k, v = linear_group(query, [self._projections[n] for n in ("query", "key", "value")], strided_ok=True)
         else:
             q = self._projections["query"](query)
             k = self._projections["key"](key)
             v = self._projections["value"](value)
+        if self._scored:
+            return self._project_out(self._scored_attention(q, k, v, mask, documents, prefix), residual)
         if (q.dtype == torch.bfloat16 and q.shape == k.shape and k.shape == v.shape and self.kernel_ok(q, mask)):
             # scores, reference fill (-1e13), softmax and probs @ v per head in libmivae's kernels, straight on the
             # (B, S, heads * d) projections (no head transposes, no bias tensor)
@@ -630,9 +697,11 @@ class PositionalEncoding(torch.nn.Module):
 
 
 class _TransformerLayer(torch.nn.Module):
-    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0, causal=False):
+    """`attention`: further arguments of the layer's MultiHeadAttention (score options, its own dropout)"""
+
+    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0, causal=False, attention=None):
         super().__init__()
-        self._attn = MultiHeadAttention(num_heads, input_size, dropout=dropout, mask_tril=causal)
+        self._attn = MultiHeadAttention(num_heads, input_size, mask_tril=causal, **{"dropout": dropout, **(attention or {})})
         self._pos_ffn = PositionwiseFeedForward(input_size, hidden_size, dropout=dropout)
         self._sublayers = torch.nn.ModuleDict({
             "attn": SublayerConnection(input_size, dropout=dropout),
@@ -640,13 +709,13 @@ class _TransformerLayer(torch.nn.Module):
 
     def attention_bias(self, x, mask):
         """the layer stack's shared attention bias for (x, mask), or None when the explicit masked-softmax path runs"""
-        if mask is None or not self._attn.fused_ok(x) or self._attn.kernel_ok(x, mask):
+        if mask is None or self._attn._scored or not self._attn.fused_ok(x) or self._attn.kernel_ok(x, mask):
             return None
         return ops.attention_bias(mask, self._attn._mask_tril, torch.bfloat16)
 
-    def forward(self, x, mask, attn_bias=None):
-        x = self._sublayers["attn"](x, lambda y, r=None: self._attn(y, y, y, mask, attn_bias, residual=r),
-                                    residual_aware=True)
+    def forward(self, x, mask, attn_bias=None, documents=None, prefix=None):
+        x = self._sublayers["attn"](x, lambda y, r=None: self._attn(y, y, y, mask, attn_bias, residual=r, documents=documents,
+                                                                    prefix=prefix), residual_aware=True)
         sub = self._sublayers["pos_ffn"]
         if USE_FUSED_FFN and ffn_block_supported(x, sub._norm, self._pos_ffn, sub):
             f = self._pos_ffn
@@ -656,15 +725,15 @@ class _TransformerLayer(torch.nn.Module):
 
 
 class TransformerEncoderLayer(_TransformerLayer):
-    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0):
-        super().__init__(input_size, hidden_size, num_heads, dropout, causal=False)
+    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0, attention=None):
+        super().__init__(input_size, hidden_size, num_heads, dropout, causal=False, attention=attention)
 
 
 class TransformerDecoderLayer(_TransformerLayer):
     """Self-attention with a causal x padding mask (nn/transformer.py:275)."""
 
-    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0):
-        super().__init__(input_size, hidden_size, num_heads, dropout, causal=True)
+    def __init__(self, input_size, hidden_size, num_heads, dropout=0.0, attention=None):
+        super().__init__(input_size, hidden_size, num_heads, dropout, causal=True, attention=attention)
 
 
 class EncoderOutput(NamedTuple):
@@ -711,11 +780,14 @@ class Encoder(torch.nn.Module, Registrable):
 
 @Encoder.register("transformer")
 class TransformerEncoder(Encoder):
-    def __init__(self, input_size, hidden_size, num_layers, num_heads, dropout=0.0):
+    """`attention`: dict of MultiHeadAttention's score options for every layer; with one of them `encoder` takes rows of
+    several documents (see ops.biased_attention)"""
+
+    def __init__(self, input_size, hidden_size, num_layers, num_heads, dropout=0.0, attention=None):
         super().__init__(input_size)
         self._pos_enc = PositionalEncoding(input_size)
         self._layers = torch.nn.ModuleList(
-            [TransformerEncoderLayer(input_size, hidden_size, num_heads, dropout) for _ in range(num_layers)])
+            [TransformerEncoderLayer(input_size, hidden_size, num_heads, dropout, attention) for _ in range(num_layers)])
         self._dropout = _maybe_dropout(dropout)
 
     def get_output_size(self):
@@ -724,11 +796,11 @@ class TransformerEncoder(Encoder):
     def _preprocess_embedding(self, x):
         return self._dropout(x)
 
-    def encoder(self, x, mask):
+    def encoder(self, x, mask, documents=None):
         x = self._pos_enc.add_and_mask(x, mask)
         bias = self._layers[0].attention_bias(x, mask) if len(self._layers) else None
         for layer in self._layers:
-            x = layer(x, mask, bias)
+            x = layer(x, mask, bias, documents)
         if x.is_cuda and x.dim() == 3 and x.dtype in (torch.float32, torch.bfloat16) and mask.shape == x.shape[:2]:
             return ops.mask_mul(x, mask)
         return x * mask.unsqueeze(-1).to(x.dtype)
@@ -867,12 +939,15 @@ class Decoder(torch.nn.Module, Registrable):
 
 @Decoder.register("nonauto-transformer")
 class TransformerDecoder(Decoder):
-    def __init__(self, input_size, hidden_size, num_layers, num_heads, dropout=0.0, skip_z=False):
+    """`attention`: dict of MultiHeadAttention's score options for every layer; with one of them `decoder` takes rows of
+    several documents and a beginning that every position sees (see ops.biased_attention)"""
+
+    def __init__(self, input_size, hidden_size, num_layers, num_heads, dropout=0.0, skip_z=False, attention=None):
         super().__init__(skip_z)
         self._input_size = input_size
         self._pos_enc = PositionalEncoding(input_size)
         self._layers = torch.nn.ModuleList(
-            [TransformerDecoderLayer(input_size, hidden_size, num_heads, dropout) for _ in range(num_layers)])
+            [TransformerDecoderLayer(input_size, hidden_size, num_heads, dropout, attention) for _ in range(num_layers)])
         self._dropout = _maybe_dropout(dropout)
 
     def get_input_size(self):
@@ -881,11 +956,11 @@ class TransformerDecoder(Decoder):
     def get_output_size(self):
         return self._input_size * (2 if self._skip_z else 1)
 
-    def decoder(self, z, mask):
+    def decoder(self, z, mask, documents=None, prefix=None):
         z = self._pos_enc.add_and_mask(self._dropout(z), mask)
         bias = self._layers[0].attention_bias(z, mask) if len(self._layers) else None
         for layer in self._layers:
-            z = layer(z, mask, bias)
+            z = layer(z, mask, bias, documents, prefix)
         return z
 
 

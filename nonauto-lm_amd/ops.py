@@ -342,34 +342,43 @@ def _qk_norm_rotary_fwd(q, k, args):
     return yq, yk
 
 
+# Both operators' autograd functions take only the tensors that may learn as inputs of their own; the constants come as a dict by
+# the argument struct's names.  What a backward pass reads is saved through save_for_backward, constants too (a constant that
+# is written to between the passes is an error, not a wrong gradient).
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, qw, kw, freqs, positions, args):
+    def forward(ctx, q, k, qw, kw, constants, args):
         yq, yk = _qk_norm_rotary_fwd(q, k, args)
-        ctx.save_for_backward(*((q, k) if args.norm else (None, None)), qw, kw, freqs, positions)
-        ctx.args, ctx.meta = args, (q.shape, k.shape, q.dtype, q.device)      # a rotation alone needs no operands in its backward
+        kept = {"q": q, "k": k} if args.norm else {}         # a rotation alone needs no operands in its backward
+        if qw is not None:
+            kept["q_weight"] = qw
+        if kw is not None:
+            kept["k_weight"] = kw
+        kept.update(constants)
+        ctx.save_for_backward(*kept.values())
+        ctx.names, ctx.args, ctx.meta = tuple(kept), args, (q.shape, k.shape, q.dtype, q.device)
         return yq, yk
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
-        q, k, qw, kw, freqs, positions = ctx.saved_tensors
+        kept = dict(zip(ctx.names, ctx.saved_tensors))
         qs, ks, dtype, dev = ctx.meta
         dyq, dyk = _aligned(dyq), _aligned(dyk)
         dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
         need_qw, need_kw = ctx.needs_input_grad[2:4]
         make = torch.empty_like if dq.numel() else torch.zeros_like
-        dqw, dkw = make(qw) if need_qw else None, make(kw) if need_kw else None
+        dqw, dkw = make(kept["q_weight"]) if need_qw else None, make(kept["k_weight"]) if need_kw else None
         if dq.numel():
             scratch = None
             if need_qw or need_kw:
                 scratch = torch.empty(_buffer_size("mivae_qk_norm_rotary_scratch_floats", ctx.args.head_size),
                                       dtype=torch.float32, device=dev)
-            args = _refill(ctx.args, q=q, k=k, q_weight=qw, k_weight=kw, freq=freqs, positions=positions, dq_out=dyq,
-                           dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw, scratch=scratch)
+            args = _refill(ctx.args, dq_out=dyq, dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw,
+                           scratch=scratch, **kept)
             with L.on_device(dev):
                 L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream_of(dev))
-        return dq, dk, dqw, dkw, None, None, None
+        return dq, dk, dqw, dkw, None, None
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optional[int] = None, *,
@@ -424,7 +433,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optio
     args.rotary_dim = 0 if frequencies is None else 2 * frequencies.numel()
     if not _learns(q, k, q_weight, k_weight):
         return _qk_norm_rotary_fwd(q, k, args)
-    return _QkNormRotary.apply(q, k, q_weight, k_weight, frequencies, positions, args)
+    constants = {n: t for n, t in (("freq", frequencies), ("positions", positions)) if t is not None}
+    return _QkNormRotary.apply(q, k, q_weight, k_weight, constants, args)
 
 
 def relative_buckets(num_buckets: int = 32, max_distance: int = 128, both_sides: bool = True, device=None) -> torch.Tensor:
@@ -445,18 +455,22 @@ def relative_buckets(num_buckets: int = 32, max_distance: int = 128, both_sides:
     return b.to(torch.int32).to(device)
 
 
-def _biased_attention_fwd(q, mask, documents, args, need_lse: bool):
+def _biased_attention_fwd(q, args, need_lse: bool):
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(args.batch, args.heads, args.q_len, dtype=torch.float32, device=dev) if need_lse else None
-    codes = None
-    if mask is not None or documents is not None:
+    args.out = out.data_ptr()
+    lse = codes = None
+    if need_lse:
+        lse = torch.empty(args.batch, args.heads, args.q_len, dtype=torch.float32, device=dev)
+        args.lse = lse.data_ptr()
+    if args.mask or args.documents:
         codes = torch.empty(_buffer_size("mivae_biased_attention_codes_ints", args.batch, args.q_len, args.k_len,
-                                         int(documents is not None)), dtype=torch.int32, device=dev)
+                                         int(bool(args.documents))), dtype=torch.int32, device=dev)
+        args.codes = codes.data_ptr()
     n = _buffer_size("mivae_biased_attention_fwd_floats", args.batch, args.q_len, args.k_len, args.heads, args.kv_heads,
                      args.head_size)
     scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    args.out, args.lse, args.codes, args.scratch = out.data_ptr(), L.ptr(lse), L.ptr(codes), L.ptr(scratch)
+    args.scratch = L.ptr(scratch)
     with L.on_device(dev), _timed("biased_attention_fwd"):
         L.call("mivae_biased_attention_fwd", ctypes.byref(args), L.stream_of(dev))
     return out, lse, codes
@@ -464,32 +478,38 @@ def _biased_attention_fwd(q, mask, documents, args, need_lse: bool):
 
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, args):
-        out, lse, codes = _biased_attention_fwd(q, mask, documents, args, True)
-        ctx.save_for_backward(q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse)
-        ctx.args = args
+    def forward(ctx, q, k, v, table, constants, args):
+        out, lse, codes = _biased_attention_fwd(q, args, True)
+        kept = {"q": q, "k": k, "v": v, "out": out, "lse": lse}
+        if table is not None:
+            kept["table"] = table
+        if codes is not None:
+            kept["codes"] = codes
+        kept.update(constants)
+        ctx.save_for_backward(*kept.values())
+        ctx.names, ctx.args = tuple(kept), args
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, codes, out, lse = ctx.saved_tensors
-        dev, a = q.device, ctx.args
+        kept = dict(zip(ctx.names, ctx.saved_tensors))
+        q, k, a = kept["q"], kept["k"], ctx.args
+        dev, dtype = q.device, q.dtype
         dout = _aligned(dout)
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
+        dq = torch.empty(q.shape, dtype=dtype, device=dev) if need_q else None
         dk = dv = None
         if need_k or need_v:
-            dk, dv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(v.shape, dtype=q.dtype, device=dev)
-        dtable = torch.empty_like(table) if need_t else None
+            dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(kept["v"].shape, dtype=dtype, device=dev)
+        dtable = torch.empty_like(kept["table"]) if need_t else None
         scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.k_len, a.heads,
-                                           a.kv_heads, a.head_size, a.num_buckets if need_t else 0), dtype=torch.float32, device=dev)
-        args = _refill(a, q=q, k=k, v=v, table=table, mask=mask, documents=documents, prefix=prefix, q_starts=q_starts,
-                       slopes=slopes, buckets=buckets, codes=codes, out=out, lse=lse, dout=dout, dq=dq, dk=dk, dv=dv,
-                       dtable=dtable, scratch=scratch)
+                                           a.kv_heads, a.head_size, a.num_buckets if need_t else 0),
+                              dtype=torch.float32, device=dev)
+        args = _refill(a, dout=dout, dq=dq, dk=dk, dv=dv, dtable=dtable, scratch=scratch, **kept)
         with L.on_device(dev), _timed("biased_attention_bwd"):
             L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream_of(dev))
-        return (dq, dk if need_k else None, dv if need_v else None, dtable) + (None,) * 7
+        return dq, dk if need_k else None, dv if need_v else None, dtable, None, None
 
 
 ATTENTION_MAX_LEN = 1 << 24
@@ -589,8 +609,11 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
                  slopes=slopes, table=table, buckets=buckets)
     args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if not _learns(q, k, v, table):
-        return _biased_attention_fwd(q, mask, documents, args, False)[0]
-    return _BiasedAttention.apply(q, k, v, table, mask, documents, prefix, q_starts, slopes, buckets, args)
+        return _biased_attention_fwd(q, args, False)[0]
+    # (mask and documents are read forward only, where they become codes)
+    constants = {n: t for n, t in (("prefix", prefix), ("q_starts", q_starts), ("slopes", slopes), ("buckets", buckets))
+                 if t is not None}
+    return _BiasedAttention.apply(q, k, v, table, constants, args)
 
 
 def segment_sum(tok: torch.Tensor, nseg: int, S: int, add: Optional[torch.Tensor] = None) -> torch.Tensor:
