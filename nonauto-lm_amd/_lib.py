@@ -21,7 +21,7 @@ F64 = ctypes.c_double
 
 class AttentionArgs(ctypes.Structure):
     """mivae_attention_args of include/mivae.h"""
-    _fields_ = ([(n, P) for n in ("q", "k", "v", "out", "lse", "mask", "documents", "prefix", "q_starts", "slopes",
+    _fields_ = ([(n, P) for n in ("q", "k", "v", "out", "out_lo", "lse", "mask", "documents", "prefix", "q_starts", "slopes",
                                   "table", "buckets", "codes", "dout", "dq", "dk", "dv", "dtable", "scratch")]
                 + [(n, I64) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_size")]
                 + [(n, I64 * 3) for n in ("q_stride", "k_stride", "v_stride")]

@@ -23,6 +23,7 @@ struct BiasedArgs {
   const void *q, *k, *v;
   int64_t qs[3], ks[3], vs[3];
   void* out;                    // (B, Sq, heads, d) contiguous
+  unsigned short* out_lo;       // bf16: what the rounding of out leaves, or null
   float* lse;                   // (B, heads, Sq): log2-domain log-sum-exp, +inf for a row that sees no key; may be null
   const void* dout;             // (B, Sq, heads, d) contiguous
   float* delta;                 // (B, heads, Sq): sum_d dout * out
@@ -203,6 +204,15 @@ __device__ __forceinline__ void store4(float* p, float a, float b, float c, floa
   const f32x4 o = {a, b, c, e};
   *reinterpret_cast<f32x4*>(p) = o;
 }
+// four values of the output, and with `lo` what their rounding leaves
+__device__ __forceinline__ void store_out(unsigned short* out, unsigned short* lo, int64_t at, float a, float b, float c, float e) {
+  const u16x4 o = {f32_to_bf16(a), f32_to_bf16(b), f32_to_bf16(c), f32_to_bf16(e)};
+  *reinterpret_cast<u16x4*>(out + at) = o;
+  if (lo != nullptr) store4(lo + at, a - bf16_to_f32(o[0]), b - bf16_to_f32(o[1]), c - bf16_to_f32(o[2]), e - bf16_to_f32(o[3]));
+}
+__device__ __forceinline__ void store_out(float* out, unsigned short*, int64_t at, float a, float b, float c, float e) {
+  store4(out + at, a, b, c, e);
+}
 template <typename T, int NDB>
 __device__ __forceinline__ void store_row(T* dst, const f32x16 (&x)[NDB], float mul, int d, int hh) {
 #pragma unroll
@@ -215,48 +225,62 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&x)[NDB], float 
     }
 }
 
-// Scores of a block in base-2 exponent units.  The raw product x of a pair becomes u = x, or with a cap
-// u = 1 / (1 + e^(-2 y)), y = scale x / cap, tanh y = 2 u - 1 (bf16 operands: absolute error about 1e-7, i.e. cap * 1e-7 in
-// a score; fp32 operands: u from the library's tanhf, a last-place error near 0 too).  The score is then A u + C, A >= 0,
-// plus the bias: linear, so that where the bias is constant over a tile everything folds into the exponential's one fma.
+// Scores of a block in base-2 exponent units.  The raw product x of a pair becomes u = x, or with a cap u = tanh(scale x / cap);
+// the score is then A u, A >= 0, plus the bias: linear, so that where the bias is constant over a tile everything folds into
+// the exponential's one fma.
 struct Score {
-  float A, C, k;      // k: factor of x in the cap's exponent
+  float A, k;         // k = scale / cap
   float slope;        // slope * log2 e
   bool cap, slopes, tab;
 };
 
-__device__ __forceinline__ Score score_of(const BiasedArgs& a, int head, bool fp32) {
+__device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
   Score p;
   p.cap = a.cap > 0.f;
-  p.A = p.cap ? 2.f * a.cap * kLog2e : a.scale * kLog2e;
-  p.C = p.cap ? -a.cap * kLog2e : 0.f;
-  p.k = p.cap ? (fp32 ? a.scale / a.cap : -2.f * kLog2e * a.scale / a.cap) : 0.f;
-  if (p.cap && fp32) { p.A = a.cap * kLog2e; p.C = 0.f; }       // fp32: u = tanh y
+  p.A = (p.cap ? a.cap : a.scale) * kLog2e;
+  p.k = p.cap ? a.scale / a.cap : 0.f;
   p.slopes = a.slopes != nullptr;
   p.slope = p.slopes ? a.slopes[head] * kLog2e : 0.f;
   p.tab = a.table != nullptr;
   return p;
 }
 
-template <typename T>
+// u <- tanh(k u).  Scores well below the cap, the usual case, take y P(y^2) for |y| <= 3/4, P of degree 5 with the smallest
+// largest relative error (fitted on Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where
+// 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  A tile
+// with a larger |y| takes the latter, whose relative error is as small there.
 __device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
+  float most = 0.f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    u[r] = sizeof(T) == 4 ? tanhf(p.k * u[r]) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p.k * u[r]));
+  for (int r = 0; r < 16; ++r) {
+    u[r] *= p.k;
+    most = fmaxf(most, fabsf(u[r]));
+  }
+  if (__builtin_amdgcn_ballot_w64(most > 0.75f) == 0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float t = u[r] * u[r];
+      float q = fmaf(t, -0.00471625663f, 0.0195829067f);
+      q = fmaf(t, q, -0.0533444285f);
+      q = fmaf(t, q, 0.133254066f);
+      q = fmaf(t, q, -0.333329588f);
+      u[r] = fmaf(t * u[r], q, u[r]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      u[r] = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * u[r]));
+  }
 }
-// d score / d x = scale * kCapSlope<T> * cap_slope(u)
-template <typename T>
-__device__ __forceinline__ float cap_slope(float u) { return sizeof(T) == 4 ? fmaf(-u, u, 1.f) : fmaf(-u, u, u); }
-template <typename T>
-__device__ __forceinline__ float cap_slope_factor() { return sizeof(T) == 4 ? 1.f : 4.f; }
+__device__ __forceinline__ float cap_slope(float u) { return fmaf(-u, u, 1.f); }
 
-// Element-wise part: u <- A u + C + bias.  Register r's relative distance key - query is rel + SIGN * acc_row(r) (SIGN = 1: the
+// Element-wise part: u <- A u + bias.  Register r's relative distance key - query is rel + SIGN * acc_row(r) (SIGN = 1: the
 // lane is a query, -1: the lane is a key); rel0 is that of the wave's first lane's row to the tile's first.
 template <int SIGN>
 __device__ __forceinline__ void bias_tile(f32x16& u, const Score& p, const float* tab, int R, int rel, int rel0) {
   const bool behind = rel0 + 31 <= 0, inside = rel0 - 31 >= -R && rel0 + 31 <= R;        // wave-uniform
 #pragma unroll
-  for (int r = 0; r < 16; ++r) u[r] = fmaf(p.A, u[r], p.C);
+  for (int r = 0; r < 16; ++r) u[r] *= p.A;
   if (p.slopes) {
     if (behind) {                       // every key at or behind its query: -slope |rel| is linear in the register's row
       const float base = p.slope * (float)rel;

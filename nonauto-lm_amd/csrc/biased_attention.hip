@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_ba_codes(const int64_t* mask, const int
 
 // ---- delta = sum_d dout * out: 16 lanes per (b, i, head) row -----------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, float* delta, int64_t rows, int Sq, int heads, int d) {
+__global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, const unsigned short* lo, float* delta, int64_t rows, int Sq, int heads, int d) {
   const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int l = threadIdx.x & 15;
   float s = 0.f;
@@ -84,6 +84,11 @@ __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, f
       RowIO<T, 4>::load(out + r * d + c, y);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = fmaf(x[i], y[i], s);
+      if (lo != nullptr) {
+        RowIO<unsigned short, 4>::load(lo + r * d + c, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fmaf(x[i], y[i], s);
+      }
     }
 #pragma unroll
   for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -242,7 +247,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
   const View v = view_of(a, b);
   const KeyWalk walk = key_walk(a, v, b, row0);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
-  const Score sp = score_of(a, head, sizeof(T) == 4);
+  const Score sp = score_of(a, head);
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
@@ -290,9 +295,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     }
     if (sp.cap) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) cap_tile<T>(u[t], sp);
+      for (int t = 0; t < TW; ++t) cap_tile(u[t], sp);
     }
-    float A = sp.A, C = sp.C;
+    float A = sp.A, C = 0.f;
     const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
     if (sees == 1 || sp.slopes || near) {
 #pragma unroll
@@ -302,9 +307,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
         if (sees == 1) hide_keys(u[t], qw, v.codes, key, kc_lds + buf * kChunk + 32 * t + 4 * hh);
       }
       A = 1.f;
-      C = 0.f;
     } else if (sp.tab) {
-      C += tab[rel0 < 0 ? 0 : 2 * a.R];
+      C = tab[rel0 < 0 ? 0 : 2 * a.R];
     }
     float top = u[0][0];
 #pragma unroll
@@ -323,6 +327,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     }
+    // Training on bf16: P is rounded for its product, an error of 2^-9 that o passes on to delta, where it counts as soon as few
+    // keys carry a row.  Chunks with a p of more than about 1/16 of its row also multiply what the rounding leaves.
+    const bool rest = sizeof(T) == 2 && a.out_lo != nullptr &&
+                      __builtin_amdgcn_ballot_w64(8.f * __builtin_amdgcn_exp2f(top - m) > l) != 0;
     const float cm = C - m;
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -340,13 +348,36 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
         o[db] = mma(L::col(vt, 32 * t, db, lane), p0, o[db]);
         o[db] = mma(L::col(vt, 32 * t + 16, db, lane), p1, o[db]);
       }
+      if (rest) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[t][j] -= (float)p0[j];
+          u[t][8 + j] -= (float)p1[j];
+        }
+        pack8(p0, u[t], 0);
+        pack8(p1, u[t], 1);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          o[db] = mma(L::col(vt, 32 * t, db, lane), p0, o[db]);
+          o[db] = mma(L::col(vt, 32 * t + 16, db, lane), p1, o[db]);
+        }
+      }
     }
     l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   }
   l += __shfl_xor(l, 32, 64);           // the half-waves hold disjoint keys of the same query
   if (live) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    store_row<T, NDB>(static_cast<T*>(a.out) + ((b * a.Sq + qw.row) * a.heads + head) * a.d, o, inv, a.d, hh);
+    const int64_t at = ((b * a.Sq + qw.row) * a.heads + head) * a.d;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int a4 = 0; a4 < 4; ++a4) {
+        const int c = 32 * db + 8 * a4 + 4 * hh;
+        if (c < a.d)
+          store_out(static_cast<T*>(a.out), a.out_lo, at + c, o[db][4 * a4] * inv, o[db][4 * a4 + 1] * inv, o[db][4 * a4 + 2] * inv,
+                    o[db][4 * a4 + 3] * inv);
+      }
     if (a.lse && hh == 0)
       a.lse[(b * a.heads + head) * a.Sq + qw.row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
@@ -360,8 +391,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 // registers instead.  The block then folds its four arrays by bucket into one partial row.
 //
 // DELTA: the first half of the same walk, delta_i = sum_j p_ij (do_i . v_j), instead of dout . out.  Needed by the table's
-// gradient on bf16 operands: the o of the forward carries the rounding of P (2^-9 of it, as does its own), which averages
-// out in dq and dk but enters the few values of an fp32 dtable in full (4e-4 of their norm).
+// gradient on bf16 operands: the o of the forward carries what is left of the rounding of P, which averages out in dq and dk
+// but enters the few values of an fp32 dtable in full (4e-4 of their norm with a once rounded P).
 template <typename T, int NDB, bool DELTA>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a) {
   using L = Tile<T, NDB>;
@@ -379,7 +410,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   const View v = view_of(a, b);
   const KeyWalk walk = key_walk(a, v, b, row0);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
-  const Score sp = score_of(a, head, sizeof(T) == 4);
+  const Score sp = score_of(a, head);
   const int TW = 2 * a.R + 1;
   float* hist = tab + TW;                                                 // [kWaves][TW]
   float* mine = hist + wave * TW;
@@ -442,21 +473,20 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       }
       f32x16 g;                          // the cap's slope
       if (sp.cap) {
-        cap_tile<T>(u, sp);
+        cap_tile(u, sp);
         if (!DELTA)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) g[r] = cap_slope<T>(u[r]);
+          for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
       }
-      float A = sp.A, C = sp.C;
+      float A = sp.A, C = 0.f;
       const int rel = key0 + 4 * hh - (v.start + qw.row);
       const bool far = sp.tab && (rel0 + 31 <= -a.R || rel0 - 31 >= a.R);
       if (sees == 1 || sp.slopes || (sp.tab && !far)) {
         bias_tile<1>(u, sp, tab, a.R, rel, rel0);
         if (sees == 1) hide_keys(u, qw, v.codes, key0 + 4 * hh, kc_lds + buf * kChunk + 32 * t + 4 * hh);
         A = 1.f;
-        C = 0.f;
       } else if (sp.tab) {
-        C += tab[rel0 < 0 ? 0 : 2 * a.R];
+        C = tab[rel0 < 0 ? 0 : 2 * a.R];
       }
       const float cm = C - lse;
       if (DELTA) {
@@ -506,8 +536,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     if (live && hh == 0) a.delta[at_l] = dsum;
     return;
   }
-  const float out_scale = a.scale * (sp.cap ? cap_slope_factor<T>() : 1.f);
-  if (live && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, out_scale, a.d, hh);
+  if (live && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, a.scale, a.d, hh);
   if (grad_tab) {
     far_lo = group_sum(far_lo, 64);
     far_hi = group_sum(far_hi, 64);
@@ -628,7 +657,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   Pos p = settle(Pos{share * a.group / split, qfirst});
   if (p.g < glast) issue(0, p);
   int tab_head = -1;
-  Score sp = score_of(a, kvh * a.group, sizeof(T) == 4);
+  Score sp = score_of(a, kvh * a.group);
   for (; p.g < glast; buf ^= NBUF - 1) {
     const Pos at = p;
     const int head = kvh * a.group + at.g;
@@ -642,7 +671,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
       qc_lds[buf * kChunk + threadIdx.x] = pq;
     }
     if (other_head) {
-      sp = score_of(a, head, sizeof(T) == 4);
+      sp = score_of(a, head);
       tab_head = head;
       if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
     }
@@ -676,11 +705,11 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
       }
       f32x16 g;
       if (sp.cap) {
-        cap_tile<T>(u, sp);
+        cap_tile(u, sp);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) g[r] = cap_slope<T>(u[r]);
+        for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
       }
-      float A = sp.A, C = sp.C;
+      float A = sp.A, C = 0.f;
       const int rel0 = k0 - (v.start + q0), rel = key - (v.start + q0 + 4 * hh);        // register r: rel - acc_row(r)
       const bool near = sp.tab && rel0 + 31 > -a.R && rel0 - 31 < a.R;
       if (!clean || sp.slopes || near) {
@@ -695,9 +724,8 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
           }
         }
         A = 1.f;
-        C = 0.f;
       } else if (sp.tab) {
-        C += tab[rel0 < 0 ? 0 : 2 * a.R];
+        C = tab[rel0 < 0 ? 0 : 2 * a.R];
       }
 #pragma unroll
       for (int a4 = 0; a4 < 4; ++a4) {
@@ -729,14 +757,13 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
     }
   }
   if (!ok) return;
-  const float out_scale = a.scale * (sp.cap ? cap_slope_factor<T>() : 1.f);
   const int64_t at = ((b * a.Sk + key) * a.kv + kvh) * a.d;
   if (part == nullptr) {
-    store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, out_scale, a.d, hh);
+    store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, hh);
     store_row<T, NDB>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, hh);
   } else {                              // [split][dk, dv][(B, Sk, kv, d)]
     const int64_t n = (int64_t)a.B * a.Sk * a.kv * a.d;
-    store_row<float, NDB>(part + 2 * share * n + at, dk, out_scale, a.d, hh);
+    store_row<float, NDB>(part + 2 * share * n + at, dk, a.scale, a.d, hh);
     store_row<float, NDB>(part + (2 * share + 1) * n + at, dv, 1.f, a.d, hh);
   }
 }
@@ -828,10 +855,12 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
                   "%s: %lld buckets up to distance %lld: 1 .. %d buckets, distance 1 .. %d", name, (long long)x->num_buckets,
                   (long long)x->distance, kMaxBuckets, kMaxDistance);
   MIVAE_REQUIRE(x->q_starts || (x->q_start >= 0 && x->q_start <= (1 << 24)), "%s: q_start %lld out of range", name, (long long)x->q_start);
+  MIVAE_REQUIRE(aligned16(x->out_lo), "%s: out_lo must be 16-byte aligned", name);
   MIVAE_REQUIRE(!(x->mask || x->documents) || (x->codes && aligned16(x->codes)), "%s: a mask or documents need the codes buffer", name);
   a.q = x->q; a.k = x->k; a.v = x->v;
   for (int i = 0; i < 3; ++i) { a.qs[i] = x->q_stride[i]; a.ks[i] = x->k_stride[i]; a.vs[i] = x->v_stride[i]; }
   a.out = x->out; a.lse = x->lse;
+  a.out_lo = x->dtype == MIVAE_BF16 ? static_cast<unsigned short*>(x->out_lo) : nullptr;
   a.B = (int)x->batch; a.Sq = (int)x->q_len; a.Sk = (int)x->k_len; a.heads = (int)x->heads; a.kv = (int)x->kv_heads;
   a.group = a.heads / a.kv; a.d = (int)x->head_size;
   a.q_start = (int)x->q_start; a.q_starts = x->q_starts; a.prefix = x->prefix; a.causal = x->causal ? 1 : 0;
@@ -927,10 +956,10 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, nblk, a.causal)), dgrid((unsigned)((rows + 15) / 16));
   if (x->dtype == MIVAE_F32)
     hipLaunchKernelGGL((k_ba_delta<float>), dgrid, dim3(256), 0, st, static_cast<const float*>(x->dout),
-                       static_cast<const float*>(x->out), a.delta, rows, a.Sq, a.heads, a.d);
+                       static_cast<const float*>(x->out), nullptr, a.delta, rows, a.Sq, a.heads, a.d);
   else if (!a.dtab)
     hipLaunchKernelGGL((k_ba_delta<unsigned short>), dgrid, dim3(256), 0, st, static_cast<const unsigned short*>(x->dout),
-                       static_cast<const unsigned short*>(x->out), a.delta, rows, a.Sq, a.heads, a.d);
+                       static_cast<const unsigned short*>(x->out), a.out_lo, a.delta, rows, a.Sq, a.heads, a.d);
   else
     by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a); });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (delta)");

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   const bool same = !v.docs || (lo == hi && __builtin_amdgcn_ballot_w64(code < 0) == 0);
   const int begin = split * t.span, end = min(min(begin + t.span, a.Sk), v.limit(last_pos));
   const int clean_end = v.limit(first_pos);                               // every row sees the keys below
-  const Score sp = score_of(a, kvh * a.group, sizeof(T) == 4);
+  const Score sp = score_of(a, kvh * a.group);
   const float slope = sp.slopes ? a.slopes[live ? head : 0] * kLog2e : 0.f;
   float far[2] = {0.f, 0.f};
   auto bias_at = [&](int rel) {
@@ -169,10 +169,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     for (int r = 0; r < 16; ++r) u[r] = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * NDB; ++s) u = mma(L::row(kt, r32, s, hh), qf[s], u);
-    if (sp.cap) cap_tile<T>(u, sp);
+    if (sp.cap) cap_tile(u, sp);
     const int key = key0 + 4 * hh, rel = key - qpos;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) u[r] = fmaf(sp.A, u[r], sp.C);
+    for (int r = 0; r < 16; ++r) u[r] *= sp.A;
     if (sp.slopes) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) u[r] = fmaf(-slope, fabsf((float)(rel + acc_row(r))), u[r]);
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     if (t.part == nullptr) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int64_t i1 = pr / a.group, h1 = kvh * a.group + pr % a.group;
-      store4(static_cast<T*>(a.out) + ((b * a.Sq + i1) * a.heads + h1) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      store_out(static_cast<T*>(a.out), a.out_lo, ((b * a.Sq + i1) * a.heads + h1) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
       if (a.lse && c == 0) a.lse[(b * a.heads + h1) * a.Sq + i1] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
     } else {
       float* p = t.part + (((int64_t)pair * t.rows + pr) * t.splits + split) * (a.d + 4);
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(64) void k_token_join(TokenArgs t) {
   const int64_t pos = row / a.group, head = pair % a.kv * a.group + row % a.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (lane < lpg && c < a.d)
-    store4(static_cast<T*>(a.out) + ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    store_out(static_cast<T*>(a.out), a.out_lo, ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
   if (a.lse && lane == 0) a.lse[(b * a.heads + head) * a.Sq + pos] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 

@@ -479,8 +479,12 @@ def _biased_attention_fwd(q, args, need_lse: bool):
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, constants, args):
+        kept = {}
+        if q.dtype == torch.bfloat16 and not ctx.needs_input_grad[3]:       # (the table's gradient sums dout.out over the keys anew)
+            kept["out_lo"] = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            args.out_lo = kept["out_lo"].data_ptr()
         out, lse, codes = _biased_attention_fwd(q, args, True)
-        kept = {"q": q, "k": k, "v": v, "out": out, "lse": lse}
+        kept.update(q=q, k=k, v=v, out=out, lse=lse)
         if table is not None:
             kept["table"] = table
         if codes is not None:
