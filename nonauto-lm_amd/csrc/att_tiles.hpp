@@ -249,16 +249,19 @@ __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
 // largest relative error (fitted on Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where
 // 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  A tile
 // with a larger |y| takes the latter, whose relative error is as small there.
-__device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
-  float most = 0.f;
+// `rough`: always the latter (bf16 without gradients, where cap * 1e-7 is far below the output's own rounding).
+__device__ __forceinline__ void cap_tile(f32x16& u, const Score& p, bool rough = false) {
+  float most = 1.f;
+  if (!rough) {
+    most = 0.f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    u[r] *= p.k;
-    most = fmaxf(most, fabsf(u[r]));
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(u[r]));
+    most *= p.k;
   }
   if (__builtin_amdgcn_ballot_w64(most > 0.75f) == 0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
+      u[r] *= p.k;
       const float t = u[r] * u[r];
       float q = fmaf(t, -0.00471625663f, 0.0195829067f);
       q = fmaf(t, q, -0.0533444285f);
@@ -269,7 +272,7 @@ __device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      u[r] = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * u[r]));
+      u[r] = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * p.k * u[r])), 1.f);
   }
 }
 __device__ __forceinline__ float cap_slope(float u) { return fmaf(-u, u, 1.f); }

@@ -100,37 +100,68 @@ __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, c
 }
 
 // ---- what a block knows about visibility -------------------------------------------------------------------------------
-// The walk of a block of queries over the keys in chunks of kChunk, shared by the forward and the dq kernel.
-struct KeyWalk {
-  int end;                // no query of the block sees a key at or beyond it
-  int lo, hi;             // range of the block's query codes
-  const i32x4* tiles;     // of this batch row, or null
-  __device__ __forceinline__ int next(int kc) const {
-    if (tiles != nullptr)
-      while (kc < end) {
-        const i32x4 t = tiles[kc / kChunk];
-        if (t[1] >= lo && t[0] <= hi) break;
-        kc += kChunk;
-      }
-    return kc;
+// The chunks of kChunk rows of a batch row that a block has to walk: all of them, or with codes those whose range of codes meets
+// the block's.  A wave looks at the summaries of 64 chunks at once, one per lane, and keeps them: one load per 4096 rows (chunk
+// after chunk, a block far down a row of packed documents waited for up to 60 loads in a row before its first product).
+struct Walk {
+  const i32x4* tiles;     // summaries of this batch row, or null
+  int n, end;             // rows, and the limit of the walk
+  int lo, hi;             // range of the block's codes
+  int base;
+  i32x4 mine;
+  uint64_t meets;
+  __device__ __forceinline__ void init(const i32x4* t, int rows, int limit, int low, int high) {
+    tiles = t; n = rows; end = limit; lo = low; hi = high;
+    base = -64;
+    meets = 0;
+    mine = i32x4{0, 0, 0, 0};
   }
-  __device__ __forceinline__ uint64_t rows(int kc, int Sk) const {       // the keys of a chunk that are not hidden
-    return tiles != nullptr ? rows_of(tiles[kc / kChunk]) : low_rows(Sk - kc);
+  // first chunk at or behind row c that counts, or something >= end; its summary.  All lanes of the wave have to be active.
+  __device__ __forceinline__ int next(int c, i32x4& info) {
+    if (tiles == nullptr) {
+      const uint64_t rows = low_rows(n - c);
+      info = i32x4{0, 0, (int)(unsigned)rows, (int)(unsigned)(rows >> 32)};
+      return c;
+    }
+    while (c < end) {
+      const int t = c / kChunk;
+      if (t >= base + 64 || t < base) {
+        base = t & ~63;
+        const int at = base + (int)(threadIdx.x & 63);
+        const bool in = at * kChunk < end;
+        mine = in ? tiles[at] : i32x4{INT32_MAX, -1, 0, 0};
+        meets = __builtin_amdgcn_ballot_w64(in && mine[1] >= lo && mine[0] <= hi);
+      }
+      const uint64_t left = meets >> (t - base);
+      if (left != 0) {
+        const int at = t - base + __builtin_ctzll(left);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) info[i] = __builtin_amdgcn_readlane(mine[i], at);
+        return (base + at) * kChunk;
+      }
+      c = (base + 64) * kChunk;
+    }
+    return c;
   }
 };
 
-__device__ __forceinline__ KeyWalk key_walk(const BiasedArgs& a, const View& v, int64_t b, int row0) {
-  KeyWalk w;
-  w.end = v.limit(min(row0 + kRows, a.Sq) - 1);
-  w.lo = w.hi = 0;
-  w.tiles = v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr;
-  if (v.docs) {
-    const i32x4* t = a.qtiles + b * (a.qpad / 64);
-    i32x4 r = t[row0 / 64];
-    if (row0 + 64 < a.Sq) r = merge(r, t[row0 / 64 + 1]);
-    w.lo = r[0];
-    w.hi = r[1];
+// codes of the block's rows [row0, row0 + kRows), from the summaries of n rows
+__device__ __forceinline__ void block_range(const i32x4* tiles, int row0, int n, int& lo, int& hi) {
+  i32x4 r = tiles[row0 / 64];
+  if (row0 + 64 < n) {
+    const i32x4 t = tiles[row0 / 64 + 1];
+    r[0] = min(r[0], t[0]);
+    r[1] = max(r[1], t[1]);
   }
+  lo = r[0];
+  hi = r[1];
+}
+
+__device__ __forceinline__ Walk key_walk(const BiasedArgs& a, const View& v, int64_t b, int row0) {
+  Walk w;
+  int lo = 0, hi = 0;
+  if (v.docs) block_range(a.qtiles + b * (a.qpad / 64), row0, a.Sq, lo, hi);
+  w.init(v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr, a.Sk, v.limit(min(row0 + kRows, a.Sq) - 1), lo, hi);
   return w;
 }
 
@@ -139,17 +170,12 @@ struct QueryWave {
   int row, limit;               // the lane's query
   int first, last;              // limits of the wave's first and last query
   int code, lo, hi;             // the lane's code and the wave's range
-  bool none;                    // some lane's query sees nothing
-  // 0: nothing of the chunk, 1: some of its pairs, 2: all of them
-  __device__ __forceinline__ int sees(const KeyWalk& w, int kc) const {
-    if (kc >= last) return 0;
-    bool all = kc + kChunk <= first;
-    if (w.tiles != nullptr) {
-      const i32x4 t = w.tiles[kc / kChunk];
-      if (t[1] < lo || t[0] > hi) return 0;
-      all = all && rows_of(t) == ~0ull && !none && lo == hi && t[0] == lo && t[1] == lo;
-    }
-    return all ? 2 : 1;
+  bool none, codes;             // some lane's query sees nothing; pairs are compared by codes
+  // 0: nothing of the chunk, 1: its pairs below the limit, 2: those of equal codes too, 3: all of them
+  __device__ __forceinline__ int sees(int kc, const i32x4& t) const {
+    if (kc >= last || t[1] < lo || t[0] > hi) return 0;
+    if (rows_of(t) != ~0ull || none || lo != hi || t[0] != lo || t[1] != lo) return codes ? 2 : 1;
+    return kc + kChunk <= first ? 3 : 1;
   }
 };
 
@@ -161,6 +187,7 @@ __device__ __forceinline__ QueryWave query_wave(const BiasedArgs& a, const View&
   w.last = q0 < a.Sq ? v.limit(min(q0 + 32, a.Sq) - 1) : 0;
   w.code = w.lo = w.hi = 0;
   w.none = false;
+  w.codes = v.codes;
   if (v.docs) {
     w.code = w.row < a.qpad ? a.qcodes[b * a.qpad + w.row] : kNoCode;
     wave_range(w.code, w.lo, w.hi);
@@ -245,7 +272,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
   const int64_t b = id.b;
   const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
-  const KeyWalk walk = key_walk(a, v, b, row0);
+  Walk walk = key_walk(a, v, b, row0);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
   const Score sp = score_of(a, head);
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
@@ -264,13 +291,14 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
   // Two LDS buffers with bf16: the next chunk is on its way while one is multiplied, one barrier per chunk.
   Stage<T, NDB, kWaves> sk, sv;
   int pc = 0, buf = 0;
+  i32x4 info = {0, 0, 0, 0};             // of the chunk on its way
   auto issue = [&](int n, int kc) {
-    const uint64_t rows = walk.rows(kc, a.Sk);
+    const uint64_t rows = rows_of(info);
     sk.issue(tiles + 2 * n * TILE, kbase, a.ks[1], kc, rows, a.d);
     sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0);
+  int kc = walk.next(0, info);
   if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
     if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
@@ -279,9 +307,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     if (v.codes && threadIdx.x < kChunk) kc_lds[buf * kChunk + threadIdx.x] = pc;
     __syncthreads();
     const int at = kc;
-    kc = walk.next(kc + kChunk);
+    const i32x4 seen = info;
+    kc = walk.next(kc + kChunk, info);
     if (kc < walk.end) issue(buf ^ (NBUF - 1), kc);
-    const int sees = qw.sees(walk, at); // wave-uniform, like every branch below
+    const int sees = qw.sees(at, seen); // wave-uniform, like every branch below
     if (sees == 0) continue;
     const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
     const int rel0 = at - (v.start + q0);                       // the wave's first query to the chunk's first key
@@ -295,16 +324,16 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     }
     if (sp.cap) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) cap_tile(u[t], sp);
+      for (int t = 0; t < TW; ++t) cap_tile(u[t], sp, sizeof(T) == 2 && a.lse == nullptr);
     }
     float A = sp.A, C = 0.f;
     const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
-    if (sees == 1 || sp.slopes || near) {
+    if (sees < 3 || sp.slopes || near) {
 #pragma unroll
       for (int t = 0; t < TW; ++t) {
         const int key = at + 32 * t + 4 * hh;
         bias_tile<1>(u[t], sp, tab, a.R, key - (v.start + qw.row), rel0 + 32 * t);
-        if (sees == 1) hide_keys(u[t], qw, v.codes, key, kc_lds + buf * kChunk + 32 * t + 4 * hh);
+        if (sees < 3) hide_keys(u[t], qw, sees == 2, key, kc_lds + buf * kChunk + 32 * t + 4 * hh);
       }
       A = 1.f;
     } else if (sp.tab) {
@@ -408,7 +437,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   const int64_t b = id.b;
   const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
-  const KeyWalk walk = key_walk(a, v, b, row0);
+  Walk walk = key_walk(a, v, b, row0);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
   const Score sp = score_of(a, head);
   const int TW = 2 * a.R + 1;
@@ -439,13 +468,14 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   float far_lo = 0.f, far_hi = 0.f;
   Stage<T, NDB, kWaves> sk, sv;
   int pc = 0, buf = 0;
+  i32x4 info = {0, 0, 0, 0};             // of the chunk on its way
   auto issue = [&](int n, int kc) {
-    const uint64_t rows = walk.rows(kc, a.Sk);
+    const uint64_t rows = rows_of(info);
     sk.issue(tiles + 2 * n * TILE, kbase, a.ks[1], kc, rows, a.d);
     sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0);
+  int kc = walk.next(0, info);
   if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
     if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
@@ -454,9 +484,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     if (v.codes && threadIdx.x < kChunk) kc_lds[buf * kChunk + threadIdx.x] = pc;
     __syncthreads();
     const int at = kc;
-    kc = walk.next(kc + kChunk);
+    const i32x4 seen = info;
+    kc = walk.next(kc + kChunk, info);
     if (kc < walk.end) issue(buf ^ (NBUF - 1), kc);
-    const int sees = qw.sees(walk, at);
+    const int sees = qw.sees(at, seen);
     if (sees == 0) continue;
     const T *kt = tiles + 2 * buf * TILE, *vt = kt + TILE;
 #pragma unroll
@@ -481,9 +512,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       float A = sp.A, C = 0.f;
       const int rel = key0 + 4 * hh - (v.start + qw.row);
       const bool far = sp.tab && (rel0 + 31 <= -a.R || rel0 - 31 >= a.R);
-      if (sees == 1 || sp.slopes || (sp.tab && !far)) {
+      if (sees < 3 || sp.slopes || (sp.tab && !far)) {
         bias_tile<1>(u, sp, tab, a.R, rel, rel0);
-        if (sees == 1) hide_keys(u, qw, v.codes, key0 + 4 * hh, kc_lds + buf * kChunk + 32 * t + 4 * hh);
+        if (sees < 3) hide_keys(u, qw, sees == 2, key0 + 4 * hh, kc_lds + buf * kChunk + 32 * t + 4 * hh);
         A = 1.f;
       } else if (sp.tab) {
         C = tab[rel0 < 0 ? 0 : 2 * a.R];
@@ -607,24 +638,17 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   const int first = v.first_row(key);                                     // the lane's key is seen from this row on
   const int wfirst = v.first_row(k0), wall = v.first_row(min(k0 + 31, a.Sk - 1));        // some / every key of the wave
   const int qfirst = v.first_row(row0) / kChunk * kChunk;
-  i32x4 br = {0, 0, 0, 0};
-  if (v.codes) {
-    const i32x4* t = a.ktiles + b * (a.kpad / 64);
-    br = t[row0 / 64];
-    if (row0 + 64 < a.Sk) br = merge(br, t[row0 / 64 + 1]);
-  }
-  const i32x4* qtiles = v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr;
+  int blo = 0, bhi = 0;
+  if (v.codes) block_range(a.ktiles + b * (a.kpad / 64), row0, a.Sk, blo, bhi);
+  Walk walk;
+  walk.init(v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr, a.Sq, a.Sq, blo, bhi);
   // next chunk of queries of the group's heads that the block's keys may be seen from
-  const int glast = (share + 1) * a.group / split;
+  const int glast = bhi < 0 ? 0 : (share + 1) * a.group / split;          // (every key of the block hidden: none)
   struct Pos { int g, qc; };
+  i32x4 info = {0, 0, 0, 0};             // of the chunk on its way
   auto settle = [&](Pos p) {
     while (p.g < glast) {
-      if (br[1] < 0) { p.g = glast; break; }                             // every key of the block is hidden
-      while (qtiles != nullptr && p.qc < a.Sq) {
-        const i32x4 t = qtiles[p.qc / kChunk];
-        if (t[1] >= br[0] && t[0] <= br[1]) break;
-        p.qc += kChunk;
-      }
+      p.qc = walk.next(p.qc, info);
       if (p.qc < a.Sq) break;
       p.g += 1;
       p.qc = qfirst;
@@ -644,7 +668,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   int pq = 0, buf = 0;
   auto issue = [&](int n, Pos p) {
     const int head = kvh * a.group + p.g;
-    const uint64_t rows = low_rows(a.Sq - p.qc);
+    const uint64_t rows = low_rows(a.Sq - p.qc);       
     sq.issue(tiles + 2 * n * TILE, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, rows, a.d);
     sd.issue(tiles + (2 * n + 1) * TILE, static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d,
              (int64_t)a.heads * a.d, p.qc, rows, a.d);
@@ -676,16 +700,16 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
       if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
     }
     __syncthreads();
+    const i32x4 seen = info;
     p = settle(Pos{p.g, p.qc + kChunk});
     if (p.g < glast) issue(buf ^ (NBUF - 1), p);
     if (k0 >= a.Sk || at.qc + kChunk <= wfirst) continue;
     bool clean = !khid && at.qc >= wall;
-    if (v.docs) {
-      const i32x4 ts = qtiles[at.qc / kChunk];
-      if (ts[1] < klo || ts[0] > khi) continue;
-      clean = clean && rows_of(ts) == ~0ull && ts[0] == ts[1] && klo == khi && ts[0] == klo;
-    } else if (v.codes && khi < 0) {
-      continue;
+    bool codes = false;                 // pairs have to be compared by codes
+    if (v.codes) {
+      if (khi < 0 || seen[1] < klo || seen[0] > khi) continue;
+      codes = v.docs && (rows_of(seen) != ~0ull || seen[0] != seen[1] || klo != khi || seen[0] != klo);
+      clean = clean && !codes && klo == khi;
     }
     const T *qt = tiles + 2 * buf * TILE, *dt = qt + TILE;
     const float *ls = lses + buf * kChunk, *de = dels + buf * kChunk;
@@ -719,7 +743,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             bool see = acc_row(r) >= from;
-            if (v.docs) see = see && qcs[32 * t + 4 * hh + acc_row(r)] == kcode;
+            if (codes) see = see && qcs[32 * t + 4 * hh + acc_row(r)] == kcode;
             u[r] = see ? u[r] : -INFINITY;
           }
         }
