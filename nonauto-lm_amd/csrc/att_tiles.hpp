@@ -249,16 +249,17 @@ __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
 // largest relative error (fitted on Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where
 // 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  A tile
 // with a larger |y| takes the latter, whose relative error is as small there.
-// `rough`: always the latter (bf16 without gradients, where cap * 1e-7 is far below the output's own rounding).
-__device__ __forceinline__ void cap_tile(f32x16& u, const Score& p, bool rough = false) {
-  float most = 1.f;
-  if (!rough) {
-    most = 0.f;
+// ROUGH: always the latter (bf16 without gradients, where cap * 1e-7 is far below the output's own rounding), in one
+// basic block with the products around it.
+template <bool ROUGH>
+__device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
+  float most = 0.f;
+  if (!ROUGH) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(u[r]));
     most *= p.k;
   }
-  if (__builtin_amdgcn_ballot_w64(most > 0.75f) == 0) {
+  if (!ROUGH && __builtin_amdgcn_ballot_w64(most > 0.75f) == 0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       u[r] *= p.k;

@@ -258,7 +258,12 @@ __device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool causal, b
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-template <typename T, int NDB>
+// kInfer: no lse, bf16 with the rough tanh.  kTrain: lse.  kTrainRest (bf16): also the rounding's rest of large probabilities and
+// the output's residue, for delta = dout . out.  (Modes, not branches: a branch between the products and the exponentials
+// of a chunk keeps them from overlapping, 7 % at 8191 queries of 128.)
+enum Mode { kInfer, kTrain, kTrainRest };
+
+template <typename T, int NDB, Mode MODE>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(BiasedArgs a) {
   using L = Tile<T, NDB>;
   constexpr int TW = kChunk / 32, TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     }
     if (sp.cap) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) cap_tile(u[t], sp, sizeof(T) == 2 && a.lse == nullptr);
+      for (int t = 0; t < TW; ++t) cap_tile<sizeof(T) == 2 && MODE == kInfer>(u[t], sp);
     }
     float A = sp.A, C = 0.f;
     const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
@@ -356,10 +361,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     }
-    // Training on bf16: P is rounded for its product, an error of 2^-9 that o passes on to delta, where it counts as soon as few
-    // keys carry a row.  Chunks with a p of more than about 1/16 of its row also multiply what the rounding leaves.
-    const bool rest = sizeof(T) == 2 && a.out_lo != nullptr &&
-                      __builtin_amdgcn_ballot_w64(8.f * __builtin_amdgcn_exp2f(top - m) > l) != 0;
+    // P is rounded to bf16 for its product, an error of 2^-9 that o passes on to delta, where it counts as soon as few keys
+    // carry a row.  Chunks with a p of more than about 1/16 of its row also multiply what the rounding leaves.
+    const bool rest = MODE == kTrainRest && __builtin_amdgcn_ballot_w64(8.f * __builtin_amdgcn_exp2f(top - m) > l) != 0;
     const float cm = C - m;
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -404,10 +408,10 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
       for (int a4 = 0; a4 < 4; ++a4) {
         const int c = 32 * db + 8 * a4 + 4 * hh;
         if (c < a.d)
-          store_out(static_cast<T*>(a.out), a.out_lo, at + c, o[db][4 * a4] * inv, o[db][4 * a4 + 1] * inv, o[db][4 * a4 + 2] * inv,
+          store_out(static_cast<T*>(a.out), MODE == kTrainRest ? a.out_lo : nullptr, at + c, o[db][4 * a4] * inv, o[db][4 * a4 + 1] * inv, o[db][4 * a4 + 2] * inv,
                     o[db][4 * a4 + 3] * inv);
       }
-    if (a.lse && hh == 0)
+    if (MODE != kInfer && hh == 0)
       a.lse[(b * a.heads + head) * a.Sq + qw.row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
 }
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       }
       f32x16 g;                          // the cap's slope
       if (sp.cap) {
-        cap_tile(u, sp);
+        cap_tile<false>(u, sp);
         if (!DELTA)
 #pragma unroll
           for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
@@ -729,7 +733,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
       }
       f32x16 g;
       if (sp.cap) {
-        cap_tile(u, sp);
+        cap_tile<false>(u, sp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
       }
@@ -879,7 +883,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
                   "%s: %lld buckets up to distance %lld: 1 .. %d buckets, distance 1 .. %d", name, (long long)x->num_buckets,
                   (long long)x->distance, kMaxBuckets, kMaxDistance);
   MIVAE_REQUIRE(x->q_starts || (x->q_start >= 0 && x->q_start <= (1 << 24)), "%s: q_start %lld out of range", name, (long long)x->q_start);
-  MIVAE_REQUIRE(aligned16(x->out_lo), "%s: out_lo must be 16-byte aligned", name);
+  MIVAE_REQUIRE(aligned16(x->out_lo) && !(x->out_lo && !x->lse), "%s: out_lo must be 16-byte aligned and needs lse", name);
   MIVAE_REQUIRE(!(x->mask || x->documents) || (x->codes && aligned16(x->codes)), "%s: a mask or documents need the codes buffer", name);
   a.q = x->q; a.k = x->k; a.v = x->v;
   for (int i = 0; i < 3; ++i) { a.qs[i] = x->q_stride[i]; a.ks[i] = x->k_stride[i]; a.vs[i] = x->v_stride[i]; }
@@ -951,7 +955,11 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
   }
   const size_t lds = tile_bytes(x->dtype, a.d, 1) + (a.table ? (2 * a.R + 1) * 4 : 0);
   const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, (a.Sq + kRows - 1) / kRows, a.causal));
-  by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_fwd<decltype(t), n()>, grid, lds, S_(stream), a); });
+  by_shape(x->dtype, a.d, [&](auto t, auto n) {
+    if (a.out_lo) start(k_ba_fwd<unsigned short, n(), kTrainRest>, grid, lds, S_(stream), a);        // bf16 alone has it
+    else if (a.lse) start(k_ba_fwd<decltype(t), n(), kTrain>, grid, lds, S_(stream), a);
+    else start(k_ba_fwd<decltype(t), n(), kInfer>, grid, lds, S_(stream), a);
+  });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd");
   return MIVAE_OK;
 }

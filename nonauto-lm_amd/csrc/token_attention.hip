@@ -169,7 +169,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     for (int r = 0; r < 16; ++r) u[r] = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * NDB; ++s) u = mma(L::row(kt, r32, s, hh), qf[s], u);
-    if (sp.cap) cap_tile(u, sp, sizeof(T) == 2 && a.lse == nullptr);
+    if (sp.cap) {
+      if (sizeof(T) == 2 && a.lse == nullptr) cap_tile<true>(u, sp);
+      else cap_tile<false>(u, sp);
+    }
     const int key = key0 + 4 * hh, rel = key - qpos;
 #pragma unroll
     for (int r = 0; r < 16; ++r) u[r] *= sp.A;
