@@ -363,4 +363,20 @@ __device__ __forceinline__ float max_halves(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Issue order for a run of N bf16 products whose A operands take DS LDS reads each: the reads stay two products ahead of the
+// matrix core.  (The compiler's own order waits for the LDS before most products.)  A no-op for fp32.
+template <typename T, int N, int DS>
+__device__ __forceinline__ void reads_ahead() {
+  if (sizeof(T) == 2 && N > 2) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * DS, 0);
+#pragma unroll
+    for (int i = 0; i < N - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 }  // namespace mivae

@@ -116,6 +116,12 @@ struct Walk {
     meets = 0;
     mine = i32x4{0, 0, 0, 0};
   }
+  // keeps part i of n equal ones (in chunks) of the walk; its first row
+  __device__ __forceinline__ int take(int i, int n) {
+    const int chunks = (end + kChunk - 1) / kChunk, from = chunks * i / n * kChunk;
+    end = min(end, chunks * (i + 1) / n * kChunk);
+    return from;
+  }
   // first chunk at or behind row c that counts, or something >= end; its summary.  All lanes of the wave have to be active.
   __device__ __forceinline__ int next(int c, i32x4& info) {
     if (tiles == nullptr) {
@@ -263,8 +269,10 @@ __device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool causal, b
 // of a chunk keeps them from overlapping, 7 % at 8191 queries of 128.)
 enum Mode { kInfer, kTrain, kTrainRest };
 
+// slices > 1: a block takes one of that many equal parts of its rows' walk and leaves (O, max, sum) in `part`, laid out for
+// token_attention_join.
 template <typename T, int NDB, Mode MODE>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(BiasedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(BiasedArgs a, int slices, float* part) {
   using L = Tile<T, NDB>;
   constexpr int TW = kChunk / 32, TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -272,12 +280,13 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
   int* kc_lds = reinterpret_cast<int*>(tiles + 2 * NBUF * TILE);          // [NBUF][kChunk]
   float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const Ids id = ids_of(a.B, a.heads, (a.Sq + kRows - 1) / kRows, a.causal != 0, true);
+  const Ids id = ids_of(a.B, a.heads * slices, (a.Sq + kRows - 1) / kRows, a.causal != 0, true);
   if (id.none) return;
   const int64_t b = id.b;
-  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
+  const int head = id.head / slices, slice = id.head % slices, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
   Walk walk = key_walk(a, v, b, row0);
+  const int begin = walk.take(slice, slices);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
   const Score sp = score_of(a, head);
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
@@ -303,7 +312,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0, info);
+  int kc = walk.next(begin, info);
   if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
     if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
@@ -399,7 +408,14 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
   }
   l += __shfl_xor(l, 32, 64);           // the half-waves hold disjoint keys of the same query
-  if (live) {
+  if (live && part != nullptr) {
+    float* p = part + (((b * a.heads + head) * a.Sq + qw.row) * slices + slice) * (a.d + 4);
+    store_row<float, NDB>(p, o, 1.f, a.d, hh);
+    if (hh == 0) {
+      p[a.d] = m;
+      p[a.d + 1] = l;
+    }
+  } else if (live) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t at = ((b * a.Sq + qw.row) * a.heads + head) * a.d;
 #pragma unroll
@@ -423,11 +439,13 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 // 190 cycles each: 686 us instead of the SKEW_US at 4 x 16 x 4096^2.)  Tiles at or beyond distance R go to two
 // registers instead.  The block then folds its four arrays by bucket into one partial row.
 //
+// slices > 1: as in the forward; dq (or delta) then goes to `part` [slice][..] in fp32 and k_ba_fold sums the slices in order.
+//
 // DELTA: the first half of the same walk, delta_i = sum_j p_ij (do_i . v_j), instead of dout . out.  Needed by the table's
 // gradient on bf16 operands: the o of the forward carries what is left of the rounding of P, which averages out in dq and dk
 // but enters the few values of an fp32 dtable in full (4e-4 of their norm with a once rounded P).
 template <typename T, int NDB, bool DELTA>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a, int slices, float* part) {
   using L = Tile<T, NDB>;
   constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -436,12 +454,13 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   float* tab = reinterpret_cast<float*>(kc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
   const int nblk = (a.Sq + kRows - 1) / kRows;
-  const Ids id = ids_of(a.B, a.heads, nblk, a.causal != 0, true);
+  const Ids id = ids_of(a.B, a.heads * slices, nblk, a.causal != 0, true);
   if (id.none) return;
   const int64_t b = id.b;
-  const int head = id.head, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
+  const int head = id.head / slices, slice = id.head % slices, kvh = head / a.group, row0 = id.blk * kRows, q0 = row0 + 32 * wave;
   const View v = view_of(a, b);
   Walk walk = key_walk(a, v, b, row0);
+  const int begin = walk.take(slice, slices);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
   const Score sp = score_of(a, head);
   const int TW = 2 * a.R + 1;
@@ -479,7 +498,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     sv.issue(tiles + (2 * n + 1) * TILE, vbase, a.vs[1], kc, rows, a.d);
     if (v.codes && threadIdx.x < kChunk) pc = codes[kc + threadIdx.x];
   };
-  int kc = walk.next(0, info);
+  int kc = walk.next(begin, info);
   if (kc < walk.end) issue(0, kc);
   for (; kc < walk.end; buf ^= NBUF - 1) {
     if (NBUF == 1) __syncthreads();     // the previous chunk has been consumed
@@ -506,6 +525,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
         u = mma(L::row(kt, 32 * t + r32, s, hh), qf[s], u);
         dp = mma(L::row(vt, 32 * t + r32, s, hh), dof[s], dp);
       }
+      reads_ahead<T, 4 * NDB, 1>();
       f32x16 g;                          // the cap's slope
       if (sp.cap) {
         cap_tile<false>(u, sp);
@@ -559,19 +579,24 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       typename Frag<T>::type d0, d1;
       pack8(d0, u, 0);
       pack8(d1, u, 1);
+      if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         dq[db] = mma(L::col(kt, 32 * t, db, lane), d0, dq[db]);
         dq[db] = mma(L::col(kt, 32 * t + 16, db, lane), d1, dq[db]);
       }
+      reads_ahead<T, 2 * NDB, 2>();
     }
   }
   if (DELTA) {
     dsum += __shfl_xor(dsum, 32, 64);
-    if (live && hh == 0) a.delta[at_l] = dsum;
+    if (live && hh == 0) (part != nullptr ? part + slice * (((int64_t)a.B * a.heads * a.Sq + 3) / 4 * 4) : a.delta)[at_l] = dsum;
     return;
   }
-  if (live && a.dq) store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, a.scale, a.d, hh);
+  if (live && a.dq) {
+    if (part != nullptr) store_row<float, NDB>(part + (int64_t)slice * a.B * a.Sq * a.heads * a.d + at_q, dq, a.scale, a.d, hh);
+    else store_row<T, NDB>(static_cast<T*>(a.dq) + at_q, dq, a.scale, a.d, hh);
+  }
   if (grad_tab) {
     far_lo = group_sum(far_lo, 64);
     far_hi = group_sum(far_hi, 64);
@@ -597,7 +622,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       for (int i = threadIdx.x % lanes; i < TW; i += lanes) s += ids[i] == n ? hist[i] : 0.f;
       s = group_sum(s, lanes);
       if (threadIdx.x % lanes == 0 && n < a.nb)
-        a.dtab[((int64_t)head * a.B * nblk + b * nblk + id.blk) * a.nb + n] = s;
+        a.dtab[(((int64_t)head * a.B * nblk + b * nblk + id.blk) * slices + slice) * a.nb + n] = s;
     }
   }
 }
@@ -613,10 +638,10 @@ __global__ __launch_bounds__(64) void k_ba_dtable(const float* part, float* dtab
 }
 
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------
-// A block's walk over the queries of all heads of a group.  Where key heads are few, `split` blocks share a group's heads
-// and leave fp32 partials that k_ba_fold sums in order.
+// A block's walk over the queries of all heads of a group.  Where there are few blocks, `split` blocks share a group's heads and
+// each share's queries are cut into `cuts` equal parts; they leave fp32 partials that k_ba_fold sums in order.
 template <typename T, int NDB>
-__global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, float* part) {
+__global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, int cuts, float* part) {
   using L = Tile<T, NDB>;
   constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -626,10 +651,10 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   int* qc_lds = reinterpret_cast<int*>(dels + NBUF * kChunk);
   float* tab = reinterpret_cast<float*>(qc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
-  const Ids id = ids_of(a.B, a.kv * split, (a.Sk + kRows - 1) / kRows, a.causal != 0, false);
+  const Ids id = ids_of(a.B, a.kv * split * cuts, (a.Sk + kRows - 1) / kRows, a.causal != 0, false);
   if (id.none) return;
   const int64_t b = id.b;
-  const int kvh = id.head / split, share = id.head % split, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
+  const int kvh = id.head / (split * cuts), piece = id.head % (split * cuts), share = piece / cuts, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
   const View v = view_of(a, b);
   const bool ok = key < a.Sk;
   const int kcode = !ok ? -1 : v.codes ? a.kcodes[b * a.kpad + key] : 0;
@@ -641,11 +666,14 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   }
   const int first = v.first_row(key);                                     // the lane's key is seen from this row on
   const int wfirst = v.first_row(k0), wall = v.first_row(min(k0 + 31, a.Sk - 1));        // some / every key of the wave
-  const int qfirst = v.first_row(row0) / kChunk * kChunk;
+  // the queries from the first that sees a key of the block on, cut into equal parts of whole chunks
+  const int first_chunk = v.first_row(row0) / kChunk, chunks = max(0, (a.Sq + kChunk - 1) / kChunk - first_chunk);
+  const int qfirst = (first_chunk + chunks * (piece % cuts) / cuts) * kChunk;
+  const int qend = min(a.Sq, (first_chunk + chunks * (piece % cuts + 1) / cuts) * kChunk);
   int blo = 0, bhi = 0;
   if (v.codes) block_range(a.ktiles + b * (a.kpad / 64), row0, a.Sk, blo, bhi);
   Walk walk;
-  walk.init(v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr, a.Sq, a.Sq, blo, bhi);
+  walk.init(v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr, a.Sq, qend, blo, bhi);
   // next chunk of queries of the group's heads that the block's keys may be seen from
   const int glast = bhi < 0 ? 0 : (share + 1) * a.group / split;          // (every key of the block hidden: none)
   struct Pos { int g, qc; };
@@ -653,7 +681,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   auto settle = [&](Pos p) {
     while (p.g < glast) {
       p.qc = walk.next(p.qc, info);
-      if (p.qc < a.Sq) break;
+      if (p.qc < qend) break;
       p.g += 1;
       p.qc = qfirst;
     }
@@ -789,41 +817,58 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   if (part == nullptr) {
     store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, hh);
     store_row<T, NDB>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, hh);
-  } else {                              // [split][dk, dv][(B, Sk, kv, d)]
+  } else {                              // [piece][dk, dv][(B, Sk, kv, d)]
     const int64_t n = (int64_t)a.B * a.Sk * a.kv * a.d;
-    store_row<float, NDB>(part + 2 * share * n + at, dk, a.scale, a.d, hh);
-    store_row<float, NDB>(part + (2 * share + 1) * n + at, dv, 1.f, a.d, hh);
+    store_row<float, NDB>(part + 2 * piece * n + at, dk, a.scale, a.d, hh);
+    store_row<float, NDB>(part + (2 * piece + 1) * n + at, dv, 1.f, a.d, hh);
   }
 }
 
-// dk and dv = the shares' partials in order; n4 groups of four values each
+// out0 (and out1) = n pieces' partials in order: [piece][out0, out1][4 n4 values]
 template <typename T>
-__global__ __launch_bounds__(256) void k_ba_fold(const float* part, T* dk, T* dv, int64_t n4, int split) {
+__global__ __launch_bounds__(256) void k_ba_fold(const float* part, T* out0, T* out1, int64_t n4, int n) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * n4) return;
+  const int outs = out1 != nullptr ? 2 : 1;
+  if (i >= outs * n4) return;
   const bool second = i >= n4;
   const int64_t e = 4 * (second ? i - n4 : i);
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < split; ++k) s += *reinterpret_cast<const f32x4*>(part + (2 * k + (second ? 1 : 0)) * 4 * n4 + e);
-  store4((second ? dv : dk) + e, s[0], s[1], s[2], s[3]);
-}
-
-// Heads of a group on separate blocks until there are four blocks per CU (1024): below that the chip is not filled, or (causal)
-// the longest walks are waited for.  The partials cost 8 bytes per value and share each way.
-int dkv_split(int64_t B, int64_t Sk, int64_t kv, int64_t group) {
-  const int64_t blocks = B * kv * ((Sk + kRows - 1) / kRows);
-  int64_t split = 1;
-  for (int64_t s = 1; s <= group; ++s)
-    if (group % s == 0) {
-      split = s;
-      if (blocks * s >= 1024) break;
-    }
-  return (int)split;
+  for (int k = 0; k < n; ++k) s += *reinterpret_cast<const f32x4*>(part + (outs * k + (second ? 1 : 0)) * 4 * n4 + e);
+  store4((second ? out1 : out0) + e, s[0], s[1], s[2], s[3]);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 // Few queries take the split form.
 bool few_queries(int64_t Sq) { return Sq <= 16; }
+
+// Parts of a walk that blocks of their own take: until the chip's 1024 SIMDs have two waves each to choose from, and of two
+// chunks at least.  A wave's walk is serial: with one wave per SIMD the longest one is waited for (4 x 8 heads x 1001
+// fp32 causal queries are 1024 waves of 1 .. 16 chunks).
+int parts_of(int64_t waves, int64_t chunks) {
+  int64_t n = (2048 + waves - 1) / waves;
+  if (n > chunks / 2) n = chunks / 2;
+  if (n > 16) n = 16;
+  return (int)(n < 1 ? 1 : n);
+}
+int key_slices(int64_t B, int64_t heads, int64_t Sq, int64_t Sk) {
+  return parts_of(B * heads * ((Sq + 31) / 32), (Sk + kChunk - 1) / kChunk);
+}
+struct Pieces {
+  int split, cuts;
+};
+// dk and dv: heads of a group first, until there are four blocks per CU, then their queries
+Pieces query_pieces(int64_t B, int64_t Sq, int64_t Sk, int64_t kv, int64_t group) {
+  const int64_t blocks = B * kv * ((Sk + kRows - 1) / kRows);
+  Pieces p = {1, 1};
+  for (int64_t s = 1; s <= group; ++s)
+    if (group % s == 0) {
+      p.split = (int)s;
+      if (blocks * s >= 1024) break;
+    }
+  p.cuts = parts_of(B * kv * p.split * ((Sk + 31) / 32), (Sq + kChunk - 1) / kChunk);
+  return p;
+}
+int64_t pad4(int64_t n) { return (n + 3) / 4 * 4; }
 
 int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
 // LDS of the buffers (two with bf16, one with fp32): two tiles and `words` 4-byte values per row of a chunk
@@ -896,7 +941,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
   a.nb = (int)x->num_buckets; a.R = x->table ? (int)x->distance : 0;
   a.scale = x->scale; a.cap = x->softcap;
   a.kpad = (int)pad64(a.Sk); a.qpad = (int)pad64(a.Sq);
-  const int64_t nq = (x->batch * x->heads) * ((a.Sq + kRows - 1) / kRows), nk = (x->batch * x->heads) * ((a.Sk + kRows - 1) / kRows);
+  const int64_t nq = (x->batch * x->heads) * ((a.Sq + kRows - 1) / kRows), nk = (x->batch * x->heads) * ((a.Sk + kRows - 1) / kRows);        // parts only where there are few
   MIVAE_REQUIRE(x->batch <= (1 << 24) && nq < (1ll << 31) - 8 && nk < (1ll << 31) - 8 && x->batch * (a.kpad + a.qpad) / 256 < (1ll << 31),
                 "%s: too many blocks", name);
   if (x->mask || x->documents) {          // [codes][key tiles], and with documents the same of the queries
@@ -924,14 +969,19 @@ int64_t mivae_biased_attention_codes_ints(int64_t batch, int64_t q_len, int64_t 
 
 int64_t mivae_biased_attention_fwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
                                           int64_t head_size) {
-  return few_queries(q_len) ? token_attention_floats(batch, q_len, k_len, heads, kv_heads, head_size) : 0;
+  if (few_queries(q_len)) return token_attention_floats(batch, q_len, k_len, heads, kv_heads, head_size);
+  const int n = key_slices(batch, heads, q_len, k_len);
+  return n > 1 ? batch * heads * q_len * n * (head_size + 4) : 0;
 }
 
+// [delta][table gradient's partials][the parts' delta, dq or dk and dv, one after another in the same place]
 int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
                                           int64_t head_size, int64_t num_buckets) {
-  const int64_t nblk = (q_len + kRows - 1) / kRows, split = dkv_split(batch, k_len, kv_heads, heads / kv_heads);
-  return (batch * heads * q_len + 3) / 4 * 4 + (batch * heads * nblk * num_buckets + 3) / 4 * 4 +
-         (split > 1 ? 2 * split * batch * k_len * kv_heads * head_size : 0);
+  const int64_t nblk = (q_len + kRows - 1) / kRows, n = key_slices(batch, heads, q_len, k_len);
+  const Pieces p = query_pieces(batch, q_len, k_len, kv_heads, heads / kv_heads);
+  const int64_t rows = batch * heads * q_len, dq = n > 1 ? n * pad4(rows * head_size) : 0;
+  const int64_t dkv = p.split * p.cuts > 1 ? 2 * p.split * p.cuts * batch * k_len * kv_heads * head_size : 0;
+  return pad4(rows) + pad4(batch * heads * nblk * n * num_buckets) + (dq > dkv ? dq : dkv);
 }
 
 int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
@@ -953,14 +1003,21 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (few queries)");
     return MIVAE_OK;
   }
+  const int slices = key_slices(a.B, a.heads, a.Sq, a.Sk);
+  MIVAE_REQUIRE(slices == 1 || (x->scratch && aligned16(x->scratch)), "mivae_biased_attention_fwd: the keys are split and need the scratch buffer");
+  float* part = slices > 1 ? x->scratch : nullptr;
   const size_t lds = tile_bytes(x->dtype, a.d, 1) + (a.table ? (2 * a.R + 1) * 4 : 0);
-  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, (a.Sq + kRows - 1) / kRows, a.causal));
+  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads * slices, (a.Sq + kRows - 1) / kRows, a.causal));
   by_shape(x->dtype, a.d, [&](auto t, auto n) {
-    if (a.out_lo) start(k_ba_fwd<unsigned short, n(), kTrainRest>, grid, lds, S_(stream), a);        // bf16 alone has it
-    else if (a.lse) start(k_ba_fwd<decltype(t), n(), kTrain>, grid, lds, S_(stream), a);
-    else start(k_ba_fwd<decltype(t), n(), kInfer>, grid, lds, S_(stream), a);
+    if (a.out_lo) start(k_ba_fwd<unsigned short, n(), kTrainRest>, grid, lds, S_(stream), a, slices, part);     // bf16 alone has it
+    else if (a.lse) start(k_ba_fwd<decltype(t), n(), kTrain>, grid, lds, S_(stream), a, slices, part);
+    else start(k_ba_fwd<decltype(t), n(), kInfer>, grid, lds, S_(stream), a, slices, part);
   });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd");
+  if (part) {
+    token_attention_join(a, part, slices, x->dtype, stream);
+    MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd (join)");
+  }
   return MIVAE_OK;
 }
 
@@ -980,48 +1037,57 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   MIVAE_REQUIRE(aligned16(x->scratch), "mivae_biased_attention_bwd: scratch must be 16-byte aligned");
   const int nblk = (a.Sq + kRows - 1) / kRows;
   a.delta = x->scratch;
-  float* dtab = x->scratch + (rows + 3) / 4 * 4;
+  float* dtab = x->scratch + pad4(rows);
   a.dtab = x->dtable ? dtab : nullptr;
-  float* part = dtab + (x->dtable ? ((int64_t)a.B * a.heads * nblk * a.nb + 3) / 4 * 4 : 0);
+  const int slices = key_slices(a.B, a.heads, a.Sq, a.Sk);
+  float* parts = dtab + (x->dtable ? pad4((int64_t)a.B * a.heads * nblk * slices * a.nb) : 0);
+  float* part = slices > 1 ? parts : nullptr;
   hipStream_t st = S_(stream);
   const size_t tw = a.table ? 2 * a.R + 1 : 0, lds = tile_bytes(x->dtype, a.d, 1) + tw * 4;
-  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads, nblk, a.causal)), dgrid((unsigned)((rows + 15) / 16));
+  const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads * slices, nblk, a.causal)), dgrid((unsigned)((rows + 15) / 16));
+  auto fold = [&](auto* out0, auto* out1, int64_t values, int n) {
+    const int64_t n4 = (values + 3) / 4;
+    hipLaunchKernelGGL((k_ba_fold<std::remove_pointer_t<decltype(out0)>>), dim3((unsigned)(((out1 ? 2 : 1) * n4 + 255) / 256)), dim3(256), 0,
+                       st, parts, out0, out1, n4, n);
+  };
   if (x->dtype == MIVAE_F32)
     hipLaunchKernelGGL((k_ba_delta<float>), dgrid, dim3(256), 0, st, static_cast<const float*>(x->dout),
                        static_cast<const float*>(x->out), nullptr, a.delta, rows, a.Sq, a.heads, a.d);
   else if (!a.dtab)
     hipLaunchKernelGGL((k_ba_delta<unsigned short>), dgrid, dim3(256), 0, st, static_cast<const unsigned short*>(x->dout),
                        static_cast<const unsigned short*>(x->out), a.out_lo, a.delta, rows, a.Sq, a.heads, a.d);
-  else
-    by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a); });
+  else {
+    by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a, slices, part); });
+    if (part) fold(a.delta, (float*)nullptr, rows, slices);
+  }
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (delta)");
   if (a.dq || a.dtab) {
     const size_t more = a.dtab ? kWaves * (tw + 32 * 64) * 4 : 0;
-    by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_dq<decltype(t), n(), false>, grid, lds + more, st, a); });
+    by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_dq<decltype(t), n(), false>, grid, lds + more, st, a, slices, part); });
+    if (part && a.dq) {
+      if (x->dtype == MIVAE_F32) fold(static_cast<float*>(a.dq), (float*)nullptr, rows * a.d, slices);
+      else fold(static_cast<unsigned short*>(a.dq), (unsigned short*)nullptr, rows * a.d, slices);
+    }
     MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dq)");
     if (a.dtab) {
-      hipLaunchKernelGGL(k_ba_dtable, dim3((unsigned)(a.heads * a.nb)), dim3(64), 0, st, a.dtab, x->dtable, (int64_t)a.B * nblk,
-                         a.nb, a.heads);
+      hipLaunchKernelGGL(k_ba_dtable, dim3((unsigned)(a.heads * a.nb)), dim3(64), 0, st, a.dtab, x->dtable,
+                         (int64_t)a.B * nblk * slices, a.nb, a.heads);
       MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dtable)");
     }
   }
   if (a.dk) {
-    const int split = dkv_split(a.B, a.Sk, a.kv, a.group);
-    const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * split, (a.Sk + kRows - 1) / kRows, a.causal));
-    float* shares = split > 1 ? part : nullptr;
-    by_shape(x->dtype, a.d,
-             [&](auto t, auto n) { start(k_ba_dkv<decltype(t), n()>, kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, split, shares); });
-    MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dk, dv)");
-    if (shares) {
-      const int64_t n4 = (int64_t)a.B * a.Sk * a.kv * a.d / 4;
-      const dim3 fgrid((unsigned)((2 * n4 + 255) / 256));
-      if (x->dtype == MIVAE_F32)
-        hipLaunchKernelGGL((k_ba_fold<float>), fgrid, dim3(256), 0, st, shares, static_cast<float*>(a.dk), static_cast<float*>(a.dv), n4, split);
-      else
-        hipLaunchKernelGGL((k_ba_fold<unsigned short>), fgrid, dim3(256), 0, st, shares, static_cast<unsigned short*>(a.dk),
-                           static_cast<unsigned short*>(a.dv), n4, split);
-      MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (fold)");
+    const Pieces p = query_pieces(a.B, a.Sq, a.Sk, a.kv, a.group);
+    const int pieces = p.split * p.cuts;
+    const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * pieces, (a.Sk + kRows - 1) / kRows, a.causal));
+    by_shape(x->dtype, a.d, [&](auto t, auto n) {
+      start(k_ba_dkv<decltype(t), n()>, kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, p.split, p.cuts, pieces > 1 ? parts : nullptr);
+    });
+    if (pieces > 1) {
+      const int64_t values = (int64_t)a.B * a.Sk * a.kv * a.d;
+      if (x->dtype == MIVAE_F32) fold(static_cast<float*>(a.dk), static_cast<float*>(a.dv), values, pieces);
+      else fold(static_cast<unsigned short*>(a.dk), static_cast<unsigned short*>(a.dv), values, pieces);
     }
+    MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (dk, dv)");
   }
   return MIVAE_OK;
 }

@@ -344,6 +344,12 @@ void start(const TokenArgs& t, unsigned grid, hipStream_t st) {
   hipLaunchKernelGGL((k_token<T, NDB>), dim3(grid), dim3(64 * kWaves), lds, st, t);
 }
 
+void join(const TokenArgs& t, int dtype, hipStream_t st) {
+  const dim3 rows((unsigned)((int64_t)t.a.B * t.a.kv * t.rows));
+  if (dtype == MIVAE_F32) hipLaunchKernelGGL((k_token_join<float>), rows, dim3(64), 0, st, t);
+  else hipLaunchKernelGGL((k_token_join<unsigned short>), rows, dim3(64), 0, st, t);
+}
+
 // Splits: 1024 blocks, two turns of two blocks per CU, each of at least one turn of its waves (64 keys).  More pay for more
 // starts and partials (2048: 178 us at the size above), fewer wait for the longest row (512: 165 us there, 56 % to 100 % full).
 int splits_of(int64_t blocks, int64_t Sk) {
@@ -385,11 +391,18 @@ void token_attention(const BiasedArgs& a, float* scratch, int dtype, void* strea
     else if (ndb == 3) start<unsigned short, 3>(t, grid, st);
     else start<unsigned short, 4>(t, grid, st);
   }
-  if (t.part) {
-    const dim3 rows((unsigned)((int64_t)a.B * a.kv * t.rows));
-    if (dtype == MIVAE_F32) hipLaunchKernelGGL((k_token_join<float>), rows, dim3(64), 0, st, t);
-    else hipLaunchKernelGGL((k_token_join<unsigned short>), rows, dim3(64), 0, st, t);
-  }
+  if (t.part) join(t, dtype, st);
+}
+
+void token_attention_join(const BiasedArgs& a, float* part, int splits, int dtype, void* stream) {
+  TokenArgs t = {};
+  t.a = a;
+  t.a.kv = a.heads;
+  t.a.group = 1;
+  t.part = part;
+  t.rows = a.Sq;
+  t.splits = splits;
+  join(t, dtype, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // namespace mivae

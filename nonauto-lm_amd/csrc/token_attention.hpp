@@ -11,4 +11,7 @@ int64_t token_attention_floats(int64_t B, int64_t Sq, int64_t Sk, int64_t heads,
 // launches; the caller has checked the arguments and looks at the launch status
 void token_attention(const BiasedArgs& a, float* scratch, int dtype, void* stream);
 
+// out (and lse, out_lo) from `splits` partials per row of (b, head, row): [row][split][d + 4] of O, max, sum
+void token_attention_join(const BiasedArgs& a, float* part, int splits, int dtype, void* stream);
+
 }  // namespace mivae
