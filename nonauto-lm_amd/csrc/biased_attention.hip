@@ -640,21 +640,32 @@ __global__ __launch_bounds__(64) void k_ba_dtable(const float* part, float* dtab
 // ---- backward: dk and dv ---------------------------------------------------------------------------------------------
 // A block's walk over the queries of all heads of a group.  Where there are few blocks, `split` blocks share a group's heads and
 // each share's queries are cut into `cuts` equal parts; they leave fp32 partials that k_ba_fold sums in order.
+//
+// Roles (bf16, d > 64): dk and dv of 32 keys, their operands and the scores do not fit the 256 registers of two waves per SIMD.
+// Eight waves a block then, wave w forming dv and wave w + 4 dk of the same keys: 5 products and two exponentials instead of 4
+// and one, but two waves to fill each other's waits (64 x 512 tokens, 4 heads of 128: ROLES_US instead of 212 us; one kernel
+// squeezed into 256 registers spills 304 bytes a lane, 238 us).
 template <typename T, int NDB>
-__global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, int cuts, float* part) {
+constexpr bool by_roles() { return sizeof(T) == 2 && NDB >= 3; }
+
+template <typename T, int NDB>
+__global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(T) == 4 ? 1 : 2) void k_ba_dkv(BiasedArgs a, int split, int cuts, float* part) {
   using L = Tile<T, NDB>;
   constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
+  constexpr bool ROLES = by_roles<T, NDB>();
+  constexpr int NT = 64 * kWaves * (ROLES ? 2 : 1);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][Q, dO]
   float* lses = reinterpret_cast<float*>(tiles + 2 * NBUF * TILE);        // [NBUF][kChunk] each
   float* dels = lses + NBUF * kChunk;
   int* qc_lds = reinterpret_cast<int*>(dels + NBUF * kChunk);
   float* tab = reinterpret_cast<float*>(qc_lds + NBUF * kChunk);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
   const Ids id = ids_of(a.B, a.kv * split * cuts, (a.Sk + kRows - 1) / kRows, a.causal != 0, false);
   if (id.none) return;
   const int64_t b = id.b;
-  const int kvh = id.head / (split * cuts), piece = id.head % (split * cuts), share = piece / cuts, row0 = id.blk * kRows, k0 = row0 + 32 * wave, key = k0 + r32;
+  const int kvh = id.head / (split * cuts), piece = id.head % (split * cuts), share = piece / cuts, row0 = id.blk * kRows, k0 = row0 + 32 * (wave % kWaves), key = k0 + r32;
+  const bool does_v = !ROLES || wave < kWaves, does_k = !ROLES || wave >= kWaves;
   const View v = view_of(a, b);
   const bool ok = key < a.Sk;
   const int kcode = !ok ? -1 : v.codes ? a.kcodes[b * a.kpad + key] : 0;
@@ -689,21 +700,27 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
   };
   typename Frag<T>::type kf[2 * NDB], vf[2 * NDB];
   load_row<T, NDB>(kf, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + kvh * a.ks[2], kcode >= 0, a.d, hh);
-  load_row<T, NDB>(vf, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + kvh * a.vs[2], kcode >= 0, a.d, hh);
-  f32x16 dk[NDB], dv[NDB];
+  load_row<T, NDB>(vf, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + kvh * a.vs[2], does_k && kcode >= 0, a.d, hh);
+  constexpr int NV = ROLES ? 1 : NDB;
+  f32x16 dk[NDB], dv[NV];                // with roles, dk holds what the wave forms
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { dk[db][r] = 0.f; dv[db][r] = 0.f; }
+    for (int r = 0; r < 16; ++r) {
+      dk[db][r] = 0.f;
+      dv[db % NV][r] = 0.f;
+    }
   Stage<T, NDB, kWaves> sq, sd;
   float pl = 0.f, pd = 0.f;
   int pq = 0, buf = 0;
   auto issue = [&](int n, Pos p) {
     const int head = kvh * a.group + p.g;
     const uint64_t rows = low_rows(a.Sq - p.qc);       
-    sq.issue(tiles + 2 * n * TILE, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, rows, a.d);
-    sd.issue(tiles + (2 * n + 1) * TILE, static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d,
-             (int64_t)a.heads * a.d, p.qc, rows, a.d);
+    if (!ROLES || wave < kWaves) {
+      sq.issue(tiles + 2 * n * TILE, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, rows, a.d);
+      sd.issue(tiles + (2 * n + 1) * TILE, static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d,
+               (int64_t)a.heads * a.d, p.qc, rows, a.d);
+    }
     const int i = p.qc + (int)threadIdx.x;
     const bool in = threadIdx.x < kChunk && i < a.Sq;
     pl = in ? a.lse[(b * a.heads + head) * a.Sq + i] : INFINITY;    // rows beyond Sq: p = exp2(. - inf) = 0
@@ -729,7 +746,7 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
     if (other_head) {
       sp = score_of(a, head);
       tab_head = head;
-      if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
+      if (sp.tab) stage_table(tab, a, head, NT);
     }
     __syncthreads();
     const i32x4 seen = info;
@@ -757,8 +774,11 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
 #pragma unroll
       for (int s = 0; s < 2 * NDB; ++s) {
         u = mma(L::row(qt, 32 * t + r32, s, hh), kf[s], u);
-        dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
+        if (!ROLES) dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
       }
+      if (ROLES && does_k)
+#pragma unroll
+        for (int s = 0; s < 2 * NDB; ++s) dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
       f32x16 g;
       if (sp.cap) {
         cap_tile<false>(u, sp);
@@ -786,41 +806,54 @@ __global__ __launch_bounds__(64 * kWaves, NDB >= 3 || sizeof(T) == 4 ? 1 : 2) vo
 #pragma unroll
       for (int a4 = 0; a4 < 4; ++a4) {
         const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * t + 8 * a4 + 4 * hh);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(de + 32 * t + 8 * a4 + 4 * hh);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * a4 + i;
-          u[r] = __builtin_amdgcn_exp2f(fmaf(A, u[r], C - l4[i]));
-          dp[r] = u[r] * (dp[r] - d4[i]);
+        for (int i = 0; i < 4; ++i) u[4 * a4 + i] = __builtin_amdgcn_exp2f(fmaf(A, u[4 * a4 + i], C - l4[i]));
+      }
+      typename Frag<T>::type x0, x1;
+      if (does_v) {
+        pack8(x0, u, 0);
+        pack8(x1, u, 1);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          f32x16& acc = ROLES ? dk[db] : dv[db % NV];
+          acc = mma(L::col(dt, 32 * t, db, lane), x0, acc);
+          acc = mma(L::col(dt, 32 * t + 16, db, lane), x1, acc);
         }
       }
-      if (sp.cap) {
+      if (does_k) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] *= g[r];
-      }
-      typename Frag<T>::type p0, p1, d0, d1;
-      pack8(p0, u, 0);
-      pack8(p1, u, 1);
-      pack8(d0, dp, 0);
-      pack8(d1, dp, 1);
+        for (int a4 = 0; a4 < 4; ++a4) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(de + 32 * t + 8 * a4 + 4 * hh);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        dv[db] = mma(L::col(dt, 32 * t, db, lane), p0, dv[db]);
-        dv[db] = mma(L::col(dt, 32 * t + 16, db, lane), p1, dv[db]);
-        dk[db] = mma(L::col(qt, 32 * t, db, lane), d0, dk[db]);
-        dk[db] = mma(L::col(qt, 32 * t + 16, db, lane), d1, dk[db]);
+          for (int i = 0; i < 4; ++i) dp[4 * a4 + i] = u[4 * a4 + i] * (dp[4 * a4 + i] - d4[i]);
+        }
+        if (sp.cap) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= g[r];
+        }
+        pack8(x0, dp, 0);
+        pack8(x1, dp, 1);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          dk[db] = mma(L::col(qt, 32 * t, db, lane), x0, dk[db]);
+          dk[db] = mma(L::col(qt, 32 * t + 16, db, lane), x1, dk[db]);
+        }
       }
     }
   }
   if (!ok) return;
   const int64_t at = ((b * a.Sk + key) * a.kv + kvh) * a.d;
-  if (part == nullptr) {
-    store_row<T, NDB>(static_cast<T*>(a.dk) + at, dk, a.scale, a.d, hh);
-    store_row<T, NDB>(static_cast<T*>(a.dv) + at, dv, 1.f, a.d, hh);
-  } else {                              // [piece][dk, dv][(B, Sk, kv, d)]
-    const int64_t n = (int64_t)a.B * a.Sk * a.kv * a.d;
-    store_row<float, NDB>(part + 2 * piece * n + at, dk, a.scale, a.d, hh);
-    store_row<float, NDB>(part + (2 * piece + 1) * n + at, dv, 1.f, a.d, hh);
+  const int64_t n = (int64_t)a.B * a.Sk * a.kv * a.d;                     // with parts: [piece][dk, dv][(B, Sk, kv, d)]
+  auto put = [&](const auto& x, void* out, int64_t which, float mul) {
+    if (part == nullptr) store_row<T, NDB>(static_cast<T*>(out) + at, x, mul, a.d, hh);
+    else store_row<float, NDB>(part + which * n + at, x, mul, a.d, hh);
+  };
+  if constexpr (ROLES) {
+    if (does_v) put(dk, a.dv, 2 * piece + 1, 1.f);
+    else put(dk, a.dk, 2 * piece, a.scale);
+  } else {
+    put(dk, a.dk, 2 * piece, a.scale);
+    put(dv, a.dv, 2 * piece + 1, 1.f);
   }
 }
 
@@ -882,6 +915,11 @@ template <typename... A>
 void start(void (*fn)(A...), dim3 grid, size_t lds, hipStream_t st, A... args) {
   if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   hipLaunchKernelGGL(fn, grid, dim3(64 * kWaves), lds, st, args...);
+}
+template <typename T, int NDB>
+void start_dkv(dim3 grid, size_t lds, hipStream_t st, const BiasedArgs& a, const Pieces& p, float* part) {
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)k_ba_dkv<T, NDB>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL((k_ba_dkv<T, NDB>), grid, dim3(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1)), lds, st, a, p.split, p.cuts, part);
 }
 
 // f(type tag, std::integral_constant NDB)
@@ -1080,7 +1118,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     const int pieces = p.split * p.cuts;
     const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * pieces, (a.Sk + kRows - 1) / kRows, a.causal));
     by_shape(x->dtype, a.d, [&](auto t, auto n) {
-      start(k_ba_dkv<decltype(t), n()>, kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, p.split, p.cuts, pieces > 1 ? parts : nullptr);
+      start_dkv<decltype(t), n()>(kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, p, pieces > 1 ? parts : nullptr);
     });
     if (pieces > 1) {
       const int64_t values = (int64_t)a.B * a.Sk * a.kv * a.d;
