@@ -371,8 +371,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     }
     // P is rounded to bf16 for its product, an error of 2^-9 that o passes on to delta, where it counts as soon as few keys
-    // carry a row.  Chunks with a p of more than about 1/16 of its row also multiply what the rounding leaves.
-    const bool rest = MODE == kTrainRest && __builtin_amdgcn_ballot_w64(8.f * __builtin_amdgcn_exp2f(top - m) > l) != 0;
+    // carry a row.  Chunks with a p of more than about 1/8 of its row so far (l is half a row's) also multiply what the
+    // rounding leaves; eight p of 1/8 without it add a sixteenth to the two roundings' error of dq and dk.
+    const bool rest = MODE == kTrainRest && __builtin_amdgcn_ballot_w64(4.f * __builtin_amdgcn_exp2f(top - m) > l) != 0;
     const float cm = C - m;
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -433,19 +434,41 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
 }
 
 // ---- backward: dq and the table's gradient ---------------------------------------------------------------------------
-// The table's gradient sums ds along the diagonals of the tiles.  A wave writes its tile into LDS skewed, query q's value at
-// distance x into column x + 31 of row q (64 columns; the corners keep their zeros), lane c sums column c and adds it to the
-// wave's array by relative distance: every sum has one order, from run to run.  (LDS float atomics, 16 per tile, took
-// 190 cycles each: 686 us instead of the SKEW_US at 4 x 16 x 4096^2.)  Tiles at or beyond distance R go to two
-// registers instead.  The block then folds its four arrays by bucket into one partial row.
+// The table's gradient sums ds along the diagonals of the tiles (diagonal_sums), a lane's diagonal at a time into the wave's
+// array by relative distance: every sum has one order, from run to run.  Tiles at or beyond distance R go to two registers
+// instead.  The block then folds its four arrays by bucket into one partial row.  (LDS float atomics, 16 per tile, took 190
+// cycles each: 686 us instead of 370 at 4 x 16 x 4096^2 causal; skewing the tile in LDS costs 8 KiB a wave, which at d = 128
+// leaves one block per CU: 163 us instead of 112 at 64 x 512 tokens, 4 heads.)
 //
 // slices > 1: as in the forward; dq (or delta) then goes to `part` [slice][..] in fp32 and k_ba_fold sums the slices in order.
 //
-// DELTA: the first half of the same walk, delta_i = sum_j p_ij (do_i . v_j), instead of dout . out.  Needed by the table's
+// kTable: with the table's gradient.  kDelta: the first half of the same walk, delta_i = sum_j p_ij (do_i . v_j), instead of dout . out.  Needed by the table's
 // gradient on bf16 operands: the o of the forward carries what is left of the rounding of P, which averages out in dq and dk
 // but enters the few values of an fp32 dtable in full (4e-4 of their norm with a once rounded P).
-template <typename T, int NDB, bool DELTA>
+// Sums of a tile's diagonals: lane c returns the sum over key - query = c - 31 (c = 63: 0).  Lane (hh, q), register r holds the value
+// of query q and key 4 hh + acc_row(r).  For one register, sending lane (hh, q) to lane 31 - q + acc_row(r) + 32 hh (mod 64) is
+// a permutation of the wave: half 0 lands on its columns acc_row(r) .. acc_row(r) + 31, half 1 everywhere else, 28 to the right
+// (mod 64) of its own.  Two running sums take the two, and one more permutation brings the second home.
+__device__ __forceinline__ float diagonal_sums(const f32x16& u, int lane) {
+  asm volatile("" : "+v"(lane));        // the 16 lane masks are formed here: kept over the walk they push scalars out of registers
+  const int base = 4 * (31 - (lane & 31) + (lane & 32));
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int to = (base + 4 * acc_row(r)) & 255;
+    const float x = __int_as_float(__builtin_amdgcn_ds_permute(to, __float_as_int(u[r])));
+    const bool first = (unsigned)(lane - acc_row(r)) < 32u;
+    s0 += first ? x : 0.f;
+    s1 += first ? 0.f : x;
+  }
+  return s0 + __int_as_float(__builtin_amdgcn_ds_permute(4 * ((lane + 36) & 63), __float_as_int(s1)));
+}
+
+enum DqKind { kPlain, kTable, kDelta };
+
+template <typename T, int NDB, DqKind KIND>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(BiasedArgs a, int slices, float* part) {
+  constexpr bool DELTA = KIND == kDelta, grad_tab = KIND == kTable;
   using L = Tile<T, NDB>;
   constexpr int TILE = kChunk * L::PITCH, NBUF = Stage<T, NDB, kWaves>::NBUF;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -466,13 +489,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   const int TW = 2 * a.R + 1;
   float* hist = tab + TW;                                                 // [kWaves][TW]
   float* mine = hist + wave * TW;
-  float* skew = hist + kWaves * TW + wave * 32 * 64;                      // [kWaves][32][64]
-  const bool grad_tab = !DELTA && a.dtab != nullptr;
   if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
-  if (grad_tab) {
+  if (grad_tab)
     for (int i = threadIdx.x; i < kWaves * TW; i += 64 * kWaves) hist[i] = 0.f;
-    for (int i = lane; i < 32 * 64; i += 64) skew[i] = 0.f;
-  }
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
@@ -559,13 +578,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
           if (rel0 < 0) far_lo += s;
           else far_hi += s;
         } else {
-          float* w = skew + r32 * 63 + 4 * hh + 31;                       // row r32, column key - query + 31
-#pragma unroll
-          for (int r = 0; r < 16; ++r) w[acc_row(r)] = u[r];
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int q = 0; q < 32; ++q) s[q & 3] += skew[q * 64 + lane];
-          const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+          const float sum = diagonal_sums(u, lane);
           const int x = rel0 - 31 + lane;
           if (x <= -a.R) far_lo += sum;
           else if (x >= a.R) far_hi += sum;
@@ -643,8 +656,8 @@ __global__ __launch_bounds__(64) void k_ba_dtable(const float* part, float* dtab
 //
 // Roles (bf16, d > 64): dk and dv of 32 keys, their operands and the scores do not fit the 256 registers of two waves per SIMD.
 // Eight waves a block then, wave w forming dv and wave w + 4 dk of the same keys: 5 products and two exponentials instead of 4
-// and one, but two waves to fill each other's waits (64 x 512 tokens, 4 heads of 128: ROLES_US instead of 212 us; one kernel
-// squeezed into 256 registers spills 304 bytes a lane, 238 us).
+// and one, but two waves to fill each other's waits (64 x 512 tokens, 4 heads of 128: 200 us instead of 214; one kernel squeezed
+// into 256 registers spills 304 bytes a lane, 238 us).
 template <typename T, int NDB>
 constexpr bool by_roles() { return sizeof(T) == 2 && NDB >= 3; }
 
@@ -1095,13 +1108,16 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     hipLaunchKernelGGL((k_ba_delta<unsigned short>), dgrid, dim3(256), 0, st, static_cast<const unsigned short*>(x->dout),
                        static_cast<const unsigned short*>(x->out), a.out_lo, a.delta, rows, a.Sq, a.heads, a.d);
   else {
-    by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), true>, grid, lds, st, a, slices, part); });
+    by_shape(MIVAE_BF16, a.d, [&](auto, auto n) { start(k_ba_dq<unsigned short, n(), kDelta>, grid, lds, st, a, slices, part); });
     if (part) fold(a.delta, (float*)nullptr, rows, slices);
   }
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_bwd (delta)");
   if (a.dq || a.dtab) {
-    const size_t more = a.dtab ? kWaves * (tw + 32 * 64) * 4 : 0;
-    by_shape(x->dtype, a.d, [&](auto t, auto n) { start(k_ba_dq<decltype(t), n(), false>, grid, lds + more, st, a, slices, part); });
+    const size_t more = a.dtab ? kWaves * tw * 4 : 0;
+    by_shape(x->dtype, a.d, [&](auto t, auto n) {
+      if (a.dtab) start(k_ba_dq<decltype(t), n(), kTable>, grid, lds + more, st, a, slices, part);
+      else start(k_ba_dq<decltype(t), n(), kPlain>, grid, lds, st, a, slices, part);
+    });
     if (part && a.dq) {
       if (x->dtype == MIVAE_F32) fold(static_cast<float*>(a.dq), (float*)nullptr, rows * a.d, slices);
       else fold(static_cast<unsigned short*>(a.dq), (unsigned short*)nullptr, rows * a.d, slices);
