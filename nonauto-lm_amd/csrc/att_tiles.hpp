@@ -33,6 +33,7 @@ struct BiasedArgs {
   // hidden.  Queries: document id, kNoCode where it is negative.  tiles: {lowest, highest visible code, visible rows} per 64
   const int *kcodes, *qcodes;
   const i32x4 *ktiles, *qtiles;
+  const i32x4* sighted;         // backward: the queries' summaries with only the rows that see a key, or null: all do
   const int *prefix, *q_starts;
   const float* slopes;          // (heads), or null
   const float* table;           // (nb, heads), or null

@@ -71,6 +71,23 @@ __global__ __launch_bounds__(256) void k_ba_codes(const int64_t* mask, const int
   }
 }
 
+// Backward: the summaries of the queries anew, with only the rows that see a key, i.e. whose log-sum-exp is finite for some
+// head.  dk and dv stage no others: whatever a blind row and its gradient hold must not meet a product, 0 * NaN is NaN.
+__global__ __launch_bounds__(256) void k_ba_sighted(const float* lse, const int* qcodes, int B, int Sq, int qpad, int heads, i32x4* tiles) {
+  const int n = qpad / 64, lane = threadIdx.x & 63;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)B * n) return;
+  const int64_t b = w / n;
+  const int i = (int)(w % n) * 64 + lane;
+  bool sees = false;
+  if (i < Sq)
+    for (int h = 0; h < heads; ++h) sees |= !(lse[(b * heads + h) * Sq + i] == INFINITY);
+  int lo, hi;
+  wave_range(!sees ? -1 : qcodes ? qcodes[b * qpad + i] : 0, lo, hi);
+  const uint64_t rows = __builtin_amdgcn_ballot_w64(sees);
+  if (lane == 0) tiles[w] = i32x4{lo, hi, (int)(unsigned)rows, (int)(unsigned)(rows >> 32)};
+}
+
 // ---- delta = sum_d dout * out: 16 lanes per (b, i, head) row -----------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, const unsigned short* lo, float* delta, int64_t rows, int Sq, int heads, int d) {
@@ -500,7 +517,14 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   typename Frag<T>::type qf[2 * NDB], dof[2 * NDB];
   load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)qw.row * a.qs[1] + head * a.qs[2], live, a.d, hh);
   load_row<T, NDB>(dof, static_cast<const T*>(a.dout) + at_q, live, a.d, hh);
-  const float lse = live ? a.lse[at_l] : INFINITY, delta = !DELTA && live ? a.delta[at_l] : 0.f;
+  const float lse = live ? a.lse[at_l] : INFINITY;
+  const bool sighted = lse != INFINITY; // a row that sees no key passes no gradient, whatever it and its gradient hold
+  const float delta = !DELTA && sighted ? a.delta[at_l] : 0.f;
+#pragma unroll
+  for (int s = 0; s < 2 * NDB; ++s) {
+    qf[s] = sighted ? qf[s] : typename Frag<T>::type{};
+    dof[s] = sighted ? dof[s] : typename Frag<T>::type{};
+  }
   float dsum = 0.f;
   f32x16 dq[NDB];
 #pragma unroll
@@ -697,7 +721,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
   int blo = 0, bhi = 0;
   if (v.codes) block_range(a.ktiles + b * (a.kpad / 64), row0, a.Sk, blo, bhi);
   Walk walk;
-  walk.init(v.docs ? a.qtiles + b * (a.qpad / 64) : nullptr, a.Sq, qend, blo, bhi);
+  walk.init(a.sighted ? a.sighted + b * (a.qpad / 64) : nullptr, a.Sq, qend, blo, bhi);
   // next chunk of queries of the group's heads that the block's keys may be seen from
   const int glast = bhi < 0 ? 0 : (share + 1) * a.group / split;          // (every key of the block hidden: none)
   struct Pos { int g, qc; };
@@ -728,7 +752,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
   int pq = 0, buf = 0;
   auto issue = [&](int n, Pos p) {
     const int head = kvh * a.group + p.g;
-    const uint64_t rows = low_rows(a.Sq - p.qc);       
+    const uint64_t rows = rows_of(info);          // (rows that see no key arrive as zeros)
     if (!ROLES || wave < kWaves) {
       sq.issue(tiles + 2 * n * TILE, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], p.qc, rows, a.d);
       sd.issue(tiles + (2 * n + 1) * TILE, static_cast<const T*>(a.dout) + (b * a.Sq * a.heads + head) * a.d,
@@ -753,7 +777,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
     sd.land(tiles + (2 * buf + 1) * TILE);
     if (threadIdx.x < kChunk) {
       lses[buf * kChunk + threadIdx.x] = pl;
-      dels[buf * kChunk + threadIdx.x] = pd;
+      dels[buf * kChunk + threadIdx.x] = pl == INFINITY ? 0.f : pd;       // such a row's dout may hold anything
       qc_lds[buf * kChunk + threadIdx.x] = pq;
     }
     if (other_head) {
@@ -973,6 +997,7 @@ int set_args(BiasedArgs& a, const mivae_attention_args* x, const char* name) {
   MIVAE_REQUIRE(!(x->prefix && !x->causal), "%s: a prefix needs the causal mask", name);
   MIVAE_REQUIRE(x->softcap >= 0.f && x->softcap < 1e30f && x->scale >= 0.f && x->scale < 1e30f,
                 "%s: softcap or scale out of range", name);
+  MIVAE_REQUIRE(x->softcap == 0.f || x->scale / x->softcap < 1e30f, "%s: softcap %g is too small for the scale", name, (double)x->softcap);
   MIVAE_REQUIRE(!(x->slopes && x->table), "%s: slopes and a table are alternatives", name);
   if (x->table)
     MIVAE_REQUIRE(x->buckets && x->num_buckets >= 1 && x->num_buckets <= kMaxBuckets && x->distance >= 1 && x->distance <= kMaxDistance,
@@ -1025,14 +1050,14 @@ int64_t mivae_biased_attention_fwd_floats(int64_t batch, int64_t q_len, int64_t 
   return n > 1 ? batch * heads * q_len * n * (head_size + 4) : 0;
 }
 
-// [delta][table gradient's partials][the parts' delta, dq or dk and dv, one after another in the same place]
+// [delta][the queries' summaries][table gradient's partials][the parts' delta, dq or dk and dv, one after another in the same place]
 int64_t mivae_biased_attention_bwd_floats(int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t kv_heads,
                                           int64_t head_size, int64_t num_buckets) {
   const int64_t nblk = (q_len + kRows - 1) / kRows, n = key_slices(batch, heads, q_len, k_len);
   const Pieces p = query_pieces(batch, q_len, k_len, kv_heads, heads / kv_heads);
   const int64_t rows = batch * heads * q_len, dq = n > 1 ? n * pad4(rows * head_size) : 0;
   const int64_t dkv = p.split * p.cuts > 1 ? 2 * p.split * p.cuts * batch * k_len * kv_heads * head_size : 0;
-  return pad4(rows) + pad4(batch * heads * nblk * n * num_buckets) + (dq > dkv ? dq : dkv);
+  return pad4(rows) + batch * pad64(q_len) / 16 + pad4(batch * heads * nblk * n * num_buckets) + (dq > dkv ? dq : dkv);
 }
 
 int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
@@ -1088,7 +1113,8 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
   MIVAE_REQUIRE(aligned16(x->scratch), "mivae_biased_attention_bwd: scratch must be 16-byte aligned");
   const int nblk = (a.Sq + kRows - 1) / kRows;
   a.delta = x->scratch;
-  float* dtab = x->scratch + pad4(rows);
+  i32x4* sighted = reinterpret_cast<i32x4*>(x->scratch + pad4(rows));
+  float* dtab = x->scratch + pad4(rows) + (int64_t)a.B * a.qpad / 16;
   a.dtab = x->dtable ? dtab : nullptr;
   const int slices = key_slices(a.B, a.heads, a.Sq, a.Sk);
   float* parts = dtab + (x->dtable ? pad4((int64_t)a.B * a.heads * nblk * slices * a.nb) : 0);
@@ -1130,6 +1156,11 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     }
   }
   if (a.dk) {
+    if (a.kcodes || a.q_starts) {         // otherwise every query sees a key
+      const int64_t waves = (int64_t)a.B * a.qpad / 64;
+      hipLaunchKernelGGL(k_ba_sighted, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a.lse, a.qcodes, a.B, a.Sq, a.qpad, a.heads, sighted);
+      a.sighted = sighted;
+    }
     const Pieces p = query_pieces(a.B, a.Sq, a.Sk, a.kv, a.group);
     const int pieces = p.split * p.cuts;
     const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * pieces, (a.Sk + kRows - 1) / kRows, a.causal));

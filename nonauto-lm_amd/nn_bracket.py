@@ -522,11 +522,16 @@ class MultiHeadAttention(torch.nn.Module):
     def _scored_constants(self, device):
         made = self._constants.get(device)
         if made is None:
-            freqs = ops.rotary_frequencies(self._rotary, self._rotary_base, device) if self._rotary else None
-            h = torch.arange(1, self._num_heads + 1, dtype=torch.float32, device=device)
-            made = (freqs, 2.0 ** (-8.0 * h / self._num_heads) if self._slopes else None)
-            if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():     # else: values of that graph alone
-                self._constants[device] = made
+            # Kept ones are made on the host and copied synchronously, so that every stream finds them ready, and as ordinary
+            # tensors, so that a call in inference mode may be the first.  While a graph is captured: values of that graph alone.
+            graph = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+            with torch.inference_mode(False):
+                at = device if graph else None
+                freqs = ops.rotary_frequencies(self._rotary, self._rotary_base, at) if self._rotary else None
+                h = torch.arange(1, self._num_heads + 1, dtype=torch.float32, device=at)
+                made = (freqs, 2.0 ** (-8.0 * h / self._num_heads) if self._slopes else None)
+                if not graph:
+                    made = self._constants[device] = tuple(None if t is None else t.to(device) for t in made)
         return made
 
     def _scored_attention(self, q, k, v, mask, documents, prefix):

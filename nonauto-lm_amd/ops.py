@@ -538,9 +538,10 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     seen     key <= query with `causal`, or key < prefix[b] (int32 (B,), needs causal); mask (B, Sk) != 0; documents
              (int32 (B, Sk)) equal and not negative, the query's taken at its position.
 
-    A query that sees no key gives zeros and has no gradient (`ops.attention` averages such a row instead).  Keys that the
-    mask or a negative document hides may hold anything; all others have to be finite, also where `causal` or documents
-    hide them from some queries."""
+    A query that sees no key gives zeros and passes no gradient (`ops.attention` averages such a row instead).  Keys that the
+    mask or a negative document hides may hold anything, and so may queries that see no key and their gradients; all
+    other operands have to be finite, also where `causal` or documents hide them from some queries.  A table entry of -inf
+    or of fp32's or bf16's lowest value hides its pairs."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
     _operand_dtype("biased_attention", q, k, v)
@@ -564,6 +565,8 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not 0 <= scale < 1e30:
         raise ValueError(f"biased_attention: scale {scale}")
+    if softcap is not None and not scale / softcap < 1e30:
+        raise ValueError(f"biased_attention: softcap {softcap} is too small for scale {scale}")
     args = L.AttentionArgs(batch=B, q_len=Sq, k_len=Sk, heads=heads, kv_heads=kv_heads, head_size=d, q_stride=qst,
                            k_stride=kst, v_stride=vst, scale=scale, softcap=softcap or 0.0, causal=int(bool(causal)),
                            dtype=L.dtype_code(q.dtype))

@@ -139,6 +139,37 @@ def test_layer_under_autocast():
         compare(make(options), x, None, mask, 5e-2, bf16=True)
 
 
+@gpu
+def test_layer_first_called_in_inference_mode_or_a_capture():
+    """the layer's constants outlive the mode, stream and graph of the call that made them"""
+    x = torch.randn(2, 30, 64, device="cuda")
+    want = None
+    for first in ("inference", "side stream", "capture"):
+        torch.manual_seed(1)
+        mha = make(dict(rotary=True, distance_slopes=True))
+        if first == "inference":
+            with torch.inference_mode():
+                mha(x, x, x)
+        elif first == "side stream":
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                mha(x, x, x)
+        else:
+            with torch.no_grad():
+                mha(x, x, x)
+                mha._constants.clear()
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    mha(x, x, x)
+            assert not mha._constants
+        out = mha(x, x, x)
+        want = out if want is None else want
+        assert torch.equal(out, want)
+        out.sum().backward()
+
+
 def test_layer_refusals_and_state_dict():
     from nonauto_lm_amd import nn_bracket as nb
     plain = nb.MultiHeadAttention(4, 64)

@@ -10,7 +10,7 @@ step, relative) and e = 2^-24 for fp32:
   dv       as out;   dtable: the fp32 part alone, delta being summed in fp32
 
 h counts d + 8 steps of the score's absolute products, 8 of its value (scaling, cap, bias, exponent) and, for the cap of bf16
-operands, 4 steps of the cap itself (tanh as 1 - 2 / (1 + e^2x))."""
+operands, 4 steps of the cap itself (as 1 - 2 / (1 + e^2x), or a polynomial of that error where the score is small)."""
 import math
 
 import pytest
@@ -27,7 +27,7 @@ def dev():
 
 # ------------------------------------------------------------------------------------------------ attention: definition
 def definition(q, k, v, heads, kv, mask=None, causal=False, prefix=None, documents=None, q_start=None, softcap=None,
-               slopes=None, table=None, buckets=None, scale=None, dout=None):
+               slopes=None, table=None, buckets=None, scale=None, dout=None, pairs=None):
     """64-bit values and bounds: {"out": (value, bound), ...}; operands (B, S, heads, d)"""
     dt = q.dtype
     u = U[dt]
@@ -69,6 +69,8 @@ def definition(q, k, v, heads, kv, mask=None, causal=False, prefix=None, documen
     if documents is not None:
         mine = documents.long().gather(1, i.clamp(0, Sk - 1))
         see &= (documents.long()[:, None, :] == mine[:, :, None]) & (mine >= 0)[:, :, None]
+    if pairs is not None:
+        see &= pairs
     see = see[:, None]
     h = E * ((d + 8) * mag + 8 * x.abs() + (4 * softcap if softcap and dt == torch.bfloat16 else 0.0) + 8)
     h = torch.where(see, h, torch.zeros_like(h)).amax(-1, keepdim=True)
@@ -433,6 +435,171 @@ def test_attention_offsets_beyond_32_bits():
     assert torch.equal(ops.biased_attention(q[:, :1], k, v, 2, 1), ops.biased_attention(q[:, :1], k.clone(), v.clone(), 2, 1))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Sq,heads,kv,d", [(1, 4, 4, 64), (1, 32, 1, 128), (4, 12, 3, 80), (16, 4, 1, 32), (7, 33, 11, 16)])
+def test_few_queries_with_masks_documents_prefix_and_bias(Sq, heads, kv, d, dtype):
+    """the split form: packed rows of several tiles, key splits that end inside a tile, rows and splits that see nothing"""
+    B, Sk = 3, 333
+    g = torch.Generator().manual_seed(Sq)
+    mask = (torch.rand(B, Sk, generator=g) < 0.6).long().cuda()
+    mask[1] = 0
+    docs = torch.randint(-1, 3, (B, Sk), generator=g).sort(1)[0].to(torch.int32).cuda()
+    start = torch.tensor([Sk - Sq, 3, 100], dtype=torch.int32, device="cuda")
+    prefix = torch.tensor([0, 50, 400], dtype=torch.int32, device="cuda")
+    grad = dtype == torch.float32 or Sq != 7
+    attention_case(B, Sq, Sk, heads, kv, d, dtype, seed=1, grad=grad, mask=mask, causal=True, q_start=start, softcap=9.0)
+    attention_case(B, Sq, Sk, heads, kv, d, dtype, seed=2, grad=grad, documents=docs, q_start=start, slopes=slopes_of(heads))
+    attention_case(B, Sq, Sk, heads, kv, d, dtype, seed=3, grad=grad, documents=docs, mask=mask, causal=True, prefix=prefix,
+                   q_start=start, **table_of(16, heads, 40, True))
+    attention_case(B, Sq, Sk, heads, kv, d, dtype, seed=4, grad=False, **table_of(256, heads, 1024, True, grad=False))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d,causal", [(torch.bfloat16, 128, True), (torch.bfloat16, 64, False), (torch.float32, 96, True)])
+def test_attention_longer_rows(dtype, d, causal):
+    """many chunks, several parts of a walk, several document tiles beyond the first 64"""
+    S = 4500 if dtype == torch.bfloat16 else 1500
+    docs = (torch.arange(S, device="cuda") // 700).to(torch.int32)[None]
+    attention_case(1, S, S, 2, 1, d, dtype, seed=1, causal=causal, softcap=30.0, documents=docs)
+    attention_case(1, S, S, 2, 1, d, dtype, seed=2, causal=causal, **table_of(32, 2, 300, not causal))
+
+
+@gpu
+def test_attention_many_rows_of_one_length():
+    """the block order over XCDs: pairs that divide by 8 and that do not, with and without a causal mask"""
+    for B, heads, kv in ((9, 4, 4), (8, 4, 2), (33, 1, 1), (16, 2, 1)):
+        for causal in (False, True):
+            attention_case(B, 140, 140, heads, kv, 16, torch.bfloat16, seed=B, causal=causal, mask=padded(B, 140, B))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_forward_and_backward_captured(dtype, d):
+    """a whole pass of both operators in one graph, replayed on new values with eager work in between"""
+    from nonauto_lm_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    B, S, H, G = 2, 150, 4, 2
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)
+    static = [n(B, S, H, d), n(B, S, G, d), n(B, S, G, d), n(B, S, H, d)]
+    const = dict(frequencies=ops.rotary_frequencies(d, device="cuda"))
+    opt = table_of(32, H, 64, False)
+    qw = torch.ones(d, device="cuda")
+    mask = padded(B, S, 1)
+
+    def passes():
+        q, k, v = (t.detach().requires_grad_(True) for t in static[:3])          # leaves of this pass alone
+        w, table = qw.detach().requires_grad_(True), opt["table"].detach().requires_grad_(True)
+        rq, rk = ops.qk_norm_rotary(q, k, H, G, q_weight=w, k_weight=w, **const)
+        out = ops.biased_attention(rq, rk, v, H, G, mask=mask, causal=True, softcap=20.0, table=table, buckets=opt["buckets"])
+        return [out.detach()] + list(torch.autograd.grad(out, [q, k, v, w, table], static[3]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = passes()
+    for _ in range(3):
+        for t in static:
+            t.copy_(n(*t.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, passes()):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_attention_saved_state():
+    """one graph walked twice, operands that are one tensor, a constant that changed between the passes"""
+    from nonauto_lm_amd import ops
+    x = torch.randn(2, 50, 2, 32, device="cuda").requires_grad_(True)
+    dout = torch.randn(2, 50, 2, 32, device="cuda")
+    out = ops.biased_attention(x, x, x, 2, causal=True, slopes=slopes_of(2))
+    a = torch.autograd.grad(out, x, dout, retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(out, x, dout)[0])
+    leaves = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    parts = torch.autograd.grad(ops.biased_attention(*leaves, 2, causal=True, slopes=slopes_of(2)), leaves, dout)
+    torch.testing.assert_close(a, parts[0] + parts[1] + parts[2], rtol=0, atol=8 * E * float(a.abs().max() + 1))
+    prefix = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
+    out = ops.biased_attention(x, x, x, 2, causal=True, prefix=prefix)
+    prefix.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, x, dout)
+    with pytest.raises(RuntimeError):                                            # no second derivative
+        y = ops.biased_attention(x, x, x, 2)
+        torch.autograd.grad(torch.autograd.grad(y.sum(), x, create_graph=True)[0].sum(), x)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 32), (torch.bfloat16, 32), (torch.bfloat16, 128)])
+def test_queries_that_see_nothing_may_hold_anything(dtype, d):
+    """causal rows before the first visible key, rows before the keys, padded documents: their q and dout meet no product"""
+    from nonauto_lm_amd import ops
+    B, S = 2, 170
+    for case in range(4):
+        mask = torch.ones(B, S, dtype=torch.long, device="cuda")
+        docs = start = None
+        blind = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+        rows = S
+        if case == 0:                                # left padding
+            mask[0, :75] = 0
+            mask[1] = 0
+            blind = mask == 0
+        elif case == 1:
+            docs = (torch.arange(S, device="cuda") // 50).to(torch.int32).repeat(B, 1)
+            docs[:, 100:135] = -1
+            blind = docs < 0
+        elif case == 2:
+            start = torch.tensor([-40, -500], dtype=torch.int32, device="cuda")
+            blind = torch.arange(S, device="cuda")[None] + start[:, None] < 0
+        else:                                        # few queries
+            rows = 9
+            start = torch.tensor([-4, 100], dtype=torch.int32, device="cuda")
+            blind = torch.arange(rows, device="cuda")[None] + start[:, None] < 0
+        _, q, k, v, dout = inputs(B, rows, S, 4, 2, d, dtype, seed=case, grad=False)
+        opt = dict(mask=mask, causal=True, documents=docs, q_start=start)
+        for bias in ({}, table_of(8, 4, 20, True)):
+            zero = blind[..., None, None]
+            ref = definition(q.masked_fill(zero, 0), k, v, 4, 2, softcap=20.0, dout=dout.masked_fill(zero, 0), **opt, **bias)
+            for junk in (0.0, float("nan"), float("inf"), torch.finfo(dtype).min):
+                leaves = [t.clone().requires_grad_(True) for t in (q.masked_fill(zero, junk), k, v)] + [t for n, t in bias.items() if n == "table"]
+                out = ops.biased_attention(*leaves[:3], 4, 2, softcap=20.0, **opt, **bias)
+                grads = torch.autograd.grad(out, leaves, dout.masked_fill(zero, junk))
+                # (a tile's scores take one of two forms of the cap together, so rows next to junk may round otherwise: bounds, not bits)
+                for n, t in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
+                    check(n, t, *ref[n])
+                assert out[blind].eq(0).all() and grads[0][blind].eq(0).all()
+
+
+@gpu
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_table_entries_that_hide(dtype, low):
+    """-inf or a lowest value in the table: those distances are out, as with a mask of that shape; a row with nothing left is zero"""
+    from nonauto_lm_amd import ops
+    S, R, H = 200, 40, 2
+    _, q, k, v, dout = inputs(2, S, S, H, H, 32, dtype, seed=5)
+    opt = table_of(4, H, R, False)
+    buckets = torch.arange(-R, R + 1, device="cuda").abs()
+    for seen in (buckets < 16, buckets == R, buckets == R + 1):               # near, far, none
+        table = opt["table"].detach().clone()
+        table[3] = low
+        ids = torch.where(seen, torch.randint(0, 3, seen.shape, device="cuda"), 3).to(torch.int32)
+        table.requires_grad_(True)
+        out = ops.biased_attention(q, k, v, H, table=table, buckets=ids)
+        grads = torch.autograd.grad(out, [q, k, v, table], dout)
+        rel = torch.arange(S, device="cuda")[None] - torch.arange(S, device="cuda")[:, None]
+        finite = table.detach().clone()
+        finite[3] = 0
+        ref = definition(q, k, v, H, H, dout=dout, table=finite.requires_grad_(True), buckets=ids, pairs=seen[rel.clamp(-R, R) + R])
+        for n, t in zip(("out", "dq", "dk", "dv", "dtable"), (out, *grads)):
+            check(n, t, *ref[n])
+        assert grads[3][3].eq(0).all()
+
+
 def refusals(fn, bad):
     for opt, match in bad:
         with pytest.raises(ValueError, match=match):
@@ -467,7 +634,7 @@ def test_attention_refusals(monkeypatch):
         (dict(table=z(8, 4), buckets=i32(4)), "odd length"), (dict(table=z(8, 4), buckets=i32(2051)), "odd length"),
         (dict(table=z(8, 4), buckets=z(5)), "odd length"),
         (dict(softcap=0.0), "softcap"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
-        (dict(softcap=float("inf")), "softcap"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=-0.5), "scale"),
+        (dict(softcap=float("inf")), "softcap"), (dict(softcap=1e-31), "too small"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=-0.5), "scale"),
         (dict(q=z(2, 10, 64)), "start at position -1"), (dict(q_start=-1), "start at position"),
         (dict(q_start=4, documents=i32(2, 9)), "documents reach"), (dict(q_start=z(2)), "q_start must be"),
         (dict(q_start=i32(3)), "q_start must be"),
@@ -635,3 +802,37 @@ def test_rotary_refusals(monkeypatch):
     for bad in ((0, 10.0), (3, 10.0), (4, 0.0)):
         with pytest.raises(ValueError):
             ops.rotary_frequencies(*bad)
+
+
+def test_entry_points_refuse_without_a_launch():
+    """the C entry points check their argument structs themselves: a status and a text, nothing enqueued"""
+    import ctypes
+    from nonauto_lm_amd import _lib as L
+    lib = L.lib()
+    p = 1 << 20                                       # never read: every call below is refused
+    base = dict(q=p, k=p, v=p, out=p, batch=2, q_len=40, k_len=40, heads=4, kv_heads=2, head_size=32, q_stride=(5120, 128, 32),
+                k_stride=(2560, 64, 32), v_stride=(2560, 64, 32), scale=0.2, dtype=1)
+    for bad, text in ((dict(dtype=2), "dtype"), (dict(kv_heads=3), "heads"), (dict(head_size=20), "head size"), (dict(head_size=136), "head size"),
+                      (dict(q_len=0), "lengths"), (dict(k_len=1 << 25), "lengths"), (dict(q=p + 8), "aligned"), (dict(v=None), "null"),
+                      (dict(q_stride=(5120, 127, 32)), "stride"), (dict(k_stride=(-64, 64, 32)), "stride"), (dict(prefix=p), "causal"),
+                      (dict(softcap=-1.0), "softcap"), (dict(softcap=1e-31), "too small"), (dict(scale=float("nan")), "scale"), (dict(slopes=p, table=p, buckets=p), "alternatives"),
+                      (dict(table=p, num_buckets=4, distance=4), "buckets"), (dict(table=p, buckets=p, num_buckets=300, distance=4), "buckets"),
+                      (dict(table=p, buckets=p, num_buckets=4, distance=2000), "distance"), (dict(mask=p), "codes"),
+                      (dict(q_start=-1), "q_start"), (dict(out=None), "out"), (dict(out_lo=p), "out_lo"), (dict(q_len=1, k_len=4000), "scratch"),
+                      (dict(batch=1 << 26), "many")):
+        rc = lib.mivae_biased_attention_fwd(ctypes.byref(L.AttentionArgs(**{**base, **bad})), None)
+        assert rc == -1 and text in lib.mivae_last_error().decode(), (bad, lib.mivae_last_error())
+    back = dict(base, lse=p, dout=p, scratch=p, dq=p)
+    for bad, text in ((dict(lse=None), "null"), (dict(dk=p), "together"), (dict(dtable=p), "table"), (dict(scratch=p + 4), "scratch"), (dict(dq=p + 2), "aligned")):
+        rc = lib.mivae_biased_attention_bwd(ctypes.byref(L.AttentionArgs(**{**back, **bad})), None)
+        assert rc == -1 and text in lib.mivae_last_error().decode(), (bad, lib.mivae_last_error())
+    rot = dict(q=p, k=p, q_out=p, k_out=p, batch=2, len=3, heads=4, kv_heads=2, head_size=32, q_stride=(384, 128, 32), k_stride=(192, 64, 32),
+               eps=1e-6, norm=1, dtype=0)
+    for bad, text in ((dict(dtype=5), "dtype"), (dict(head_size=31), "head size"), (dict(head_size=258), "head size"), (dict(batch=0), "batch"),
+                      (dict(heads=4095), "heads"), (dict(batch=1 << 20, len=1 << 12), "batch"), (dict(freq=p, rotary_dim=34), "rotary"),
+                      (dict(freq=p, rotary_dim=3), "rotary"), (dict(norm=0), "neither"), (dict(norm=0, freq=p, rotary_dim=4, q_weight=p), "weights"),
+                      (dict(eps=-1.0), "eps"), (dict(q_out=None), "output"), (dict(k=None), "operand"), (dict(dq_weight=p), "weight gradients")):
+        rc = lib.mivae_qk_norm_rotary_fwd(ctypes.byref(L.RotaryArgs(**{**rot, **bad})), None)
+        assert rc == -1 and text in lib.mivae_last_error().decode(), (bad, lib.mivae_last_error())
+    assert lib.mivae_qk_norm_rotary_bwd(ctypes.byref(L.RotaryArgs(**rot)), None) == -1 and "gradient" in lib.mivae_last_error().decode()
+    assert lib.mivae_biased_attention_fwd(None, None) == -1 and lib.mivae_qk_norm_rotary_fwd(None, None) == -1
