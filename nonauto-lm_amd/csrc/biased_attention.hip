@@ -122,13 +122,13 @@ __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, c
 // after chunk, a block far down a row of packed documents waited for up to 60 loads in a row before its first product).
 struct Walk {
   const i32x4* tiles;     // summaries of this batch row, or null
-  int n, end;             // rows, and the limit of the walk
+  int end;                // the limit of the walk
   int lo, hi;             // range of the block's codes
   int base;
   i32x4 mine;
   uint64_t meets;
-  __device__ __forceinline__ void init(const i32x4* t, int rows, int limit, int low, int high) {
-    tiles = t; n = rows; end = limit; lo = low; hi = high;
+  __device__ __forceinline__ void init(const i32x4* t, int limit, int low, int high) {
+    tiles = t; end = limit; lo = low; hi = high;
     base = -64;
     meets = 0;
     mine = i32x4{0, 0, 0, 0};
@@ -139,10 +139,11 @@ struct Walk {
     end = min(end, chunks * (i + 1) / n * kChunk);
     return from;
   }
-  // first chunk at or behind row c that counts, or something >= end; its summary.  All lanes of the wave have to be active.
+  // first chunk at or behind row c that counts, or something >= end; its summary, with only the rows before `end`: what keys
+  // behind every query's limit hold (the rest of a cache) must not meet a product.  All lanes of the wave have to be active.
   __device__ __forceinline__ int next(int c, i32x4& info) {
     if (tiles == nullptr) {
-      const uint64_t rows = low_rows(n - c);
+      const uint64_t rows = low_rows(end - c);
       info = i32x4{0, 0, (int)(unsigned)rows, (int)(unsigned)(rows >> 32)};
       return c;
     }
@@ -160,7 +161,11 @@ struct Walk {
         const int at = t - base + __builtin_ctzll(left);
 #pragma unroll
         for (int i = 0; i < 4; ++i) info[i] = __builtin_amdgcn_readlane(mine[i], at);
-        return (base + at) * kChunk;
+        c = (base + at) * kChunk;
+        const uint64_t rows = low_rows(end - c);
+        info[2] &= (int)(unsigned)rows;
+        info[3] &= (int)(unsigned)(rows >> 32);
+        return c;
       }
       c = (base + 64) * kChunk;
     }
@@ -184,7 +189,7 @@ __device__ __forceinline__ Walk key_walk(const BiasedArgs& a, const View& v, int
   Walk w;
   int lo = 0, hi = 0;
   if (v.docs) block_range(a.qtiles + b * (a.qpad / 64), row0, a.Sq, lo, hi);
-  w.init(v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr, a.Sk, v.limit(min(row0 + kRows, a.Sq) - 1), lo, hi);
+  w.init(v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr, v.limit(min(row0 + kRows, a.Sq) - 1), lo, hi);
   return w;
 }
 
@@ -721,7 +726,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
   int blo = 0, bhi = 0;
   if (v.codes) block_range(a.ktiles + b * (a.kpad / 64), row0, a.Sk, blo, bhi);
   Walk walk;
-  walk.init(a.sighted ? a.sighted + b * (a.qpad / 64) : nullptr, a.Sq, qend, blo, bhi);
+  walk.init(a.sighted ? a.sighted + b * (a.qpad / 64) : nullptr, qend, blo, bhi);
   // next chunk of queries of the group's heads that the block's keys may be seen from
   const int glast = bhi < 0 ? 0 : (share + 1) * a.group / split;          // (every key of the block hidden: none)
   struct Pos { int g, qc; };
@@ -736,8 +741,8 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
     return p;
   };
   typename Frag<T>::type kf[2 * NDB], vf[2 * NDB];
-  load_row<T, NDB>(kf, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + kvh * a.ks[2], kcode >= 0, a.d, hh);
-  load_row<T, NDB>(vf, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + kvh * a.vs[2], does_k && kcode >= 0, a.d, hh);
+  load_row<T, NDB>(kf, static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)key * a.ks[1] + kvh * a.ks[2], kcode >= 0 && first < a.Sq, a.d, hh);
+  load_row<T, NDB>(vf, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)key * a.vs[1] + kvh * a.vs[2], does_k && kcode >= 0 && first < a.Sq, a.d, hh);
   constexpr int NV = ROLES ? 1 : NDB;
   f32x16 dk[NDB], dv[NV];                // with roles, dk holds what the wave forms
 #pragma unroll

@@ -1,10 +1,10 @@
 // The biased attention (biased_attention.hip) for a few new queries over long keys: bound by reading the keys and values once.
 //
 // The queries of a batch row that share a key head, (position, head of the group), are packed into tiles of up to 32 rows, so
-// that one read of the keys serves all of them.  The keys are split over blocks and, inside a block, over four waves that
+// that one read of the keys serves all of them.  The keys are split over blocks and, inside a block, over two waves that
 // work by themselves: a wave brings 32 keys and values at a time into its own part of LDS (bf16: two buffers, direct loads,
 // two tiles of 16 KiB a wave on their way at d = 128, 128 KiB a CU), takes S^T = K Q^T, the softmax step and O^T += V^T P^T,
-// and no wave waits for another until its walk ends.  Then the block joins its four (max, sum, O), and with more than one
+// and no wave waits for another until its walk ends.  Then the block joins its waves' (max, sum, O), and with more than one
 // split a second kernel joins the blocks' in order.
 //
 // bf16: P enters its product as the sum of two bf16 values, P and what its rounding leaves.  The extra products are free
@@ -130,7 +130,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
   const i32x4* ktiles = v.codes ? a.ktiles + b * (a.kpad / 64) : nullptr;
   auto rows_at = [&](int key) -> unsigned {
-    const uint64_t all = ktiles ? rows_of(ktiles[key / 64]) : low_rows(a.Sk - key / 64 * 64);
+    uint64_t all = low_rows(end - key / 64 * 64);       // what keys behind every query's limit hold must not meet a product
+    if (ktiles) all &= rows_of(ktiles[key / 64]);
     return (unsigned)(all >> (key & 32));
   };
   S sk, sv;

@@ -538,10 +538,11 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     seen     key <= query with `causal`, or key < prefix[b] (int32 (B,), needs causal); mask (B, Sk) != 0; documents
              (int32 (B, Sk)) equal and not negative, the query's taken at its position.
 
-    A query that sees no key gives zeros and passes no gradient (`ops.attention` averages such a row instead).  Keys that the
-    mask or a negative document hides may hold anything, and so may queries that see no key and their gradients; all
-    other operands have to be finite, also where `causal` or documents hide them from some queries.  A table entry of -inf
-    or of fp32's or bf16's lowest value hides its pairs."""
+    A query that sees no key gives zeros and passes no gradient (`ops.attention` averages such a row instead).  Keys that no
+    query can see, for the mask, a negative document or because they lie behind the last query's limit (the unwritten end
+    of a cache), may hold anything, and so may queries that see no key and their gradients; all other operands have to be
+    finite, also where `causal` or documents hide them from some queries.  A table entry of -inf or of fp32's or
+    bf16's lowest value hides its pairs."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
     _operand_dtype("biased_attention", q, k, v)

@@ -575,6 +575,36 @@ def test_queries_that_see_nothing_may_hold_anything(dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 48), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("Sq", [1, 7, 16, 40, 150])
+def test_unwritten_end_of_a_cache(Sq, dtype, d):
+    """keys behind the last query's limit hold NaN: same bits as zeros, no gradient; with and without a mask, documents, a prefix"""
+    from nonauto_lm_amd import ops
+    B, Sk = 3, 500
+    _, q, k, v, dout = inputs(B, Sq, Sk, 4, 2, d, dtype, seed=Sq, grad=False)
+    start = torch.tensor([0, 33, 250], dtype=torch.int32, device="cuda")
+    prefix = torch.tensor([0, 60, 0], dtype=torch.int32, device="cuda")
+    for opt in (dict(), dict(mask=(torch.arange(Sk, device="cuda") % 3 > 0).long().expand(B, Sk)), dict(prefix=prefix),
+                dict(documents=(torch.arange(Sk, device="cuda") // 120).to(torch.int32).repeat(B, 1)), dict(slopes=slopes_of(4))):
+        limit = start + Sq
+        if "prefix" in opt:
+            limit = torch.maximum(limit, prefix)
+        behind = torch.arange(Sk, device="cuda")[None] >= limit[:, None]
+        results = []
+        for junk in (0.0, float("nan"), float("inf")):
+            fill = lambda t: t.masked_fill(behind[..., None, None], junk)
+            leaves = [q.clone().requires_grad_(True), fill(k).requires_grad_(True), fill(v).requires_grad_(True)]
+            out = ops.biased_attention(*leaves, 4, 2, causal=True, q_start=start, **opt)
+            with torch.no_grad():
+                assert torch.isfinite(ops.biased_attention(*leaves, 4, 2, causal=True, q_start=start, **opt)).all()
+            results.append([out] + list(torch.autograd.grad(out, leaves, dout)))
+        for r in results:
+            for a, b in zip(results[0], r):
+                assert torch.equal(a, b)
+            assert r[2][behind].eq(0).all() and r[3][behind].eq(0).all()
+
+
+@gpu
 @pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_table_entries_that_hide(dtype, low):
