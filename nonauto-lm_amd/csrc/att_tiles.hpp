@@ -38,7 +38,7 @@ struct BiasedArgs {
   const float* slopes;          // (heads), or null
   const float* table;           // (nb, heads), or null
   const int* buckets;           // (2 R + 1)
-  int B, Sq, Sk, heads, kv, group, d, q_start, causal, nb, R, kpad, qpad;
+  int B, Sq, Sk, heads, kv, group, d, q_start, causal, nb, R, kpad, qpad, makes_delta;
   float scale, cap;             // cap = 0: no cap
 };
 

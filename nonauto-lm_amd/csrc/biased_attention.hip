@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void k_ba_sighted(const float* lse, const int*
   if (lane == 0) tiles[w] = i32x4{lo, hi, (int)(unsigned)rows, (int)(unsigned)(rows >> 32)};
 }
 
-// ---- delta = sum_d dout * out: 16 lanes per (b, i, head) row -----------------------------------------------------------
+// ---- delta = sum_d dout * out where dk and dv alone are asked for (else the dq kernel forms it): 16 lanes per (b, i, head) row -----------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void k_ba_delta(const T* dout, const T* out, const unsigned short* lo, float* delta, int64_t rows, int Sq, int heads, int d) {
   const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -486,6 +486,26 @@ __device__ __forceinline__ float diagonal_sums(const f32x16& u, int lane) {
   return s0 + __int_as_float(__builtin_amdgcn_ds_permute(4 * ((lane + 36) & 63), __float_as_int(s1)));
 }
 
+// sum_d dout out of the lane's row, whose dout it holds (both half-waves)
+template <typename T, int NDB>
+__device__ __forceinline__ float row_delta(const typename Frag<T>::type (&dof)[2 * NDB], const BiasedArgs& a, int64_t at, bool live, int hh) {
+  float sum = 0.f;
+  typename Frag<T>::type o[2 * NDB];
+  load_row<T, NDB>(o, static_cast<const T*>(a.out) + at, live, a.d, hh);
+#pragma unroll
+  for (int s = 0; s < 2 * NDB; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf((float)dof[s][j], (float)o[s][j], sum);
+  if (sizeof(T) == 2 && a.out_lo != nullptr) {
+    load_row<T, NDB>(o, reinterpret_cast<const T*>(a.out_lo) + at, live, a.d, hh);
+#pragma unroll
+    for (int s = 0; s < 2 * NDB; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf((float)dof[s][j], (float)o[s][j], sum);
+  }
+  return sum + __shfl_xor(sum, 32, 64);
+}
+
 enum DqKind { kPlain, kTable, kDelta };
 
 template <typename T, int NDB, DqKind KIND>
@@ -524,11 +544,17 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   load_row<T, NDB>(dof, static_cast<const T*>(a.dout) + at_q, live, a.d, hh);
   const float lse = live ? a.lse[at_l] : INFINITY;
   const bool sighted = lse != INFINITY; // a row that sees no key passes no gradient, whatever it and its gradient hold
-  const float delta = !DELTA && sighted ? a.delta[at_l] : 0.f;
 #pragma unroll
   for (int s = 0; s < 2 * NDB; ++s) {
     qf[s] = sighted ? qf[s] : typename Frag<T>::type{};
     dof[s] = sighted ? dof[s] : typename Frag<T>::type{};
+  }
+  float delta = 0.f;
+  if (!DELTA && a.makes_delta) {
+    delta = row_delta<T, NDB>(dof, a, at_q, live, hh);
+    if (live && hh == 0 && slice == 0) a.delta[at_l] = delta;
+  } else if (!DELTA && sighted) {
+    delta = a.delta[at_l];
   }
   float dsum = 0.f;
   f32x16 dq[NDB];
@@ -1132,10 +1158,13 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     hipLaunchKernelGGL((k_ba_fold<std::remove_pointer_t<decltype(out0)>>), dim3((unsigned)(((out1 ? 2 : 1) * n4 + 255) / 256)), dim3(256), 0,
                        st, parts, out0, out1, n4, n);
   };
-  if (x->dtype == MIVAE_F32)
+  const bool exact = a.dtab && x->dtype == MIVAE_BF16;        // delta from a walk of its own
+  a.makes_delta = !exact && (a.dq || a.dtab);                 // by the dq kernel, on its way
+  if (a.makes_delta) {
+  } else if (x->dtype == MIVAE_F32)
     hipLaunchKernelGGL((k_ba_delta<float>), dgrid, dim3(256), 0, st, static_cast<const float*>(x->dout),
                        static_cast<const float*>(x->out), nullptr, a.delta, rows, a.Sq, a.heads, a.d);
-  else if (!a.dtab)
+  else if (!exact)
     hipLaunchKernelGGL((k_ba_delta<unsigned short>), dgrid, dim3(256), 0, st, static_cast<const unsigned short*>(x->dout),
                        static_cast<const unsigned short*>(x->out), a.out_lo, a.delta, rows, a.Sq, a.heads, a.d);
   else {

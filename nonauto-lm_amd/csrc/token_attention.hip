@@ -302,33 +302,47 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
 template <typename T>
 __global__ __launch_bounds__(64) void k_token_join(TokenArgs t) {
   const BiasedArgs& a = t.a;
-  const int64_t pr = blockIdx.x;
+  const int64_t pr = blockIdx.x;         // a row per block: below 2^31
   const int lane = threadIdx.x, pitch = a.d + 4;
   const float* p = t.part + pr * t.splits * pitch;
-  float top = -__FLT_MAX__;
-  for (int s = lane; s < t.splits; s += 64) top = fmaxf(top, p[s * pitch + a.d]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  float sum = 0.f;
-  for (int s = lane; s < t.splits; s += 64) sum = fmaf(__builtin_amdgcn_exp2f(p[s * pitch + a.d] - top), p[s * pitch + a.d + 1], sum);
-  sum = group_sum(sum, 64);
   int lpg = 1;                           // lanes per row of d / 4 groups, a power of two
   while (lpg < a.d / 4) lpg <<= 1;
-  const int c = (lane % lpg) * 4, stripes = 64 / lpg;
+  const int c = (lane % lpg) * 4, stripes = 64 / lpg, first = lane / lpg;
+  const bool on = c < a.d && first < t.splits;
+  // the first loads of all three parts go out together: with few splits they are all there are
+  float m0 = -__FLT_MAX__, l0 = 0.f, mx = 0.f;
+  f32x4 y0 = {0.f, 0.f, 0.f, 0.f};
+  if (lane < t.splits) {
+    m0 = p[lane * pitch + a.d];
+    l0 = p[lane * pitch + a.d + 1];
+  }
+  if (on) {
+    y0 = *reinterpret_cast<const f32x4*>(p + first * pitch + c);
+    mx = p[first * pitch + a.d];
+  }
+  float top = m0;
+  for (int s = lane + 64; s < t.splits; s += 64) top = fmaxf(top, p[s * pitch + a.d]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  float sum = __builtin_amdgcn_exp2f(m0 - top) * l0;
+  for (int s = lane + 64; s < t.splits; s += 64) sum = fmaf(__builtin_amdgcn_exp2f(p[s * pitch + a.d] - top), p[s * pitch + a.d + 1], sum);
+  sum = group_sum(sum, 64);
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  if (c < a.d)
+  if (on) {
+    x = y0 * __builtin_amdgcn_exp2f(mx - top);
 #pragma unroll 4
-    for (int s = lane / lpg; s < t.splits; s += stripes) {
+    for (int s = first + stripes; s < t.splits; s += stripes) {
       const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * pitch + c);
       const float f = __builtin_amdgcn_exp2f(p[s * pitch + a.d] - top);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = fmaf(f, y[j], x[j]);
     }
+  }
   for (int off = 32; off >= lpg; off >>= 1)
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], off, 64);
-  const int64_t pair = pr / t.rows, row = pr % t.rows, b = pair / a.kv;
-  const int64_t pos = row / a.group, head = pair % a.kv * a.group + row % a.group;
+  const unsigned pair = blockIdx.x / (unsigned)t.rows, row = blockIdx.x % (unsigned)t.rows, kvh = pair % (unsigned)a.kv;
+  const int64_t b = pair / (unsigned)a.kv, pos = row / (unsigned)a.group, head = kvh * a.group + row % (unsigned)a.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (lane < lpg && c < a.d)
     store_out(static_cast<T*>(a.out), a.out_lo, ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
