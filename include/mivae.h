@@ -105,7 +105,7 @@ typedef struct mivae_attention_args {
   void* out;
   void* out_lo;               /* bfloat16 training: shaped like out, receives what its rounding leaves (the backward's
                                  sum_d dout out takes it in); or NULL */
-  float* lse;                 /* (batch, heads, q_len): written forward (or NULL), read backward */
+  float* lse;                 /* (2, batch, heads, q_len): written forward (or NULL), read backward */
   const int64_t* mask;        /* (batch, k_len), or NULL.  The backward reads codes instead and only looks whether these */
   const int32_t* documents;   /* (batch, k_len), or NULL   two are NULL */
   const int32_t* prefix;      /* (batch), or NULL; needs causal */

@@ -24,7 +24,9 @@ struct BiasedArgs {
   int64_t qs[3], ks[3], vs[3];
   void* out;                    // (B, Sq, heads, d) contiguous
   unsigned short* out_lo;       // bf16: what the rounding of out leaves, or null
-  float* lse;                   // (B, heads, Sq): log2-domain log-sum-exp, +inf for a row that sees no key; may be null
+  // (2, B, heads, Sq), or null: m, then 1 / l, with p = 2^(score - m) / l; m = +inf and 0 for a row that sees no key.  (One
+  // m + log2 l instead is off by half its last place, 1e-6 at 20, in every p of the row alike: that much of an fp32 gradient.)
+  float* lse;
   const void* dout;             // (B, Sq, heads, d) contiguous
   float* delta;                 // (B, heads, Sq): sum_d dout * out
   void *dq, *dk, *dv;           // contiguous, may be null
@@ -195,6 +197,11 @@ struct Stage<float, NDB, NW> {
     }
   }
 };
+
+__device__ __forceinline__ void store_lse(const BiasedArgs& a, int64_t at, float m, float l) {
+  a.lse[at] = l == 0.f ? INFINITY : m;
+  a.lse[(int64_t)a.B * a.heads * a.Sq + at] = l == 0.f ? 0.f : 1.f / l;
+}
 
 // rows d = 32 db + 8 a + 4 hh .. + 3 of the transposed accumulators -> one row of a contiguous (.., d) tensor
 __device__ __forceinline__ void store4(unsigned short* p, float a, float b, float c, float e) {

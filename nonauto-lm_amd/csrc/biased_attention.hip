@@ -71,8 +71,7 @@ __global__ __launch_bounds__(256) void k_ba_codes(const int64_t* mask, const int
   }
 }
 
-// Backward: the summaries of the queries anew, with only the rows that see a key, i.e. whose log-sum-exp is finite for some
-// head.  dk and dv stage no others: whatever a blind row and its gradient hold must not meet a product, 0 * NaN is NaN.
+// Backward: the summaries of the queries anew, with only the rows that see a key, i.e. whose maximum is finite for some head.  dk and dv stage no others: whatever a blind row and its gradient hold must not meet a product, 0 * NaN is NaN.
 __global__ __launch_bounds__(256) void k_ba_sighted(const float* lse, const int* qcodes, int B, int Sq, int qpad, int heads, i32x4* tiles) {
   const int n = qpad / 64, lane = threadIdx.x & 63;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -450,8 +449,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
           store_out(static_cast<T*>(a.out), MODE == kTrainRest ? a.out_lo : nullptr, at + c, o[db][4 * a4] * inv, o[db][4 * a4 + 1] * inv, o[db][4 * a4 + 2] * inv,
                     o[db][4 * a4 + 3] * inv);
       }
-    if (MODE != kInfer && hh == 0)
-      a.lse[(b * a.heads + head) * a.Sq + qw.row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (MODE != kInfer && hh == 0) store_lse(a, (b * a.heads + head) * a.Sq + qw.row, m, l);
   }
 }
 
@@ -542,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   typename Frag<T>::type qf[2 * NDB], dof[2 * NDB];
   load_row<T, NDB>(qf, static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)qw.row * a.qs[1] + head * a.qs[2], live, a.d, hh);
   load_row<T, NDB>(dof, static_cast<const T*>(a.dout) + at_q, live, a.d, hh);
-  const float lse = live ? a.lse[at_l] : INFINITY;
+  const float lse = live ? a.lse[at_l] : INFINITY, inv = live ? a.lse[(int64_t)a.B * a.heads * a.Sq + at_l] : 0.f;
   const bool sighted = lse != INFINITY; // a row that sees no key passes no gradient, whatever it and its gradient hold
 #pragma unroll
   for (int s = 0; s < 2 * NDB; ++s) {
@@ -556,6 +554,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   } else if (!DELTA && sighted) {
     delta = a.delta[at_l];
   }
+  const float di = delta * inv;
   float dsum = 0.f;
   f32x16 dq[NDB];
 #pragma unroll
@@ -624,7 +623,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
         continue;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) u[r] = __builtin_amdgcn_exp2f(fmaf(A, u[r], cm)) * (dp[r] - delta);     // ds
+      for (int r = 0; r < 16; ++r) u[r] = __builtin_amdgcn_exp2f(fmaf(A, u[r], cm)) * fmaf(dp[r], inv, -di);     // ds
       if (grad_tab) {
         if (far) {
           float s = 0.f;
@@ -657,7 +656,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
     }
   }
   if (DELTA) {
-    dsum += __shfl_xor(dsum, 32, 64);
+    dsum = (dsum + __shfl_xor(dsum, 32, 64)) * inv;
     if (live && hh == 0) (part != nullptr ? part + slice * (((int64_t)a.B * a.heads * a.Sq + 3) / 4 * 4) : a.delta)[at_l] = dsum;
     return;
   }
@@ -726,7 +725,8 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
   T* tiles = reinterpret_cast<T*>(smem);                                  // [NBUF][Q, dO]
   float* lses = reinterpret_cast<float*>(tiles + 2 * NBUF * TILE);        // [NBUF][kChunk] each
   float* dels = lses + NBUF * kChunk;
-  int* qc_lds = reinterpret_cast<int*>(dels + NBUF * kChunk);
+  float* invs = dels + NBUF * kChunk;                                     // fp32 alone
+  int* qc_lds = reinterpret_cast<int*>(sizeof(T) == 4 ? invs + NBUF * kChunk : invs);
   float* tab = reinterpret_cast<float*>(qc_lds + NBUF * kChunk);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, hh = lane >> 5;
   const Ids id = ids_of(a.B, a.kv * split * cuts, (a.Sk + kRows - 1) / kRows, a.causal != 0, false);
@@ -779,7 +779,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
       dv[db % NV][r] = 0.f;
     }
   Stage<T, NDB, kWaves> sq, sd;
-  float pl = 0.f, pd = 0.f;
+  float pl = 0.f, pd = 0.f, pi = 0.f;
   int pq = 0, buf = 0;
   auto issue = [&](int n, Pos p) {
     const int head = kvh * a.group + p.g;
@@ -792,6 +792,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
     const int i = p.qc + (int)threadIdx.x;
     const bool in = threadIdx.x < kChunk && i < a.Sq;
     pl = in ? a.lse[(b * a.heads + head) * a.Sq + i] : INFINITY;    // rows beyond Sq: p = exp2(. - inf) = 0
+    pi = in ? a.lse[(b + a.B) * a.heads * a.Sq + (int64_t)head * a.Sq + i] : 0.f;
     pd = in ? a.delta[(b * a.heads + head) * a.Sq + i] : 0.f;
     if (v.docs && threadIdx.x < kChunk) pq = a.qcodes[b * a.qpad + i];
   };
@@ -807,7 +808,9 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
     sq.land(tiles + 2 * buf * TILE);
     sd.land(tiles + (2 * buf + 1) * TILE);
     if (threadIdx.x < kChunk) {
-      lses[buf * kChunk + threadIdx.x] = pl;
+      // bf16: m + log2 l, whose rounding is far below that of p to the operands' type
+      lses[buf * kChunk + threadIdx.x] = sizeof(T) == 4 || pl == INFINITY ? pl : pl - __builtin_amdgcn_logf(pi);
+      if (sizeof(T) == 4) invs[buf * kChunk + threadIdx.x] = pi;
       dels[buf * kChunk + threadIdx.x] = pl == INFINITY ? 0.f : pd;       // such a row's dout may hold anything
       qc_lds[buf * kChunk + threadIdx.x] = pq;
     }
@@ -876,6 +879,11 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
         const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * t + 8 * a4 + 4 * hh);
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[4 * a4 + i] = __builtin_amdgcn_exp2f(fmaf(A, u[4 * a4 + i], C - l4[i]));
+        if (sizeof(T) == 4) {
+          const f32x4 i4 = *reinterpret_cast<const f32x4*>(invs + buf * kChunk + 32 * t + 8 * a4 + 4 * hh);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[4 * a4 + i] *= i4[i];
+        }
       }
       typename Frag<T>::type x0, x1;
       if (does_v) {
@@ -1199,7 +1207,7 @@ int mivae_biased_attention_bwd(const mivae_attention_args* x, void* stream) {
     const int pieces = p.split * p.cuts;
     const dim3 kgrid((unsigned)grid_of((int64_t)a.B * a.kv * pieces, (a.Sk + kRows - 1) / kRows, a.causal));
     by_shape(x->dtype, a.d, [&](auto t, auto n) {
-      start_dkv<decltype(t), n()>(kgrid, tile_bytes(x->dtype, a.d, 3) + tw * 4, st, a, p, pieces > 1 ? parts : nullptr);
+      start_dkv<decltype(t), n()>(kgrid, tile_bytes(x->dtype, a.d, x->dtype == MIVAE_F32 ? 4 : 3) + tw * 4, st, a, p, pieces > 1 ? parts : nullptr);
     });
     if (pieces > 1) {
       const int64_t values = (int64_t)a.B * a.Sk * a.kv * a.d;

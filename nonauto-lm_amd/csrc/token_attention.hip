@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int64_t i1 = pr / a.group, h1 = kvh * a.group + pr % a.group;
       store_out(static_cast<T*>(a.out), a.out_lo, ((b * a.Sq + i1) * a.heads + h1) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-      if (a.lse && c == 0) a.lse[(b * a.heads + h1) * a.Sq + i1] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+      if (a.lse && c == 0) store_lse(a, (b * a.heads + h1) * a.Sq + i1, top, sum);
     } else {
       float* p = t.part + (((int64_t)pair * t.rows + pr) * t.splits + split) * (a.d + 4);
       store4(p + c, x[0], x[1], x[2], x[3]);
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(64) void k_token_join(TokenArgs t) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (lane < lpg && c < a.d)
     store_out(static_cast<T*>(a.out), a.out_lo, ((b * a.Sq + pos) * a.heads + head) * a.d + c, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-  if (a.lse && lane == 0) a.lse[(b * a.heads + head) * a.Sq + pos] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+  if (a.lse && lane == 0) store_lse(a, (b * a.heads + head) * a.Sq + pos, top, sum);
 }
 
 template <typename T, int NDB>

@@ -461,7 +461,7 @@ def _biased_attention_fwd(q, args, need_lse: bool):
     args.out = out.data_ptr()
     lse = codes = None
     if need_lse:
-        lse = torch.empty(args.batch, args.heads, args.q_len, dtype=torch.float32, device=dev)
+        lse = torch.empty(2, args.batch, args.heads, args.q_len, dtype=torch.float32, device=dev)
         args.lse = lse.data_ptr()
     if args.mask or args.documents:
         codes = torch.empty(_buffer_size("mivae_biased_attention_codes_ints", args.batch, args.q_len, args.k_len,
