@@ -233,22 +233,29 @@ __device__ __forceinline__ void store_row(T* dst, const f32x16 (&x)[NDB], float 
     }
 }
 
-// Scores of a block in base-2 exponent units.  The raw product x of a pair becomes u = x, or with a cap u = tanh(scale x / cap);
-// the score is then A u, A >= 0, plus the bias: linear, so that where the bias is constant over a tile everything folds into
-// the exponential's one fma.
+// Scores of a block.  The raw product x of a pair becomes u = x, or with a cap u = tanh(scale x / cap); the score is then
+// A u, A >= 0, plus the bias.  bf16: in base-2 exponent units, log2 e inside A and the bias, so that where the bias is constant
+// over a tile everything folds into the exponential's one fma.  fp32: in natural units, and log2 e in that fma: a rounded
+// A log2 e would err by up to 6e-8 of every score, alike over the row (log2 e itself: 1.3e-8).
+template <typename T>
+constexpr float kUnit = sizeof(T) == 4 ? 1.f : kLog2e;
+template <typename T>
+constexpr float kPost = sizeof(T) == 4 ? kLog2e : 1.f;
+
 struct Score {
   float A, k;         // k = scale / cap
-  float slope;        // slope * log2 e
+  float slope;
   bool cap, slopes, tab;
 };
 
+template <typename T>
 __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
   Score p;
   p.cap = a.cap > 0.f;
-  p.A = (p.cap ? a.cap : a.scale) * kLog2e;
+  p.A = (p.cap ? a.cap : a.scale) * kUnit<T>;
   p.k = p.cap ? a.scale / a.cap : 0.f;
   p.slopes = a.slopes != nullptr;
-  p.slope = p.slopes ? a.slopes[head] * kLog2e : 0.f;
+  p.slope = p.slopes ? a.slopes[head] * kUnit<T> : 0.f;
   p.tab = a.table != nullptr;
   return p;
 }
@@ -286,13 +293,17 @@ __device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
 }
 __device__ __forceinline__ float cap_slope(float u) { return fmaf(-u, u, 1.f); }
 
+__device__ __forceinline__ void scale_tile(f32x16& u, const Score& p) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) u[r] *= p.A;
+}
+
 // Element-wise part: u <- A u + bias.  Register r's relative distance key - query is rel + SIGN * acc_row(r) (SIGN = 1: the
 // lane is a query, -1: the lane is a key); rel0 is that of the wave's first lane's row to the tile's first.
 template <int SIGN>
 __device__ __forceinline__ void bias_tile(f32x16& u, const Score& p, const float* tab, int R, int rel, int rel0) {
   const bool behind = rel0 + 31 <= 0, inside = rel0 - 31 >= -R && rel0 + 31 <= R;        // wave-uniform
-#pragma unroll
-  for (int r = 0; r < 16; ++r) u[r] *= p.A;
+  scale_tile(u, p);
   if (p.slopes) {
     if (behind) {                       // every key at or behind its query: -slope |rel| is linear in the register's row
       const float base = p.slope * (float)rel;
@@ -315,11 +326,12 @@ __device__ __forceinline__ void bias_tile(f32x16& u, const Score& p, const float
   }
 }
 
-// the bias by relative distance of one head, in base-2 exponent units: tab[R + rel], rel = -R .. R
+// the bias by relative distance of one head: tab[R + rel], rel = -R .. R
+template <typename T>
 __device__ __forceinline__ void stage_table(float* tab, const BiasedArgs& a, int head, int nthreads) {
   for (int i = threadIdx.x; i <= 2 * a.R; i += nthreads) {
     const int b = min(max(a.buckets[i], 0), a.nb - 1);
-    tab[i] = a.table[(int64_t)b * a.heads + head] * kLog2e;
+    tab[i] = a.table[(int64_t)b * a.heads + head] * kUnit<T>;
   }
 }
 

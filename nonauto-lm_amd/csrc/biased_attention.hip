@@ -309,8 +309,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
   Walk walk = key_walk(a, v, b, row0);
   const int begin = walk.take(slice, slices);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
-  const Score sp = score_of(a, head);
-  if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
+  const Score sp = score_of<T>(a, head);
+  if (sp.tab) stage_table<T>(tab, a, head, 64 * kWaves);
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
   const T* vbase = static_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int* codes = v.codes ? a.kcodes + b * a.kpad : nullptr;
@@ -370,9 +370,14 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
         bias_tile<1>(u[t], sp, tab, a.R, key - (v.start + qw.row), rel0 + 32 * t);
         if (sees < 3) hide_keys(u[t], qw, sees == 2, key, kc_lds + buf * kChunk + 32 * t + 4 * hh);
       }
-      A = 1.f;
-    } else if (sp.tab) {
-      C = tab[rel0 < 0 ? 0 : 2 * a.R];
+      A = kPost<T>;
+    } else {
+      if (sizeof(T) == 4) {
+#pragma unroll
+        for (int t = 0; t < TW; ++t) scale_tile(u[t], sp);
+        A = kPost<T>;
+      }
+      if (sp.tab) C = tab[rel0 < 0 ? 0 : 2 * a.R] * kPost<T>;
     }
     float top = u[0][0];
 #pragma unroll
@@ -525,11 +530,11 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
   Walk walk = key_walk(a, v, b, row0);
   const int begin = walk.take(slice, slices);
   const QueryWave qw = query_wave(a, v, b, q0, r32);
-  const Score sp = score_of(a, head);
+  const Score sp = score_of<T>(a, head);
   const int TW = 2 * a.R + 1;
   float* hist = tab + TW;                                                 // [kWaves][TW]
   float* mine = hist + wave * TW;
-  if (sp.tab) stage_table(tab, a, head, 64 * kWaves);
+  if (sp.tab) stage_table<T>(tab, a, head, 64 * kWaves);
   if (grad_tab)
     for (int i = threadIdx.x; i < kWaves * TW; i += 64 * kWaves) hist[i] = 0.f;
   const T* kbase = static_cast<const T*>(a.k) + b * a.ks[0] + kvh * a.ks[2];
@@ -612,9 +617,13 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       if (sees < 3 || sp.slopes || (sp.tab && !far)) {
         bias_tile<1>(u, sp, tab, a.R, rel, rel0);
         if (sees < 3) hide_keys(u, qw, sees == 2, key0 + 4 * hh, kc_lds + buf * kChunk + 32 * t + 4 * hh);
-        A = 1.f;
-      } else if (sp.tab) {
-        C = tab[rel0 < 0 ? 0 : 2 * a.R];
+        A = kPost<T>;
+      } else {
+        if (sizeof(T) == 4) {
+          scale_tile(u, sp);
+          A = kPost<T>;
+        }
+        if (sp.tab) C = tab[rel0 < 0 ? 0 : 2 * a.R] * kPost<T>;
       }
       const float cm = C - lse;
       if (DELTA) {
@@ -799,7 +808,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
   Pos p = settle(Pos{share * a.group / split, qfirst});
   if (p.g < glast) issue(0, p);
   int tab_head = -1;
-  Score sp = score_of(a, kvh * a.group);
+  Score sp = score_of<T>(a, kvh * a.group);
   for (; p.g < glast; buf ^= NBUF - 1) {
     const Pos at = p;
     const int head = kvh * a.group + at.g;
@@ -815,9 +824,9 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
       qc_lds[buf * kChunk + threadIdx.x] = pq;
     }
     if (other_head) {
-      sp = score_of(a, head);
+      sp = score_of<T>(a, head);
       tab_head = head;
-      if (sp.tab) stage_table(tab, a, head, NT);
+      if (sp.tab) stage_table<T>(tab, a, head, NT);
     }
     __syncthreads();
     const i32x4 seen = info;
@@ -870,9 +879,13 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
             u[r] = see ? u[r] : -INFINITY;
           }
         }
-        A = 1.f;
-      } else if (sp.tab) {
-        C = tab[rel0 < 0 ? 0 : 2 * a.R];
+        A = kPost<T>;
+      } else {
+        if (sizeof(T) == 4) {
+          scale_tile(u, sp);
+          A = kPost<T>;
+        }
+        if (sp.tab) C = tab[rel0 < 0 ? 0 : 2 * a.R] * kPost<T>;
       }
 #pragma unroll
       for (int a4 = 0; a4 < 4; ++a4) {

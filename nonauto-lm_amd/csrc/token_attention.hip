@@ -106,12 +106,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   const bool same = !v.docs || (lo == hi && __builtin_amdgcn_ballot_w64(code < 0) == 0);
   const int begin = split * t.span, end = min(min(begin + t.span, a.Sk), v.limit(last_pos));
   const int clean_end = v.limit(first_pos);                               // every row sees the keys below
-  const Score sp = score_of(a, kvh * a.group);
-  const float slope = sp.slopes ? a.slopes[live ? head : 0] * kLog2e : 0.f;
+  const Score sp = score_of<T>(a, kvh * a.group);
+  const float slope = sp.slopes ? a.slopes[live ? head : 0] * kUnit<T> : 0.f;
   float far[2] = {0.f, 0.f};
   auto bias_at = [&](int rel) {
     const int n = min(max(a.buckets[min(max(rel, -a.R), a.R) + a.R], 0), a.nb - 1);
-    return a.table[(int64_t)n * a.heads + (live ? head : 0)] * kLog2e;
+    return a.table[(int64_t)n * a.heads + (live ? head : 0)] * kUnit<T>;
   };
   if (sp.tab) {
     far[0] = bias_at(-a.R);
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     float top = u[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, u[r]);
-    top = max_halves(top);
+    top = max_halves(top) * kPost<T>;
     const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - mn);
     if (__builtin_amdgcn_ballot_w64(mn > m) != 0) {
 #pragma unroll
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     float ps = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      u[r] = __builtin_amdgcn_exp2f(u[r] - m);
+      u[r] = __builtin_amdgcn_exp2f(fmaf(kPost<T>, u[r], -m));
       ps += u[r];
     }
     l += ps;
