@@ -302,17 +302,12 @@ __device__ __forceinline__ void scale_tile(f32x16& u, const Score& p) {
 // lane is a query, -1: the lane is a key); rel0 is that of the wave's first lane's row to the tile's first.
 template <int SIGN>
 __device__ __forceinline__ void bias_tile(f32x16& u, const Score& p, const float* tab, int R, int rel, int rel0) {
-  const bool behind = rel0 + 31 <= 0, inside = rel0 - 31 >= -R && rel0 + 31 <= R;        // wave-uniform
+  const bool inside = rel0 - 31 >= -R && rel0 + 31 <= R;        // wave-uniform
   scale_tile(u, p);
-  if (p.slopes) {
-    if (behind) {                       // every key at or behind its query: -slope |rel| is linear in the register's row
-      const float base = p.slope * (float)rel;
+  if (p.slopes) {                       // one rounding, of the score itself: forward and backward agree on it
+    const float from = (float)rel;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) u[r] += fmaf(p.slope, (float)(SIGN * acc_row(r)), base);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) u[r] = fmaf(-p.slope, fabsf((float)(rel + SIGN * acc_row(r))), u[r]);
-    }
+    for (int r = 0; r < 16; ++r) u[r] = fmaf(-p.slope, fabsf(from + (float)(SIGN * acc_row(r))), u[r]);
   }
   if (p.tab) {
     const float* t = tab + R + rel;

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     for (int r = 0; r < 16; ++r) u[r] *= sp.A;
     if (sp.slopes) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) u[r] = fmaf(-slope, fabsf((float)(rel + acc_row(r))), u[r]);
+      for (int r = 0; r < 16; ++r) u[r] = fmaf(-slope, fabsf((float)rel + (float)acc_row(r)), u[r]);
     }
     if (sp.tab) {
       const int rel_lo = key0 - (v.start + last_pos), rel_hi = key0 + 31 - (v.start + first_pos);
