@@ -72,6 +72,18 @@ __device__ __forceinline__ void pack8(f32x8& f, const f32x16& x, int s) {
   for (int j = 0; j < 8; ++j) f[j] = x[8 * s + j];
 }
 
+// what the rounding of x to fragments f0, f1 left, as fragments
+template <typename F>
+__device__ __forceinline__ void pack_rest(F& f0, F& f1, f32x16& x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] -= (float)f0[j];
+    x[8 + j] -= (float)f1[j];
+  }
+  pack8(f0, x, 0);
+  pack8(f1, x, 1);
+}
+
 __device__ __forceinline__ float to_f32(unsigned short u) { return bf16_to_f32(u); }
 __device__ __forceinline__ float to_f32(float f) { return f; }
 

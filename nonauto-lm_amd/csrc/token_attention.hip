@@ -232,13 +232,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
       o[db] = mma(L::col(vt, 16, db, lane), p1, o[db]);
     }
     if (sizeof(T) == 2) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u[j] -= (float)p0[j];
-        u[8 + j] -= (float)p1[j];
-      }
-      pack8(p0, u, 0);
-      pack8(p1, u, 1);
+      pack_rest(p0, p1, u);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         o[db] = mma(L::col(vt, 0, db, lane), p0, o[db]);
