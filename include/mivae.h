@@ -94,7 +94,8 @@ int mivae_attention_bwd(const void* q, const void* k, const void* v, const int64
  *   out_i = sum_j softmax_j(s) v_j over the keys j that query i sees, 0 where it sees none (and no gradient then).
  * i = q_start + row is the query's position, j the key's.  A query sees a key if (not causal, or j <= i, or j < prefix[b])
  * and mask[b][j] != 0 and documents[b][j] == documents[b][i] >= 0; each condition only where its pointer is given.
- * Keys that mask or a negative document hides may hold anything, NaN included.
+ * Keys that mask or a negative document hides, or that lie behind the last query's limit under causal, may hold anything,
+ * NaN included, and so may queries that see no key, and their dout.  A table entry of -inf hides its pairs.
  * Query head h reads key head h / (heads / kv_heads).  Operands float32 or bfloat16 (all of one dtype), element
  * (b, row, head, c) at base + b stride[0] + row stride[1] + head stride[2] + c, 16-byte aligned; out / dout / dq
  * (batch, q_len, heads, head_size) and dk / dv (batch, k_len, kv_heads, head_size) contiguous.
@@ -105,7 +106,8 @@ typedef struct mivae_attention_args {
   void* out;
   void* out_lo;               /* bfloat16 training: shaped like out, receives what its rounding leaves (the backward's
                                  sum_d dout out takes it in); or NULL */
-  float* lse;                 /* (2, batch, heads, q_len): written forward (or NULL), read backward */
+  float* lse;                 /* (2, batch, heads, q_len): m, then 1 / l, with p = 2^(s log2 e - m) / l; m = +inf for a query
+                                 that sees no key.  Written forward (or NULL), read backward */
   const int64_t* mask;        /* (batch, k_len), or NULL.  The backward reads codes instead and only looks whether these */
   const int32_t* documents;   /* (batch, k_len), or NULL   two are NULL */
   const int32_t* prefix;      /* (batch), or NULL; needs causal */
