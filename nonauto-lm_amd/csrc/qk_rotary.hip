@@ -3,7 +3,9 @@
 //   r = (mean_d x^2 + eps)^-1/2;  n = x r w;  a pair (a, b) of n at angle t: (a cos t - b sin t, a sin t + b cos t)
 //   dn = R(-t) dy;  dw = sum over rows of dn x r;  dx = r (dn w - x r mean_d(dn w x r))
 //
-// Bound by HBM: reads x and writes y once (backward: reads x and dy, writes dx).  A lane holds one or more chunks of VEC
+// Bound by HBM: reads x and writes y once (backward: reads x and dy, writes dx).  (2 x 8191 tokens, 16 + 4 heads of 96, fp32,
+// half rotated: 53 us and 76 us, 4.8 and 5.0 TB/s; 64 x 512, 4 + 4 heads of 128, bf16: 34 and 60 us, 4.0 and 3.4 TB/s, where
+// the VALU issues in 78 % and 65 % of the cycles.)  A lane holds one or more chunks of VEC
 // pairs of a head row, so the two halves of a pair meet in its registers whatever the pairing, and a row is a power of two
 // of neighbouring lanes.  The angles of a token are shared by all its heads: a block takes a few whole tokens and puts
 // their cosines and sines into LDS once.  t = 2 pi frac(position f) is reduced in 64 bits, where positions of 2^31 keep
