@@ -630,6 +630,42 @@ def test_table_entries_that_hide(dtype, low):
         assert grads[3][3].eq(0).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_widest_heads_with_the_longest_table(dtype):
+    """the largest LDS blocks: heads of 128, 2049 distances and their gradient"""
+    attention_case(1, 150, 150, 2, 1, 128, dtype, seed=1, softcap=25.0, **table_of(256, 2, 1024, True))
+    attention_case(1, 1500, 1500, 1, 1, 128, dtype, seed=2, causal=True, **table_of(64, 1, 1024, False))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_calls_in_flight(dtype):
+    """forward and backward on two streams at once: every call has workspaces of its own"""
+    from nonauto_lm_amd import ops
+    mask = padded(2, 400, 3)
+    sets = [inputs(2, 400, 400, 4, 2, 64, dtype, seed=s)[1:] for s in (1, 2)]
+    tables = [table_of(16, 4, 50, True, seed=s) for s in (1, 2)]
+
+    def passes(i):
+        q, k, v, dout = sets[i]
+        out = ops.biased_attention(q, k, v, 4, 2, mask=mask, causal=True, **tables[i])
+        return [out.detach()] + list(torch.autograd.grad(out, [q, k, v, tables[i]["table"]], dout))
+
+    want = [passes(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(passes(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
 def refusals(fn, bad):
     for opt, match in bad:
         with pytest.raises(ValueError, match=match):
