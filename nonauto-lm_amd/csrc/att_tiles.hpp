@@ -274,33 +274,53 @@ __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
 
 // u <- tanh(k u).  Scores well below the cap, the usual case, take y P(y^2) for |y| <= 3/4, P of degree 5 with the smallest
 // largest relative error (fitted on Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where
-// 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  A tile
-// with a larger |y| takes the latter, whose relative error is as small there.
-// ROUGH: always the latter (bf16 without gradients, where cap * 1e-7 is far below the output's own rounding), in one
-// basic block with the products around it.
-template <bool ROUGH>
+// 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  Larger |y|
+// take the latter, whose relative error is as small there.
+//   kCapRough: always the latter, in one basic block with the products around it (bf16 without gradients, where cap * 1e-7 is far
+//              below the output's own rounding; 8191 queries of 128: 515 us, 540 with kCapAhead)
+//   kCapEach:  by element (fp32, whose matrix instructions leave the VALU idle)
+//   kCapTile:  by tile: one with a larger |y| takes the latter for all (bf16 backward)
+//   kCapAhead: as kCapTile with the polynomial before the branch, where it overlaps the products (bf16 training forward: 114
+//              instead of 130 us at 4 x 16 x 4096 documents, 132 instead of 124 where every tile has larger ones; in dq and dk / dv
+//              it makes no difference there and costs registers)
+enum Cap { kCapRough, kCapEach, kCapTile, kCapAhead };
+__device__ __forceinline__ float tanh_near(float y) {
+  const float t = y * y;
+  float q = fmaf(t, -0.00471625663f, 0.0195829067f);
+  q = fmaf(t, q, -0.0533444285f);
+  q = fmaf(t, q, 0.133254066f);
+  q = fmaf(t, q, -0.333329588f);
+  return fmaf(t * y, q, y);
+}
+__device__ __forceinline__ float tanh_far(float y2) {      // of y2 / (2 log2 e)
+  return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y2)), 1.f);
+}
+template <Cap KIND>
 __device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
-  float most = 0.f;
-  if (!ROUGH) {
+  const float k2 = 2.f * kLog2e * p.k;
+  bool far = true;
+  f32x16 near = u;
+  if (KIND != kCapRough) {
+    float most = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(u[r]));
-    most *= p.k;
+    far = __builtin_amdgcn_ballot_w64(most * p.k > 0.75f) != 0;
   }
-  if (!ROUGH && __builtin_amdgcn_ballot_w64(most > 0.75f) == 0) {
+  if (KIND == kCapEach || KIND == kCapAhead) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      u[r] *= p.k;
-      const float t = u[r] * u[r];
-      float q = fmaf(t, -0.00471625663f, 0.0195829067f);
-      q = fmaf(t, q, -0.0533444285f);
-      q = fmaf(t, q, 0.133254066f);
-      q = fmaf(t, q, -0.333329588f);
-      u[r] = fmaf(t * u[r], q, u[r]);
+      near[r] = tanh_near(p.k * u[r]);
+      if (KIND == kCapAhead) asm volatile("" : "+v"(near[r]));          // here, not in the branch below
     }
-  } else {
+  }
+  if (far) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      u[r] = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * p.k * u[r])), 1.f);
+    for (int r = 0; r < 16; ++r) u[r] = KIND == kCapEach && fabsf(p.k * u[r]) <= 0.75f ? near[r] : tanh_far(k2 * u[r]);
+  } else if (KIND == kCapTile) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) u[r] = tanh_near(p.k * u[r]);
+  } else {
+    u = near;
   }
 }
 __device__ __forceinline__ float cap_slope(float u) { return fmaf(-u, u, 1.f); }

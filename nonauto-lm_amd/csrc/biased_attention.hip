@@ -17,7 +17,7 @@
 // Bound: bf16 by the VALU (a score costs an exponential, with a cap a tanh, and two conversions), fp32 by its matrix instructions.
 //   8191 causal queries of 16 + 4 heads of 128 with a cap, no gradient: 472 us, 583 TFLOP/s; the VALU issues in 76 % of the cycles
 //   4 x 4096, 16 + 4 heads of 64, causal, a table and its gradient: forward 265 us, delta 195, dq 390, dk and dv 480
-//   4 x 4096 in documents of 600, 16 heads of 64, a cap: forward 133 us, dq 136, dk and dv 185
+//   4 x 4096 in documents of 600, 16 heads of 64, a cap: forward 113 us, dq 136, dk and dv 185
 //   4 x 1001, 8 + 2 heads of 80, fp32, a prefix and slopes: forward 115 us, dq 143, dk and dv 193, joining the parts 29
 #include <type_traits>
 
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     }
     if (sp.cap) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) cap_tile<sizeof(T) == 2 && MODE == kInfer>(u[t], sp);
+      for (int t = 0; t < TW; ++t) cap_tile<sizeof(T) == 4 ? kCapEach : MODE == kInfer ? kCapRough : kCapAhead>(u[t], sp);
     }
     float A = sp.A, C = 0.f;
     const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       reads_ahead<T, 4 * NDB, 1>();
       f32x16 g;                          // the cap's slope
       if (sp.cap) {
-        cap_tile<false>(u, sp);
+        cap_tile<sizeof(T) == 4 ? kCapEach : kCapTile>(u, sp);
         if (!DELTA)
 #pragma unroll
           for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
@@ -870,7 +870,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
         for (int s = 0; s < 2 * NDB; ++s) dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
       f32x16 g;
       if (sp.cap) {
-        cap_tile<false>(u, sp);
+        cap_tile<sizeof(T) == 4 ? kCapEach : kCapTile>(u, sp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
       }
