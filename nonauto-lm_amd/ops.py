@@ -319,13 +319,46 @@ def _buffer_size(name: str, *args) -> int:
     return L.query(name, *args)
 
 
-def _refill(args, **tensors):
-    """A copy of a filled argument struct whose pointers are those of `tensors` (saved tensors may have moved)"""
+def _refill(args, strides, **tensors):
+    """A copy of a filled argument struct with the pointers of `tensors` and `strides` (field name -> values)"""
     args = type(args).from_buffer_copy(args)
     for name, t in tensors.items():
         if t is not None:
             setattr(args, name, t.data_ptr())
+    for name, st in strides.items():
+        setattr(args, name, st)
     return args
+
+
+def _keep(ctx, kept) -> None:
+    """Saves `kept` (argument struct's field name -> tensor) for the backward pass"""
+    ctx.save_for_backward(*kept.values())
+    ctx.names, ctx.kinds = tuple(kept), tuple((t.shape, t.dtype, t.device) for t in kept.values())
+
+
+def _kept(ctx, what: str, heads):
+    """What `_keep` saved as the kernels can read it, and the strides of the operands (`heads`: field name -> heads) and of
+    the positions.  A saved-tensor hook may return a tensor elsewhere and in another layout than the forward pass saw, so
+    both come from what it returned; another shape, type or device is an error."""
+    kept, strides = {}, {}
+    for name, kind, t in zip(ctx.names, ctx.kinds, ctx.saved_tensors):
+        if (t.shape, t.dtype, t.device) != kind:
+            raise RuntimeError(f"{what}: a saved-tensor hook returned {name} as {t.dtype} {tuple(t.shape)} on {t.device}, saved was "
+                               f"{kind[1]} {tuple(kind[0])} on {kind[2]}")
+        if name in heads:
+            t, _, _, _, strides[name + "_stride"] = _head_rows(t, heads[name], f"{what}: {name}")
+        elif name == "positions":
+            strides["position_stride"] = _position_strides(t)
+        else:
+            t = _aligned(t)
+        kept[name] = t
+    return kept, strides
+
+
+def _position_strides(positions):
+    """(batch, token) strides of positions (S,), (1, S) or (B, S)"""
+    st = positions.stride()
+    return (st[0] if positions.dim() == 2 and positions.size(0) > 1 else 0, st[-1])
 
 
 def _learns(*tensors) -> bool:
@@ -355,14 +388,14 @@ class _QkNormRotary(torch.autograd.Function):
         if kw is not None:
             kept["k_weight"] = kw
         kept.update(constants)
-        ctx.save_for_backward(*kept.values())
-        ctx.names, ctx.args, ctx.meta = tuple(kept), args, (q.shape, k.shape, q.dtype, q.device)
+        _keep(ctx, kept)
+        ctx.args, ctx.meta = args, (q.shape, k.shape, q.dtype, q.device)
         return yq, yk
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
-        kept = dict(zip(ctx.names, ctx.saved_tensors))
+        kept, strides = _kept(ctx, "qk_norm_rotary", {"q": ctx.args.heads, "k": ctx.args.kv_heads})
         qs, ks, dtype, dev = ctx.meta
         dyq, dyk = _aligned(dyq), _aligned(dyk)
         dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
@@ -374,7 +407,7 @@ class _QkNormRotary(torch.autograd.Function):
             if need_qw or need_kw:
                 scratch = torch.empty(_buffer_size("mivae_qk_norm_rotary_scratch_floats", ctx.args.head_size),
                                       dtype=torch.float32, device=dev)
-            args = _refill(ctx.args, dq_out=dyq, dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw,
+            args = _refill(ctx.args, strides, dq_out=dyq, dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw,
                            scratch=scratch, **kept)
             with L.on_device(dev):
                 L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream_of(dev))
@@ -422,8 +455,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optio
         if positions.dtype != torch.int64 or positions.shape not in ((S,), (1, S), (B, S)):
             raise ValueError(f"qk_norm_rotary: positions must be int64 (S,), (1, S) or (B, S), got {positions.dtype} {tuple(positions.shape)}")
         L.require_gpu(positions)
-        st = positions.stride()
-        args.position_stride = (st[0] if positions.shape == (B, S) and B > 1 else 0, st[-1])
+        args.position_stride = _position_strides(positions)
     elif positions is not None:
         args.start, positions = int(positions), None
     _same_device("qk_norm_rotary", q, k=k, q_weight=q_weight, k_weight=k_weight, frequencies=frequencies, positions=positions)
@@ -490,15 +522,16 @@ class _BiasedAttention(torch.autograd.Function):
         if codes is not None:
             kept["codes"] = codes
         kept.update(constants)
-        ctx.save_for_backward(*kept.values())
-        ctx.names, ctx.args = tuple(kept), args
+        _keep(ctx, kept)
+        ctx.args = args
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        kept = dict(zip(ctx.names, ctx.saved_tensors))
-        q, k, a = kept["q"], kept["k"], ctx.args
+        a = ctx.args
+        kept, strides = _kept(ctx, "biased_attention", {"q": a.heads, "k": a.kv_heads, "v": a.kv_heads})
+        q, k = kept["q"], kept["k"]
         dev, dtype = q.device, q.dtype
         dout = _aligned(dout)
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
@@ -510,7 +543,7 @@ class _BiasedAttention(torch.autograd.Function):
         scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.k_len, a.heads,
                                            a.kv_heads, a.head_size, a.num_buckets if need_t else 0),
                               dtype=torch.float32, device=dev)
-        args = _refill(a, dout=dout, dq=dq, dk=dk, dv=dv, dtable=dtable, scratch=scratch, **kept)
+        args = _refill(a, strides, dout=dout, dq=dq, dk=dk, dv=dv, dtable=dtable, scratch=scratch, **kept)
         with L.on_device(dev), _timed("biased_attention_bwd"):
             L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream_of(dev))
         return dq, dk if need_k else None, dv if need_v else None, dtable, None, None
