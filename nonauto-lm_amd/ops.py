@@ -11,6 +11,7 @@ from typing import Optional, Sequence, Tuple
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -361,6 +362,12 @@ def _position_strides(positions):
     return (st[0] if positions.dim() == 2 and positions.size(0) > 1 else 0, st[-1])
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """A launch would drop a forward-mode tangent without a word, so operands that carry one are refused"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: forward-mode derivatives are not offered")
+
+
 def _learns(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -397,6 +404,7 @@ class _QkNormRotary(torch.autograd.Function):
     def backward(ctx, dyq, dyk):
         kept, strides = _kept(ctx, "qk_norm_rotary", {"q": ctx.args.heads, "k": ctx.args.kv_heads})
         qs, ks, dtype, dev = ctx.meta
+        _no_tangents("qk_norm_rotary", dyq, dyk)
         dyq, dyk = _aligned(dyq), _aligned(dyk)
         dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
         need_qw, need_kw = ctx.needs_input_grad[2:4]
@@ -425,9 +433,11 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, heads: int, kv_heads: Optio
 
     q (B, S, heads * d) or (B, S, heads, d), k with kv_heads (default: heads), fp32 or bf16, d even, 2 .. 256.  positions:
     int64 (S,), (B, S) or (1, S), an int (position of the first token) or None (0).  The angle is reduced in 64 bits: far
-    positions lose nothing.  Outputs have the inputs' shapes, contiguous; gradients flow to q, k and the weights."""
+    positions lose nothing.  Outputs have the inputs' shapes, contiguous; gradients flow to q, k and the weights (in reverse
+    mode, once; operands with forward-mode tangents are refused)."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, q_weight, k_weight, frequencies)
+    _no_tangents("qk_norm_rotary", q, k, q_weight, k_weight, frequencies)
     _operand_dtype("qk_norm_rotary", q, k)
     if heads < 1 or kv_heads < 1:
         raise ValueError(f"qk_norm_rotary: {heads} and {kv_heads} heads")
@@ -533,6 +543,7 @@ class _BiasedAttention(torch.autograd.Function):
         kept, strides = _kept(ctx, "biased_attention", {"q": a.heads, "k": a.kv_heads, "v": a.kv_heads})
         q, k = kept["q"], kept["k"]
         dev, dtype = q.device, q.dtype
+        _no_tangents("biased_attention", dout)
         dout = _aligned(dout)
         need_q, need_k, need_v, need_t = ctx.needs_input_grad[:4]
         dq = torch.empty(q.shape, dtype=dtype, device=dev) if need_q else None
@@ -575,9 +586,10 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     query can see, for the mask, a negative document or because they lie behind the last query's limit (the unwritten end
     of a cache), may hold anything, and so may queries that see no key and their gradients; all other operands have to be
     finite, also where `causal` or documents hide them from some queries.  A table entry of -inf or of fp32's or
-    bf16's lowest value hides its pairs."""
+    bf16's lowest value hides its pairs.  Gradients in reverse mode, once; operands with forward-mode tangents are refused."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
+    _no_tangents("biased_attention", q, k, v, slopes, table)
     _operand_dtype("biased_attention", q, k, v)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"biased_attention: {heads} heads over {kv_heads} key heads")
