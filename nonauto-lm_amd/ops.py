@@ -331,27 +331,28 @@ def _refill(args, strides, **tensors):
     return args
 
 
-def _keep(ctx, kept) -> None:
-    """Saves `kept` (argument struct's field name -> tensor) for the backward pass"""
+def _keep(ctx, kept, read_by_stride) -> None:
+    """Saves `kept` (argument struct's field name -> tensor) for the backward pass.  The kernels read the tensors named in
+    `read_by_stride` by their strides, all others as contiguous ones."""
     ctx.save_for_backward(*kept.values())
-    ctx.names, ctx.kinds = tuple(kept), tuple((t.shape, t.dtype, t.device) for t in kept.values())
+    ctx.kinds = [(name, t.numel(), t.dtype, (t.shape, t.stride()) if name in read_by_stride else None) for name, t in kept.items()]
 
 
-def _kept(ctx, what: str, heads):
-    """What `_keep` saved as the kernels can read it, and the strides of the operands (`heads`: field name -> heads) and of
-    the positions.  A saved-tensor hook may return a tensor elsewhere and in another layout than the forward pass saw, so
-    both come from what it returned; another shape, type or device is an error."""
+def _kept(ctx, what: str, device, **heads):
+    """What `_keep` saved as the kernels can read it, and the strides (struct's field name -> values) that are not the forward
+    pass's.  A saved-tensor hook may return a tensor elsewhere and in another layout than the forward pass saw, so
+    both come from what it returned; another size, type or device is an error.  `heads`: of the operands."""
     kept, strides = {}, {}
-    for name, kind, t in zip(ctx.names, ctx.kinds, ctx.saved_tensors):
-        if (t.shape, t.dtype, t.device) != kind:
-            raise RuntimeError(f"{what}: a saved-tensor hook returned {name} as {t.dtype} {tuple(t.shape)} on {t.device}, saved was "
-                               f"{kind[1]} {tuple(kind[0])} on {kind[2]}")
-        if name in heads:
-            t, _, _, _, strides[name + "_stride"] = _head_rows(t, heads[name], f"{what}: {name}")
+    for (name, size, dtype, layout), t in zip(ctx.kinds, ctx.saved_tensors):
+        if t.numel() != size or t.dtype is not dtype or t.device != device or (layout is not None and t.shape != layout[0]):
+            raise RuntimeError(f"{what}: a saved-tensor hook returned {name} as {t.dtype} {tuple(t.shape)} on {t.device}, saved were "
+                               f"{size} elements of {dtype} on {device}" + (f", {tuple(layout[0])}" if layout is not None else ""))
+        if layout is None:
+            t = _aligned(t)
         elif name == "positions":
             strides["position_stride"] = _position_strides(t)
-        else:
-            t = _aligned(t)
+        elif t.stride() != layout[1] or t.data_ptr() % 16:
+            t, _, _, _, strides[name + "_stride"] = _head_rows(t, heads[name], f"{what}: {name}")
         kept[name] = t
     return kept, strides
 
@@ -395,15 +396,15 @@ class _QkNormRotary(torch.autograd.Function):
         if kw is not None:
             kept["k_weight"] = kw
         kept.update(constants)
-        _keep(ctx, kept)
+        _keep(ctx, kept, ("q", "k", "positions"))
         ctx.args, ctx.meta = args, (q.shape, k.shape, q.dtype, q.device)
         return yq, yk
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
-        kept, strides = _kept(ctx, "qk_norm_rotary", {"q": ctx.args.heads, "k": ctx.args.kv_heads})
         qs, ks, dtype, dev = ctx.meta
+        kept, strides = _kept(ctx, "qk_norm_rotary", dev, q=ctx.args.heads, k=ctx.args.kv_heads)
         _no_tangents("qk_norm_rotary", dyq, dyk)
         dyq, dyk = _aligned(dyq), _aligned(dyk)
         dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
@@ -532,15 +533,15 @@ class _BiasedAttention(torch.autograd.Function):
         if codes is not None:
             kept["codes"] = codes
         kept.update(constants)
-        _keep(ctx, kept)
-        ctx.args = args
+        _keep(ctx, kept, ("q", "k", "v"))
+        ctx.args, ctx.device = args, q.device
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         a = ctx.args
-        kept, strides = _kept(ctx, "biased_attention", {"q": a.heads, "k": a.kv_heads, "v": a.kv_heads})
+        kept, strides = _kept(ctx, "biased_attention", ctx.device, q=a.heads, k=a.kv_heads, v=a.kv_heads)
         q, k = kept["q"], kept["k"]
         dev, dtype = q.device, q.dtype
         _no_tangents("biased_attention", dout)

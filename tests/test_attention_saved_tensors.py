@@ -100,8 +100,9 @@ def test_backward_takes_the_strides_of_what_it_is_given(monkeypatch, dtype, layo
 def test_a_hook_that_returns_something_else_is_refused(monkeypatch):
     from nonauto_lm_amd import ops
     Recorder(monkeypatch)
-    x, q, k, v = packed(1, 20, 2, 2, 32, torch.float32, "cpu")
-    for other in (lambda t: t.double() if t.is_floating_point() else t, lambda t: t[..., :-1], lambda t: t.to("meta")):
+    x, q, k, v = packed(2, 20, 2, 2, 32, torch.float32, "cpu")
+    for other in (lambda t: t.double() if t.is_floating_point() else t, lambda t: t[..., :-1], lambda t: t.to("meta"),
+                  lambda t: t.transpose(0, 1) if t.dim() == 3 else t):
         with Hooks(other):
             out = ops.biased_attention(q, k, v, 2)
             rq, rk = ops.qk_norm_rotary(q, k, 2, frequencies=ops.rotary_frequencies(32))
