@@ -272,18 +272,19 @@ __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
   return p;
 }
 
-// u <- tanh(k u).  Scores well below the cap, the usual case, take y P(y^2) for |y| <= 3/4, P of degree 5 with the smallest
-// largest relative error (fitted on Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where
-// 1 - 2 / (1 + e^2y) takes two transcendental ones and is off by 1e-7 absolutely, i.e. by cap * 1e-7 in every score.  Larger |y|
-// take the latter, whose relative error is as small there.
-//   kCapRough: always the latter, in one basic block with the products around it (bf16 without gradients, where cap * 1e-7 is far
-//              below the output's own rounding; 8191 queries of 128: 515 us, 540 with kCapAhead)
-//   kCapEach:  by element (fp32, whose matrix instructions leave the VALU idle)
-//   kCapTile:  by tile: one with a larger |y| takes the latter for all (bf16 backward)
-//   kCapAhead: as kCapTile with the polynomial before the branch, where it overlaps the products (bf16 training forward: 114
-//              instead of 130 us at 4 x 16 x 4096 documents, 132 instead of 124 where every tile has larger ones; in dq and dk / dv
-//              it makes no difference there and costs registers)
-enum Cap { kCapRough, kCapEach, kCapTile, kCapAhead };
+// u <- tanh(k u).  |y| <= 3/4, the usual case, takes y P(y^2), P of degree 5 with the smallest largest relative error (fitted on
+// Chebyshev nodes; 1.5e-7 evaluated in fp32): 8 plain instructions an element, where 1 - 2 / (1 + e^2y) takes two
+// transcendental ones and is off by 2e-7 absolutely, i.e. by cap * 2e-7 in every score.  Larger |y| take the latter, whose relative
+// error is as small there.  Each element by itself: next to a score near a large cap, small ones keep their places.
+//   kCapRough: always the latter, in one basic block with the products around it (bf16 without gradients and caps up to kRoughCap,
+//              where an error of 1e-4 in the exponent stands against the 2e-3 of a probability's rounding; 8191 queries of 128:
+//              515 us, 540 with kCapAhead)
+//   kCapTile:  a tile whose |y| are all small leaves the transcendental instructions out (4 x 16 x 4096 documents, bf16: dq 139 us,
+//              dk and dv 187; with a larger one in every tile 162 and 207)
+//   kCapAhead: as kCapTile with the polynomial before that branch, where it overlaps the products (bf16 training forward: 115
+//              instead of 130 us at the same size, 126 with a larger one in every tile; in dq and dk / dv it makes no difference there and costs registers)
+enum Cap { kCapRough, kCapTile, kCapAhead };
+constexpr float kRoughCap = 512.f;
 __device__ __forceinline__ float tanh_near(float y) {
   const float t = y * y;
   float q = fmaf(t, -0.00471625663f, 0.0195829067f);
@@ -298,24 +299,29 @@ __device__ __forceinline__ float tanh_far(float y2) {      // of y2 / (2 log2 e)
 template <Cap KIND>
 __device__ __forceinline__ void cap_tile(f32x16& u, const Score& p) {
   const float k2 = 2.f * kLog2e * p.k;
-  bool far = true;
-  f32x16 near = u;
-  if (KIND != kCapRough) {
-    float most = 0.f;
+  if (KIND == kCapRough) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(u[r]));
-    far = __builtin_amdgcn_ballot_w64(most * p.k > 0.75f) != 0;
+    for (int r = 0; r < 16; ++r) u[r] = tanh_far(k2 * u[r]);
+    return;
   }
-  if (KIND == kCapEach || KIND == kCapAhead) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(u[r]));
+  const bool far = __builtin_amdgcn_ballot_w64(most * p.k > 0.75f) != 0;
+  f32x16 near = u;
+  if (KIND == kCapAhead) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       near[r] = tanh_near(p.k * u[r]);
-      if (KIND == kCapAhead) asm volatile("" : "+v"(near[r]));          // here, not in the branch below
+      asm volatile("" : "+v"(near[r]));          // here, not in the branch below
     }
   }
   if (far) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) u[r] = KIND == kCapEach && fabsf(p.k * u[r]) <= 0.75f ? near[r] : tanh_far(k2 * u[r]);
+    for (int r = 0; r < 16; ++r) {
+      const float y = p.k * u[r], n = KIND == kCapAhead ? near[r] : tanh_near(y);
+      u[r] = fabsf(y) <= 0.75f ? n : tanh_far(k2 * u[r]);
+    }
   } else if (KIND == kCapTile) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) u[r] = tanh_near(p.k * u[r]);

@@ -291,9 +291,10 @@ __device__ __forceinline__ Ids ids_of(int B, int heads, int nblk, bool causal, b
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-// kInfer: no lse, bf16 with the rough tanh.  kTrain: lse.  kTrainRest (bf16): also the rounding's rest of large probabilities and
-// the output's residue, for delta = dout . out.  (Modes, not branches: a branch between the products and the exponentials
-// of a chunk keeps them from overlapping, 7 % at 8191 queries of 128.)
+// kInfer: no lse, bf16 with the rough tanh (a cap above kRoughCap takes kTrain, which then leaves no lse).  kTrain: lse.
+// kTrainRest (bf16): also the rounding's rest of large probabilities and the output's residue, for delta = dout . out.
+// (Modes, not branches: a branch between the products and the exponentials of a chunk keeps them from overlapping, 7 % at
+// 8191 queries of 128.)
 enum Mode { kInfer, kTrain, kTrainRest };
 
 // slices > 1: a block takes one of that many equal parts of its rows' walk and leaves (O, max, sum) in `part`, laid out for
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
     }
     if (sp.cap) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) cap_tile<sizeof(T) == 4 ? kCapEach : MODE == kInfer ? kCapRough : kCapAhead>(u[t], sp);
+      for (int t = 0; t < TW; ++t) cap_tile<sizeof(T) == 4 ? kCapTile : MODE == kInfer ? kCapRough : kCapAhead>(u[t], sp);
     }
     float A = sp.A, C = 0.f;
     const bool near = sp.tab && rel0 + kChunk - 1 > -a.R && rel0 - 31 < a.R;
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_fwd(
           store_out(static_cast<T*>(a.out), MODE == kTrainRest ? a.out_lo : nullptr, at + c, o[db][4 * a4] * inv, o[db][4 * a4 + 1] * inv, o[db][4 * a4 + 2] * inv,
                     o[db][4 * a4 + 3] * inv);
       }
-    if (MODE != kInfer && hh == 0) store_lse(a, (b * a.heads + head) * a.Sq + qw.row, m, l);
+    if (MODE != kInfer && a.lse != nullptr && hh == 0) store_lse(a, (b * a.heads + head) * a.Sq + qw.row, m, l);
   }
 }
 
@@ -610,7 +611,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 ? 1 : 2) void k_ba_dq(B
       reads_ahead<T, 4 * NDB, 1>();
       f32x16 g;                          // the cap's slope
       if (sp.cap) {
-        cap_tile<sizeof(T) == 4 ? kCapEach : kCapTile>(u, sp);
+        cap_tile<kCapTile>(u, sp);
         if (!DELTA)
 #pragma unroll
           for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
@@ -870,7 +871,7 @@ __global__ __launch_bounds__(64 * kWaves * (by_roles<T, NDB>() ? 2 : 1), sizeof(
         for (int s = 0; s < 2 * NDB; ++s) dp = mma(L::row(dt, 32 * t + r32, s, hh), vf[s], dp);
       f32x16 g;
       if (sp.cap) {
-        cap_tile<sizeof(T) == 4 ? kCapEach : kCapTile>(u, sp);
+        cap_tile<kCapTile>(u, sp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) g[r] = cap_slope(u[r]);
       }
@@ -1153,7 +1154,7 @@ int mivae_biased_attention_fwd(const mivae_attention_args* x, void* stream) {
   const dim3 grid((unsigned)grid_of((int64_t)a.B * a.heads * slices, (a.Sq + kRows - 1) / kRows, a.causal));
   by_shape(x->dtype, a.d, [&](auto t, auto n) {
     if (a.out_lo) start(k_ba_fwd<unsigned short, n(), kTrainRest>, grid, lds, S_(stream), a, slices, part);     // bf16 alone has it
-    else if (a.lse) start(k_ba_fwd<decltype(t), n(), kTrain>, grid, lds, S_(stream), a, slices, part);
+    else if (a.lse || a.cap > kRoughCap) start(k_ba_fwd<decltype(t), n(), kTrain>, grid, lds, S_(stream), a, slices, part);
     else start(k_ba_fwd<decltype(t), n(), kInfer>, grid, lds, S_(stream), a, slices, part);
   });
   MIVAE_CHECK_LAUNCH("mivae_biased_attention_fwd");

@@ -172,8 +172,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
 #pragma unroll
     for (int s = 0; s < 2 * NDB; ++s) u = mma(L::row(kt, r32, s, hh), qf[s], u);
     if (sp.cap) {
-      if (sizeof(T) == 2 && a.lse == nullptr) cap_tile<kCapRough>(u, sp);
-      else cap_tile<sizeof(T) == 4 ? kCapEach : kCapTile>(u, sp);
+      if (sizeof(T) == 2 && a.lse == nullptr && a.cap <= kRoughCap) cap_tile<kCapRough>(u, sp);
+      else cap_tile<kCapTile>(u, sp);
     }
     const int key = key0 + 4 * hh, rel = key - qpos;
 #pragma unroll
