@@ -13,6 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmivae.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
+RECIPE = os.path.abspath(__file__)       # an object compiled with other flags is out of date like one of another source
 SOURCES = ["elementwise.hip", "nice_stack.hip", "nice_small.hip", "nice_big.hip", "invlinear.hip", "pairwise.hip", "mixed_stack.hip", "attention.hip", "biased_attention.hip", "token_attention.hip", "qk_rotary.hip", "nll.hip", "optim.hip", "layernorm.hip", "linear.hip", "maf.hip"]
 # packed-fp32-ops off: hipcc -O3 otherwise forms v_pk_{add,mul,fma}_f32 from ordinary float code, and some operand forms
 # of these have been seen to return wrong values now and then.  (The host pass warns that it does not know the feature.)
@@ -41,7 +42,7 @@ def build(force=False, verbose=True):
     def compile_one(pair):
         src, obj = pair
         with open(src) as f:
-            deps = [src] + headers + ([abi] if '"mivae.h"' in f.read() else [])
+            deps = [src, RECIPE] + headers + ([abi] if '"mivae.h"' in f.read() else [])
         if force or _newer(obj, deps):
             cmd = [hipcc] + FLAGS + ["-I", INCLUDE] + EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
             if verbose:
