@@ -514,6 +514,7 @@ class MultiHeadAttention(torch.nn.Module):
             self._relative_bias = torch.nn.Parameter(torch.zeros(count, num_heads))
             self.register_buffer("_buckets", ops.relative_buckets(count, relative_bias.get("max_distance", 128),
                                                                   not mask_tril), persistent=False)
+        self._query_norm = self._key_norm = None
         if self._qk_norm:
             self._query_norm = torch.nn.Parameter(torch.ones(self._attn_size))
             self._key_norm = torch.nn.Parameter(torch.ones(self._attn_size))
@@ -537,9 +538,10 @@ class MultiHeadAttention(torch.nn.Module):
     def _scored_attention(self, q, k, v, mask, documents, prefix):
         """(B, Sq, heads * d), (B, Sk, kv_heads * d) projections -> (B, Sq, heads * d)"""
         freqs, slopes = self._scored_constants(q.device)
+        # the operators read scales and table as fp32, also where the module is cast to bf16
+        query_norm, key_norm, table = (None if p is None else p.float() for p in (self._query_norm, self._key_norm, self._relative_bias))
         if self._qk_norm or self._rotary:
-            norm = dict(norm=self._qk_norm, q_weight=self._query_norm if self._qk_norm else None,
-                        k_weight=self._key_norm if self._qk_norm else None, frequencies=freqs)
+            norm = dict(norm=self._qk_norm, q_weight=query_norm, k_weight=key_norm, frequencies=freqs)
             if q.size(1) == k.size(1):
                 q, k = ops.qk_norm_rotary(q, k, self._num_heads, self._kv_heads, **norm)
             else:                       # the queries are the last positions of the keys: two passes, one half of each kept
@@ -548,8 +550,8 @@ class MultiHeadAttention(torch.nn.Module):
                 q = ops.qk_norm_rotary(q_, k_[:, back:], self._num_heads, self._kv_heads, positions=back, **norm)[0]
                 k = ops.qk_norm_rotary(k_, k_, self._kv_heads, self._kv_heads, **norm)[1]
         return ops.biased_attention(q, k, v, self._num_heads, self._kv_heads, mask=mask, causal=self._mask_tril, prefix=prefix,
-                                    documents=documents, softcap=self._softcap, slopes=slopes, table=self._relative_bias,
-                                    buckets=None if self._relative_bias is None else self._buckets)
+                                    documents=documents, softcap=self._softcap, slopes=slopes, table=table,
+                                    buckets=None if table is None else self._buckets)
 
     def _split(self, x):
         b, s, _ = x.shape
