@@ -67,11 +67,17 @@ struct WaveStage<float, NDB> {
   }
 };
 
+// No read or write of memory is moved across it by the compiler.  A wave's tile is written by other lanes than read it (and with
+// bf16 by loads that the compiler does not know), with no barrier in between: the LDS serves a wave's own accesses in order.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
+
 // wait until at most `newer` of the wave's vector loads are outstanding
 template <int NEWER>
 __device__ __forceinline__ void wait_loads() {
   static_assert(NEWER < 64, "six bits");
+  keep_order();
   __builtin_amdgcn_s_waitcnt(0x0f70 | (NEWER & 15) | (NEWER >> 4) << 14);
+  keep_order();
 }
 
 struct TokenArgs {
@@ -146,7 +152,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
   if (key0 < end) issue(0, key0);
   for (; key0 < end; key0 += kSpan, buf ^= NBUF - 1) {
     const int next = key0 + kSpan;
+    keep_order();
     __builtin_amdgcn_s_waitcnt(0xc07f);                 // lgkmcnt(0): the other buffer has been read to its end
+    keep_order();
     if (NBUF == 2) {
       if (next < end) {
         issue(buf ^ 1, next);
@@ -159,6 +167,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_token(TokenArgs t) {
     T* vt = kt + TILE;
     sk.land(kt);
     sv.land(vt);
+    keep_order();
     if (NBUF == 1 && next < end) issue(0, next);
     bool clean = key0 + kKeys <= clean_end;
     if (ktiles != nullptr) {
