@@ -620,7 +620,7 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     if mask is not None:
         if mask.shape != (B, Sk):
             raise ValueError(f"biased_attention: mask {tuple(mask.shape)} does not match (B, Sk) = {(B, Sk)}")
-        mask = _mask_i64(mask)
+        mask = _mask_i64(mask.ne(0) if mask.is_floating_point() else mask)       # (0.5 counts, and would become 0)
         args.mask = mask.data_ptr()
     for name, t, shape, dtype in (("prefix", prefix, (B,), torch.int32), ("documents", documents, (B, Sk), torch.int32),
                                   ("slopes", slopes, (heads,), torch.float32)):
