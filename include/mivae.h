@@ -95,7 +95,8 @@ int mivae_attention_bwd(const void* q, const void* k, const void* v, const int64
  * i = q_start + row is the query's position, j the key's.  A query sees a key if (not causal, or j <= i, or j < prefix[b])
  * and mask[b][j] != 0 and documents[b][j] == documents[b][i] >= 0; each condition only where its pointer is given.
  * Keys that mask or a negative document hides, or that lie behind the last query's limit under causal, may hold anything,
- * NaN included, and so may queries that see no key, and their dout.  A table entry of -inf hides its pairs.
+ * NaN included, and so may queries that see no key, and their dout.  A table entry of -inf hides its pairs after the products:
+ * what they are made of has to be finite, also for a query that keeps none (out 0, no gradient).
  * Query head h reads key head h / (heads / kv_heads).  Operands float32 or bfloat16 (all of one dtype), element
  * (b, row, head, c) at base + b stride[0] + row stride[1] + head stride[2] + c, 16-byte aligned; out / dout / dq
  * (batch, q_len, heads, head_size) and dk / dv (batch, k_len, kv_heads, head_size) contiguous.

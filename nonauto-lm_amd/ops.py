@@ -587,7 +587,8 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     query can see, for the mask, a negative document or because they lie behind the last query's limit (the unwritten end
     of a cache), may hold anything, and so may queries that see no key and their gradients; all other operands have to be
     finite, also where `causal` or documents hide them from some queries.  A table entry of -inf or of fp32's or
-    bf16's lowest value hides its pairs.  Gradients in reverse mode, once; operands with forward-mode tangents are refused."""
+    bf16's lowest value hides its pairs; a query whose pairs the table hides one and all gives zeros too, but has to be finite,
+    as its gradient has.  Gradients in reverse mode, once; operands with forward-mode tangents are refused."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
     _no_tangents("biased_attention", q, k, v, slopes, table)
