@@ -320,17 +320,6 @@ def _buffer_size(name: str, *args) -> int:
     return L.query(name, *args)
 
 
-def _refill(args, strides, **tensors):
-    """A copy of a filled argument struct with the pointers of `tensors` and `strides` (field name -> values)"""
-    args = type(args).from_buffer_copy(args)
-    for name, t in tensors.items():
-        if t is not None:
-            setattr(args, name, t.data_ptr())
-    for name, st in strides.items():
-        setattr(args, name, st)
-    return args
-
-
 def _keep(ctx, kept, read_by_stride) -> None:
     """Saves `kept` (argument struct's field name -> tensor) for the backward pass.  The kernels read the tensors named in
     `read_by_stride` by their strides, all others as contiguous ones."""
@@ -339,10 +328,10 @@ def _keep(ctx, kept, read_by_stride) -> None:
 
 
 def _kept(ctx, what: str, device, **heads):
-    """What `_keep` saved as the kernels can read it, and the strides (struct's field name -> values) that are not the forward
-    pass's.  A saved-tensor hook may return a tensor elsewhere and in another layout than the forward pass saw, so
-    both come from what it returned; another size, type or device is an error.  `heads`: of the operands."""
-    kept, strides = {}, {}
+    """What `_keep` saved, as the kernels can read it, and a copy of the forward pass's struct that points there.  A saved-tensor
+    hook may return a tensor elsewhere and in another layout than the forward pass saw, so addresses and strides are those of
+    what it returned; another size, type or device is an error.  `heads`: of the operands."""
+    kept, args = {}, type(ctx.args).from_buffer_copy(ctx.args)
     for (name, size, dtype, layout), t in zip(ctx.kinds, ctx.saved_tensors):
         if t.numel() != size or t.dtype is not dtype or t.device != device or (layout is not None and t.shape != layout[0]):
             raise RuntimeError(f"{what}: a saved-tensor hook returned {name} as {t.dtype} {tuple(t.shape)} on {t.device}, saved were "
@@ -350,11 +339,13 @@ def _kept(ctx, what: str, device, **heads):
         if layout is None:
             t = _aligned(t)
         elif name == "positions":
-            strides["position_stride"] = _position_strides(t)
+            args.position_stride = _position_strides(t)
         elif t.stride() != layout[1] or t.data_ptr() % 16:
-            t, _, _, _, strides[name + "_stride"] = _head_rows(t, heads[name], f"{what}: {name}")
+            t, _, _, _, st = _head_rows(t, heads[name], f"{what}: {name}")
+            setattr(args, name + "_stride", st)
         kept[name] = t
-    return kept, strides
+        setattr(args, name, t.data_ptr())
+    return kept, args
 
 
 def _position_strides(positions):
@@ -404,7 +395,7 @@ class _QkNormRotary(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dyq, dyk):
         qs, ks, dtype, dev = ctx.meta
-        kept, strides = _kept(ctx, "qk_norm_rotary", dev, q=ctx.args.heads, k=ctx.args.kv_heads)
+        kept, args = _kept(ctx, "qk_norm_rotary", dev, q=ctx.args.heads, k=ctx.args.kv_heads)
         _no_tangents("qk_norm_rotary", dyq, dyk)
         dyq, dyk = _aligned(dyq), _aligned(dyk)
         dq, dk = torch.empty(qs, dtype=dtype, device=dev), torch.empty(ks, dtype=dtype, device=dev)
@@ -412,12 +403,11 @@ class _QkNormRotary(torch.autograd.Function):
         make = torch.empty_like if dq.numel() else torch.zeros_like
         dqw, dkw = make(kept["q_weight"]) if need_qw else None, make(kept["k_weight"]) if need_kw else None
         if dq.numel():
-            scratch = None
             if need_qw or need_kw:
                 scratch = torch.empty(_buffer_size("mivae_qk_norm_rotary_scratch_floats", ctx.args.head_size),
                                       dtype=torch.float32, device=dev)
-            args = _refill(ctx.args, strides, dq_out=dyq, dk_out=dyk, q_out=dq, k_out=dk, dq_weight=dqw, dk_weight=dkw,
-                           scratch=scratch, **kept)
+                args.scratch, args.dq_weight, args.dk_weight = scratch.data_ptr(), L.ptr(dqw), L.ptr(dkw)
+            args.dq_out, args.dk_out, args.q_out, args.k_out = dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(), dk.data_ptr()
             with L.on_device(dev):
                 L.call("mivae_qk_norm_rotary_bwd", ctypes.byref(args), L.stream_of(dev))
         return dq, dk, dqw, dkw, None, None
@@ -540,8 +530,8 @@ class _BiasedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        a = ctx.args
-        kept, strides = _kept(ctx, "biased_attention", ctx.device, q=a.heads, k=a.kv_heads, v=a.kv_heads)
+        heads, kv_heads = ctx.args.heads, ctx.args.kv_heads
+        kept, a = _kept(ctx, "biased_attention", ctx.device, q=heads, k=kv_heads, v=kv_heads)
         q, k = kept["q"], kept["k"]
         dev, dtype = q.device, q.dtype
         _no_tangents("biased_attention", dout)
@@ -555,9 +545,9 @@ class _BiasedAttention(torch.autograd.Function):
         scratch = torch.empty(_buffer_size("mivae_biased_attention_bwd_floats", a.batch, a.q_len, a.k_len, a.heads,
                                            a.kv_heads, a.head_size, a.num_buckets if need_t else 0),
                               dtype=torch.float32, device=dev)
-        args = _refill(a, strides, dout=dout, dq=dq, dk=dk, dv=dv, dtable=dtable, scratch=scratch, **kept)
+        a.dout, a.dq, a.dk, a.dv, a.dtable, a.scratch = dout.data_ptr(), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(dtable), scratch.data_ptr()
         with L.on_device(dev), _timed("biased_attention_bwd"):
-            L.call("mivae_biased_attention_bwd", ctypes.byref(args), L.stream_of(dev))
+            L.call("mivae_biased_attention_bwd", ctypes.byref(a), L.stream_of(dev))
         return dq, dk if need_k else None, dv if need_v else None, dtable, None, None
 
 
