@@ -282,7 +282,8 @@ __device__ __forceinline__ Score score_of(const BiasedArgs& a, int head) {
 //   kCapTile:  a tile whose |y| are all small leaves the transcendental instructions out (4 x 16 x 4096 documents, bf16: dq 139 us,
 //              dk and dv 187; with a larger one in every tile 162 and 207)
 //   kCapAhead: as kCapTile with the polynomial before that branch, where it overlaps the products (bf16 training forward: 115
-//              instead of 130 us at the same size, 126 with a larger one in every tile; in dq and dk / dv it makes no difference there and costs registers)
+//              instead of 130 us at the same size, 126 with a larger one in every tile; in dq and dk / dv it
+//              makes no difference and costs registers)
 enum Cap { kCapRough, kCapTile, kCapAhead };
 constexpr float kRoughCap = 512.f;
 __device__ __forceinline__ float tanh_near(float y) {

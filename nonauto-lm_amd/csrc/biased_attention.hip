@@ -12,13 +12,20 @@
 //   dk / dv:      a wave owns 32 keys, S = Q K^T, then dV^T = dO^T P, dK^T = Q^T dS
 // The backward recomputes the scores in both kernels (7 products, not 5): every output is written once, without atomics.
 // Softmax statistics, sums and all score arithmetic are fp32; P and dS are rounded to the operands' type for the second
-// products, which is what lets them run on the bf16 matrix instruction.
+// products, which is what lets them run on the bf16 matrix instruction.  That is one rounding more than the result's own: errors
+// relative to the norm 2.3e-3 (outputs without gradients, or with the table's) and 2.35e-3 (gradients) where the result's alone
+// leaves 1.66e-3.  Second bf16 values for what they leave reach 1.66e-3 everywhere and were measured: for P in the forward
+// 535 us instead of 470 (8191 queries of 128), for P and dS in all products 460 instead of 420 (documents), 549 instead of 439
+// (64 x 512, table), 1482 instead of 1220 (4 x 4096, table).  They are kept where the error grows or stays for good: P where few
+// keys carry a row (k_ba_fwd), the output for delta (out_lo), delta of the table's gradient (kDelta), dS of up to 16 columns.
 //
-// Bound: bf16 by the VALU (a score costs an exponential, with a cap a tanh, and two conversions), fp32 by its matrix instructions.
-//   8191 causal queries of 16 + 4 heads of 128 with a cap, no gradient: 472 us, 583 TFLOP/s; the VALU issues in 76 % of the cycles
-//   4 x 4096, 16 + 4 heads of 64, causal, a table and its gradient: forward 265 us, delta 195, dq 390, dk and dv 480
-//   4 x 4096 in documents of 600, 16 heads of 64, a cap: forward 113 us, dq 136, dk and dv 185
-//   4 x 1001, 8 + 2 heads of 80, fp32, a prefix and slopes: forward 115 us, dq 143, dk and dv 193, joining the parts 29
+// Bound: fp32 by its matrix instructions (55 - 64 % busy), the bf16 forward by the VALU (a score costs an exponential, with a cap
+// a tanh, and two conversions: issued in 75 - 84 % of the cycles of long walks).  The bf16 backward fills neither (long walks: dq VALU
+// 59 - 62 %, dk and dv 45 - 48 %, matrix cores 11 - 26 %): at 177 - 256 registers two waves share a SIMD and wait together.
+//   8191 causal queries of 16 + 4 heads of 128 with a cap, no gradient: 470 us, 585 TFLOP/s
+//   4 x 4096, 16 + 4 heads of 64, causal, a table and its gradient: forward 212 us, delta 202, dq 354, dk and dv 440
+//   4 x 4096 in documents of 600, 16 heads of 64, a cap: forward 106 us, dq 129, dk and dv 174
+//   4 x 1001, 8 + 2 heads of 80, fp32, a prefix and slopes: forward 109 us, dq 134, dk and dv 183, joining the parts 29
 #include <type_traits>
 
 #include "att_tiles.hpp"
@@ -975,7 +982,10 @@ __global__ __launch_bounds__(256) void k_ba_fold(const float* part, T* out0, T* 
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
-// Few queries take the split form.
+// Few queries take the split form, which packs (position, head of the group) into tiles of 32 rows.  8 rows of 32 + 8 heads of 128
+// over 8192 keys, bf16: 51 us instead of 172 for one query, 93 instead of 176 for 16; 157 against 177 for 17, 164 against 181 for
+// 32, and 300 against 210 for 64, whose 8 tiles a key head read the keys 8 times.  4 rows of 8 + 2 heads of 80 over 2000
+// keys, fp32: 19 instead of 43 for 16.
 bool few_queries(int64_t Sq) { return Sq <= 16; }
 
 // Parts of a walk that blocks of their own take: until the chip's 1024 SIMDs have two waves each to choose from, and of two
@@ -994,7 +1004,8 @@ int key_slices(int64_t B, int64_t heads, int64_t Sq, int64_t Sk) {
 struct Pieces {
   int split, cuts;
 };
-// dk and dv: heads of a group first, until there are four blocks per CU, then their queries
+// dk and dv: heads of a group first, until there are four blocks per CU, then their queries.  (4 x 4096, 16 + 4 heads of 64, training:
+// 1224 us; 1495 with two blocks per CU, 1237 with eight)
 Pieces query_pieces(int64_t B, int64_t Sq, int64_t Sk, int64_t kv, int64_t group) {
   const int64_t blocks = B * kv * ((Sk + kRows - 1) / kRows);
   Pieces p = {1, 1};

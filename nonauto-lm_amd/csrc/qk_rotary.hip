@@ -4,7 +4,7 @@
 //   dn = R(-t) dy;  dw = sum over rows of dn x r;  dx = r (dn w - x r mean_d(dn w x r))
 //
 // Bound by HBM: reads x and writes y once (backward: reads x and dy, writes dx).  (2 x 8191 tokens, 16 + 4 heads of 96, fp32,
-// half rotated: 53 us and 76 us, 4.8 and 5.0 TB/s; 64 x 512, 4 + 4 heads of 128, bf16: 34 and 60 us, 4.0 and 3.4 TB/s, where
+// half rotated: 55 us and 76 us, 4.7 and 5.0 TB/s; 64 x 512, 4 + 4 heads of 128, bf16: 32 and 59 us, 4.2 and 3.4 TB/s, where
 // the VALU issues in 78 % and 65 % of the cycles.)  A lane holds one or more chunks of VEC
 // pairs of a head row, so the two halves of a pair meet in its registers whatever the pairing, and a row is a power of two
 // of neighbouring lanes.  The angles of a token are shared by all its heads: a block takes a few whole tokens and puts
@@ -289,7 +289,10 @@ __global__ __launch_bounds__(1024) void k_qk_dw(const float* part, float* dqw, f
   if (g == 0 && e < 2 * d && dst) dst[e < d ? e : e - d] = red[0][c];
 }
 
-constexpr int kMaxBlocks = 1024;        // four per CU; the backward leaves a row of partials for each
+// Four blocks per CU; the backward leaves a row of partials for each.  Forward, backward, fold: 32 + 60 + 7 us at 64 x 512 tokens, 4 + 4
+// heads of 128, bf16, and 59 + 79 + 7 at 2 x 8191, 16 + 4 heads of 96, fp32.  With two per CU 38 + 56 + 4 and 86 + 110 + 4, with
+// eight 35 + 59 + 12 and 59 + 80 + 12.
+constexpr int kMaxBlocks = 1024;
 
 struct Geometry {
   bool vec;
@@ -306,7 +309,9 @@ Geometry geometry(const mivae_rotary_args* x) {
   const int64_t chunks = (half + rest) / (g.vec ? V : 1);
   g.lpr = 1;
   while (g.lpr < chunks && g.lpr < 64) g.lpr <<= 1;
-  // whole tokens per block: enough rows for two turns of its lanes, while there are blocks for every CU
+  // Whole tokens at a time: enough rows for two turns of a block's lanes, up to 16 tokens (64 x 512 tokens with 1 + 1 heads of 32, bf16:
+  // 11 + 22 us forward and backward, 14 + 29 with 8, 21 + 43 with 4), while there are two blocks for every CU (8 x 1024 tokens, 1 + 1
+  // heads of 16: 5 + 11 us, 8 + 21 if eight are asked for; half a block per CU: no difference)
   const int64_t HG = x->heads + x->kv_heads, tokens = x->batch * x->len, slots = kThreads / g.lpr;
   int64_t tpb = (2 * slots + HG - 1) / HG;
   if (tpb > 16) tpb = 16;

@@ -1,5 +1,6 @@
 // The biased attention (biased_attention.hip) for a few new queries over long keys: bound by reading the keys and values once
-// (one query for each of 32 rows of up to 8192 keys, 8 key heads of 128, bf16: 161 us, 5.0 TB/s, as fast as a large copy).
+// (one query for each of 32 rows of up to 8192 keys, 8 key heads of 128, bf16: 160 to 168 us by card, 4.8 to 5.0 TB/s, as
+// fast as a large copy).
 //
 // The queries of a batch row that share a key head, (position, head of the group), are packed into tiles of up to 32 rows, so
 // that one read of the keys serves all of them.  The keys are split over blocks and, inside a block, over two waves that
