@@ -578,7 +578,9 @@ def biased_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     of a cache), may hold anything, and so may queries that see no key and their gradients; all other operands have to be
     finite, also where `causal` or documents hide them from some queries.  A table entry of -inf or of fp32's or
     bf16's lowest value hides its pairs; a query whose pairs the table hides one and all gives zeros too, but has to be finite,
-    as its gradient has.  Gradients in reverse mode, once; operands with forward-mode tangents are refused."""
+    as its gradient has.  Gradients in reverse mode, once; operands with forward-mode tangents are refused.  A backward pass that
+    is captured into a graph needs leaves without a live eager graph (torch accumulates their gradients on the stream of that
+    graph): leaves of the captured pass's own, `t.detach().requires_grad_()`, and torch.autograd.grad."""
     kv_heads = heads if kv_heads is None else kv_heads
     L.require_gpu(q, k, v, mask, prefix, documents, slopes, table, buckets)
     _no_tangents("biased_attention", q, k, v, slopes, table)

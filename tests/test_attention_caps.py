@@ -30,6 +30,18 @@ def test_caps_far_above_the_scores(Sq, Sk, cap, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("cap", [100.0, 512.0, 513.0])
+@pytest.mark.parametrize("Sq", [1, 9, 60, 150])
+def test_both_sides_of_the_short_form(Sq, cap):
+    """bf16 without gradients: the largest cap whose tanh takes two instructions, and the smallest beyond"""
+    from nonauto_lm_amd import ops
+    _, q, k, v, _ = inputs(2, Sq, 200, 4, 2, 64, torch.bfloat16, seed=Sq, grad=False)
+    for loud in (2, 200):                                      # scores far below the cap and around it
+        out = ops.biased_attention(q * loud, k, v, 4, 2, softcap=cap, causal=True)
+        check("out", out, *definition(q * loud, k, v, 4, 2, softcap=cap, causal=True)["out"])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("Sq", [2, 16, 33, 150])
 def test_scores_next_to_ones_near_the_cap(Sq, dtype):
